@@ -316,6 +316,45 @@ int rsllm_hip_moe_routed(float *out, size_t out_len, const float *x, size_t x_le
                          size_t n_ff, size_t n_expert, size_t k, uint32_t dtype_gate_up,
                          uint32_t dtype_down, float clamp);
 
+/* ---- expert routing ---------------------------------------------------------
+ * No single reference function: the router's product is matmul_weight_f32,
+ * and what follows it, the ids and weights rsllm_hip_moe_routed takes, is made
+ * here. logits: n_tok rows of n_expert values of `dtype` (F32, F16 or BF16),
+ * logits_stride elements apart. Per token, in 64 bits:
+ *   s_e   = softmax(l)_e | 1 / (1 + exp(-l_e)) | sqrt(log(1 + exp(l_e)))
+ *   key_e = s_e + bias_e     (bias: n_expert values that balance the load and
+ *                             take part in the choice alone, or NULL)
+ * With n_group > 1, group g holds experts [g n_expert / n_group, ...), counts
+ * the sum of its group_top (1 or 2) largest keys (of the experts that can be
+ * chosen; the one key where there is only one), and the topk_group groups that
+ * count most stay. Of the experts left the k with the largest keys are
+ * chosen: ids[t * k + i] in falling order of key, equal keys in rising order of
+ * id (groups likewise); without a bias the logits themselves are compared, which
+ * is the same order. weights[t * k + i] = scale * s_e, divided by the sum of the
+ * chosen experts' s when `renormalise` is nonzero (0 if that sum is 0), rounded
+ * once to f32.
+ * An expert whose logit or key is NaN or -inf is never chosen (a group without
+ * any other neither); places that stay empty get id -1 and weight 0, which
+ * rsllm_hip_moe_routed_dev skips. A +inf logit counts as the softmax's limit:
+ * the +inf experts share it evenly.
+ * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for an unknown
+ * score, n_expert 0 or above 16384, n_group 0, above 1024 or no divisor of
+ * n_expert, topk_group 0 or above n_group, group_top other than 1 and 2, k 0 or
+ * above min(64, topk_group * n_expert / n_group), a scale that is not finite,
+ * NULL pointers or logits not aligned to their elements; SHAPE_MISMATCH for
+ * logits_stride < n_expert, logits_len < (n_tok - 1) * logits_stride + n_expert,
+ * bias_len other than 0 and n_expert, ids_len != n_tok * k. Enqueued on
+ * `stream`; no workspace. */
+enum {
+    RSLLM_HIP_SCORE_SOFTMAX = 0, RSLLM_HIP_SCORE_SIGMOID = 1, RSLLM_HIP_SCORE_SQRT_SOFTPLUS = 2
+};
+int rsllm_hip_moe_route_dev(int32_t *ids, float *weights, size_t ids_len, const void *logits,
+                            size_t logits_len, size_t logits_stride, const float *bias,
+                            size_t bias_len, size_t n_tok, size_t n_expert, size_t k,
+                            size_t n_group, size_t topk_group, size_t group_top, uint32_t score,
+                            int renormalise, float scale, uint32_t dtype,
+                            rsllm_hip_stream_t stream);
+
 /* ---- caller chain: matmul_weight_f32, matmul_grouped_lora_down ------------
  * rsllm_hip_matmul_weight_f32 replaces matmul_weight_f32
  * (rsllm-models/src/dsv4/weight.rs:113-169): out[t, o] = sum_i W[o, i] x[t, i]
@@ -450,6 +489,92 @@ int rsllm_hip_matmul_q8_0_batch_dev(float *out, size_t out_len, const uint8_t *w
                                     size_t weights_len, const int8_t *xq, size_t xq_len,
                                     const float *xscale, size_t xscale_len, size_t n_tok,
                                     size_t in_dim, size_t out_dim, rsllm_hip_stream_t stream);
+
+/* ---- int8 product with a scale per token and per channel ---------------------
+ * No reference counterpart (its int8 path scales blocks of 32): for weights
+ * quantised to int8 with one scale per output row.
+ *   d_t       = f32(max_i |x[t, i]| / 127)
+ *   q[t, i]   = x[t, i] / d_t to the nearest integer, halves to even (of the
+ *               exact quotient; within +-127; 0 where d_t is 0)
+ *   out[t, o] = (f32(sum_i q[t, i] w[o, i]) * d_t) * wscale[o] + bias[o]
+ * the sum exact in 32-bit integers. A token with a non-finite value gets d_t =
+ * NaN and q = 0, so its outputs are NaN and no other token's are touched.
+ * Rows of int8 codes (weights, xq) lie rsllm_hip_int8_row_bytes(in_dim) =
+ * in_dim rounded up to 64 bytes apart, 16-byte aligned. The quantiser fills the
+ * rest of a row with zeros; what a weight row holds there does not matter. It
+ * quantises weight rows as well as tokens (n_tok = out_dim).
+ * x: n_tok rows of in_dim values of `dtype` / `dtype_x` (F32, F16 or BF16),
+ * x_stride elements apart; out: rows of out_dim values of dtype_out (F32, F16 or
+ * BF16; rounded once from f32), out_stride elements apart, what lies between
+ * rows left as it was. bias: out_dim values or NULL.
+ * rsllm_hip_matmul_int8_dev takes x; _quantize_int8_dev and
+ * _matmul_int8_prequant_dev are its halves, for one x through several matrices:
+ * the same results, bit for bit. `work`: rsllm_hip_int8_work_bytes(n_tok,
+ * in_dim, out_dim) bytes of the caller's (it never falls as n_tok grows),
+ * 256-byte aligned, used by this call alone until it has run: calls that may
+ * overlap, and graphs that may replay at once, get one each.
+ * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for in_dim 0 or
+ * above 131071 (where the sum could leave 32 bits), out_dim 0, NULL or
+ * misaligned pointers; SHAPE_MISMATCH for a stride below its row, x_len or
+ * out_len below (n_tok - 1) * stride + row, weights_len != out_dim * row bytes,
+ * wscale_len != out_dim, bias_len other than 0 and out_dim, xq_len != n_tok *
+ * row bytes, scale_len or xscale_len != n_tok, work_len below work_bytes. */
+size_t rsllm_hip_int8_row_bytes(size_t in_dim);
+size_t rsllm_hip_int8_work_bytes(size_t n_tok, size_t in_dim, size_t out_dim);
+int rsllm_hip_quantize_int8_dev(const void *x, size_t x_len, size_t x_stride, int8_t *xq,
+                                size_t xq_len, float *scale, size_t scale_len, size_t n_tok,
+                                size_t in_dim, uint32_t dtype, rsllm_hip_stream_t stream);
+int rsllm_hip_matmul_int8_prequant_dev(void *out, size_t out_len, size_t out_stride,
+                                       const int8_t *weights, size_t weights_len,
+                                       const float *wscale, size_t wscale_len, const float *bias,
+                                       size_t bias_len, const int8_t *xq, size_t xq_len,
+                                       const float *xscale, size_t xscale_len, uint8_t *work,
+                                       size_t work_len, size_t n_tok, size_t in_dim,
+                                       size_t out_dim, uint32_t dtype_out,
+                                       rsllm_hip_stream_t stream);
+int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, const int8_t *weights,
+                              size_t weights_len, const float *wscale, size_t wscale_len,
+                              const float *bias, size_t bias_len, const void *x, size_t x_len,
+                              size_t x_stride, uint8_t *work, size_t work_len, size_t n_tok,
+                              size_t in_dim, size_t out_dim, uint32_t dtype_x, uint32_t dtype_out,
+                              rsllm_hip_stream_t stream);
+
+/* ---- token log-probabilities --------------------------------------------------
+ * No reference counterpart among its compute ops: what a caller reads from the
+ * vocabulary projection's product (matmul_weight_f32 or one of the others)
+ * beside the token it samples. logits: n_tok rows of `vocab` values of `dtype`
+ * (F32, F16 or BF16), logits_stride elements apart. Per row, with m = max l,
+ * S = sum exp(l - m), p = exp(l - m) / S:
+ *   logprob  = l[token] - m - log S      tokens[t] the given token's id
+ *   rank     = 1 + the number of logits above the given token's
+ *   entropy  = -sum p log p (natural log)
+ *   top_ids, top_logprobs [n_tok x n_top]: the n_top largest logits, in falling
+ *              order, equal ones in rising order of id, and their log-
+ *              probabilities
+ * A logit of -inf (a masked token) has probability 0, adds nothing to the
+ * entropy and is never listed; places that stay empty get id -1 and -inf. A row
+ * of nothing but -inf: logprob -inf, entropy 0. +inf counts as the limit: the
+ * +inf logits share the row evenly. A NaN anywhere in a row makes its logprob,
+ * entropy and listed log-probabilities NaN (a NaN logit is not listed or counted).
+ * A token id outside [0, vocab) gives logprob NaN and rank 0, a token whose
+ * logit is NaN rank 0.
+ * tokens (with tokens_len 0) may be NULL: logprob and rank are then not written
+ * and may be NULL; rank and entropy may be NULL; n_top 0 takes NULL lists.
+ * out_len counts logprob, rank and entropy each. `work`:
+ * rsllm_hip_token_logprobs_work_bytes(n_tok, vocab, n_top) bytes of the
+ * caller's, 256-byte aligned, used by this call alone until it has run.
+ * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for vocab 0 or above
+ * 2^31 - 1, n_top above min(64, vocab), NULL or misaligned pointers;
+ * SHAPE_MISMATCH for logits_stride < vocab, logits_len < (n_tok - 1) *
+ * logits_stride + vocab, tokens_len other than 0 and n_tok, out_len != n_tok,
+ * top_len != n_tok * n_top, work_len below work_bytes. */
+size_t rsllm_hip_token_logprobs_work_bytes(size_t n_tok, size_t vocab, size_t n_top);
+int rsllm_hip_token_logprobs_dev(float *logprob, float *entropy, int32_t *rank, size_t out_len,
+                                 int32_t *top_ids, float *top_logprobs, size_t top_len,
+                                 const void *logits, size_t logits_len, size_t logits_stride,
+                                 const int32_t *tokens, size_t tokens_len, uint8_t *work,
+                                 size_t work_len, size_t n_tok, size_t vocab, size_t n_top,
+                                 uint32_t dtype, rsllm_hip_stream_t stream);
 
 /* ---- dequantisation ------------------------------------------------------ */
 

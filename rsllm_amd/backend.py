@@ -172,6 +172,18 @@ SIGNATURES = {
                                        _S, _S, _S, ctypes.c_float], _I),
     "rsllm_hip_apply_shared_expert_dev": ([_P, _S, _P, _S, _P, _S, _U32, _P, _S, _U32, _P, _S,
                                            _U32, _S, _S, _S, ctypes.c_float, _P], _I),
+    "rsllm_hip_moe_route_dev": ([_P, _P, _S, _P, _S, _S, _P, _S, _S, _S, _S, _S, _S, _S, _U32, _I,
+                                 ctypes.c_float, _U32, _P], _I),
+    "rsllm_hip_int8_row_bytes": ([_S], _S),
+    "rsllm_hip_int8_work_bytes": ([_S, _S, _S], _S),
+    "rsllm_hip_quantize_int8_dev": ([_P, _S, _S, _P, _S, _P, _S, _S, _S, _U32, _P], _I),
+    "rsllm_hip_matmul_int8_prequant_dev": ([_P, _S, _S, _P, _S, _P, _S, _P, _S, _P, _S, _P, _S, _P,
+                                            _S, _S, _S, _S, _U32, _P], _I),
+    "rsllm_hip_matmul_int8_dev": ([_P, _S, _S, _P, _S, _P, _S, _P, _S, _P, _S, _S, _P, _S, _S, _S,
+                                   _S, _U32, _U32, _P], _I),
+    "rsllm_hip_token_logprobs_work_bytes": ([_S, _S, _S], _S),
+    "rsllm_hip_token_logprobs_dev": ([_P, _P, _P, _S, _P, _P, _S, _P, _S, _S, _P, _S, _P, _S, _S,
+                                      _S, _S, _U32, _P], _I),
     "rsllm_hip_stream_read_dev": ([_P, _S, _P, _S, _I, _I, _I, _I, _P], _I),
     "rsllm_hip_mfma_issue_dev": ([_P, _S, _I, _I, _I, _I, _P], _I),
 }
@@ -525,6 +537,96 @@ def matmul_q8_0_batch_dev(out_ptr: int, out_len: int, w_ptr: int, w_len: int, xq
                                                stream or None))
 
 
+class RouteScore(enum.IntEnum):
+    """How moe_route_dev turns a router logit into a score."""
+
+    Softmax = 0
+    Sigmoid = 1
+    SqrtSoftplus = 2
+
+
+def moe_route_dev(ids_ptr: int, weights_ptr: int, ids_len: int, logits_ptr: int, logits_len: int,
+                  logits_stride: int, bias_ptr: int, bias_len: int, n_tok: int, n_expert: int,
+                  k: int, n_group: int = 1, topk_group: int = 1, group_top: int = 1,
+                  score=RouteScore.Softmax, renormalise: bool = True, scale: float = 1.0,
+                  dtype=GgmlType.F32, stream: int = 0) -> None:
+    """Router logits -> the ids (int32) and weights (f32) moe_routed_dev takes:
+    score, balancing bias, groups, the k best, weights renormalised over them."""
+    _check(LIB.rsllm_hip_moe_route_dev(ids_ptr or None, weights_ptr or None, ids_len,
+                                       logits_ptr or None, logits_len, logits_stride,
+                                       bias_ptr or None, bias_len, n_tok, n_expert, k, n_group,
+                                       topk_group, group_top, int(score), int(bool(renormalise)),
+                                       scale, int(dtype), stream or None))
+
+
+def int8_row_bytes(in_dim: int) -> int:
+    """Bytes from one row of int8 codes to the next (in_dim rounded up to 64)."""
+    return LIB.rsllm_hip_int8_row_bytes(in_dim)
+
+
+def int8_work_bytes(n_tok: int, in_dim: int, out_dim: int) -> int:
+    """Workspace of matmul_int8_dev and matmul_int8_prequant_dev."""
+    return LIB.rsllm_hip_int8_work_bytes(n_tok, in_dim, out_dim)
+
+
+def quantize_int8_dev(x_ptr: int, x_len: int, x_stride: int, xq_ptr: int, xq_len: int,
+                      scale_ptr: int, scale_len: int, n_tok: int, in_dim: int,
+                      dtype=GgmlType.F32, stream: int = 0) -> None:
+    """Rows of floats (tokens, or weight channels) -> int8 codes and one f32
+    scale per row."""
+    _check(LIB.rsllm_hip_quantize_int8_dev(x_ptr or None, x_len, x_stride, xq_ptr or None, xq_len,
+                                           scale_ptr or None, scale_len, n_tok, in_dim, int(dtype),
+                                           stream or None))
+
+
+def matmul_int8_prequant_dev(out_ptr: int, out_len: int, out_stride: int, w_ptr: int, w_len: int,
+                             wscale_ptr: int, wscale_len: int, bias_ptr: int, bias_len: int,
+                             xq_ptr: int, xq_len: int, xscale_ptr: int, xscale_len: int,
+                             work_ptr: int, work_len: int, n_tok: int, in_dim: int, out_dim: int,
+                             dtype_out=GgmlType.F32, stream: int = 0) -> None:
+    """matmul_int8_dev on the codes quantize_int8_dev made."""
+    _check(LIB.rsllm_hip_matmul_int8_prequant_dev(out_ptr or None, out_len, out_stride,
+                                                  w_ptr or None, w_len, wscale_ptr or None,
+                                                  wscale_len, bias_ptr or None, bias_len,
+                                                  xq_ptr or None, xq_len, xscale_ptr or None,
+                                                  xscale_len, work_ptr or None, work_len, n_tok,
+                                                  in_dim, out_dim, int(dtype_out), stream or None))
+
+
+def matmul_int8_dev(out_ptr: int, out_len: int, out_stride: int, w_ptr: int, w_len: int,
+                    wscale_ptr: int, wscale_len: int, bias_ptr: int, bias_len: int, x_ptr: int,
+                    x_len: int, x_stride: int, work_ptr: int, work_len: int, n_tok: int,
+                    in_dim: int, out_dim: int, dtype_x=GgmlType.F32, dtype_out=GgmlType.F32,
+                    stream: int = 0) -> None:
+    """x quantised to int8 with a scale per token, times int8 weights with a scale
+    per channel (and a bias): out rows of dtype_out."""
+    _check(LIB.rsllm_hip_matmul_int8_dev(out_ptr or None, out_len, out_stride, w_ptr or None, w_len,
+                                         wscale_ptr or None, wscale_len, bias_ptr or None, bias_len,
+                                         x_ptr or None, x_len, x_stride, work_ptr or None, work_len,
+                                         n_tok, in_dim, out_dim, int(dtype_x), int(dtype_out),
+                                         stream or None))
+
+
+def token_logprobs_work_bytes(n_tok: int, vocab: int, n_top: int) -> int:
+    """Workspace of token_logprobs_dev."""
+    return LIB.rsllm_hip_token_logprobs_work_bytes(n_tok, vocab, n_top)
+
+
+def token_logprobs_dev(logprob_ptr: int, entropy_ptr: int, rank_ptr: int, out_len: int,
+                       top_ids_ptr: int, top_ptr: int, top_len: int, logits_ptr: int,
+                       logits_len: int, logits_stride: int, tokens_ptr: int, tokens_len: int,
+                       work_ptr: int, work_len: int, n_tok: int, vocab: int, n_top: int,
+                       dtype=GgmlType.F32, stream: int = 0) -> None:
+    """Log-probability and rank of each row's given token, the row's entropy, and
+    its n_top most likely tokens with their log-probabilities."""
+    _check(LIB.rsllm_hip_token_logprobs_dev(logprob_ptr or None, entropy_ptr or None,
+                                            rank_ptr or None, out_len, top_ids_ptr or None,
+                                            top_ptr or None, top_len, logits_ptr or None,
+                                            logits_len, logits_stride, tokens_ptr or None,
+                                            tokens_len, work_ptr or None, work_len, n_tok, vocab,
+                                            n_top, int(dtype), stream or None))
+
+
 def prepare_weights_dev(dst_ptr: int, src_ptr: int, nbytes: int, dtype, in_dim: int,
                         stream: int = 0) -> None:
     _check(LIB.rsllm_hip_prepare_weights_dev(dst_ptr or None, src_ptr or None, nbytes, int(dtype),
@@ -592,5 +694,7 @@ __all__ = [
     "dequant_to_f32_dev", "xq_bytes", "quantize_x_dev", "matmul_prequant_dev",
     "matmul_q4k_bf16_dev", "moe_routed", "moe_routed_dev", "quantize_q8_0_batch",
     "matmul_q8_0_batch", "quantize_q8_0_batch_dev", "matmul_q8_0_batch_dev", "HipBackend",
-    "BackendCapability", "LIB", "LIB_PATH", "SIGNATURES",
+    "RouteScore", "moe_route_dev", "int8_row_bytes", "int8_work_bytes", "quantize_int8_dev",
+    "matmul_int8_dev", "matmul_int8_prequant_dev", "token_logprobs_work_bytes",
+    "token_logprobs_dev", "BackendCapability", "LIB", "LIB_PATH", "SIGNATURES",
 ]

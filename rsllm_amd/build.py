@@ -25,7 +25,8 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librsllm_hip.so")
 
 SOURCES = ["abi.hip", "dequant.hip", "gemv.hip", "gemv_mfma.hip", "gemm_exact.hip", "moe_gemm.hip",
-           "prefill.hip", "moe.hip", "q8_int8.hip", "residency.hip", "probe.hip"]
+           "prefill.hip", "moe.hip", "q8_int8.hip", "residency.hip", "probe.hip",
+           "abi_serving.hip", "route.hip", "int8.hip", "logprobs.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

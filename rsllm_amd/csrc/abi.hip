@@ -774,6 +774,10 @@ int set_error(int status, const char *msg) { return set_err(status, msg); }
 int ok_status() { return ok(); }
 int device_error(hipError_t e, const char *where) { return dev_err(e, where); }
 int ensure_current_device() { return ensure_device(); }
+int make_device_current() {
+    int dev;
+    return current_device_noalloc(&dev);
+}
 void registry_add(const uint8_t *host, size_t len, uint32_t dtype, size_t in_dim, uint8_t *dev,
                   uint64_t owner, std::shared_ptr<void> keep) {
     std::lock_guard<std::mutex> lk(g_mu);

@@ -37,6 +37,9 @@ int device_error(hipError_t e, const char *where);
 // Make the process's device current on this thread (and create the thread's
 // stream); returns a status.
 int ensure_current_device();
+// The process's device made current on this thread, nothing created or
+// allocated (so also while a stream is being captured); returns a status.
+int make_device_current();
 // Host tensor (host, len, dtype, in_dim) -> device copy at dev, owned by the
 // uploaded model `owner` (never 0), inside the allocation `keep` holds alive.
 // Host-pointer entry points find it.

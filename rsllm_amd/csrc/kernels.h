@@ -264,6 +264,57 @@ hipError_t launch_q8_int8_matmul(const uint8_t *w, size_t w_bytes, const int8_t 
                                  const float *xscale, float *out, int n_tok, int in_dim,
                                  int out_dim, hipStream_t s);
 
+// route.hip: expert routing of n_tok rows of router logits (dtype F32, F16 or
+// BF16, `stride` elements apart) into ids and weights [n_tok x k]; k <= 64.
+enum { ROUTE_SOFTMAX = 0, ROUTE_SIGMOID = 1, ROUTE_SQRT_SOFTPLUS = 2 };
+struct RouteArgs {
+    const void *logits;
+    size_t stride;
+    const float *bias;  // or null
+    int *ids;
+    float *weights;
+    int n_expert, k, n_group, topk_group, group_top, score, renormalise;
+    float scale;
+    uint32_t dtype;
+};
+hipError_t launch_moe_route(const RouteArgs &a, int n_tok, hipStream_t s);
+
+// int8.hip: rows of floats (dtype F32, F16 or BF16, `stride` elements apart) to
+// int8 codes, i8_row_bytes(in_dim) apart and zero behind in_dim, and a scale a
+// row; and the product of two such code matrices with the scales applied.
+inline size_t i8_row_bytes(size_t in_dim) { return (in_dim + 63) / 64 * 64; }
+hipError_t launch_i8_quantize(const void *x, size_t stride, int8_t *xq, float *scale, int n_tok,
+                              int in_dim, uint32_t dtype, hipStream_t s);
+struct I8Args {
+    const int8_t *w;   // out_dim rows of row_bytes
+    const int8_t *xq;  // n_tok rows of row_bytes, zero behind in_dim
+    const float *wscale, *xscale, *bias;  // bias or null
+    void *out;         // rows of dtype_out, out_stride elements apart
+    size_t out_stride;
+    int n_tok, out_dim, row_bytes;
+    uint32_t dtype_out;
+};
+// `split` holds i8_split_bytes(n_tok, in_dim, out_dim) bytes.
+size_t i8_split_bytes(int n_tok, int in_dim, int out_dim);
+hipError_t launch_i8_matmul(const I8Args &a, uint8_t *split, hipStream_t s);
+
+// logprobs.hip: per row of logits (dtype F32, F16 or BF16, `stride` elements
+// apart) what rsllm_hip_token_logprobs_dev gives. tokens may be null (logprob
+// and rank are then not written); rank, entropy may be null. `work` holds
+// logprobs_scratch_bytes(n_tok, vocab, n_top) bytes.
+struct LogprobArgs {
+    const void *logits;
+    size_t stride;
+    const int *tokens;
+    float *logprob, *entropy;
+    int *rank, *top_ids;
+    float *top_logprobs;
+    int vocab, n_top;
+    uint32_t dtype;
+};
+size_t logprobs_scratch_bytes(int n_tok, int vocab, int n_top);
+hipError_t launch_logprobs(const LogprobArgs &a, uint8_t *work, int n_tok, hipStream_t s);
+
 // Largest weight tensor the buffer-addressed kernels accept (offsets are
 // 32-bit).
 constexpr size_t kMaxWeightBytes = 0xFFFFFF00u;
