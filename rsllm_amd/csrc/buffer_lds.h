@@ -38,5 +38,9 @@ __device__ __forceinline__ void bl_dma16(const bl_rsrc &r, uint32_t voff, uint32
 template <int N> __device__ __forceinline__ void bl_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+// The same for a wavefront alone.
+template <int N> __device__ __forceinline__ void bl_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
 
 }  // namespace rsllm_hip

@@ -1,5 +1,8 @@
 // The int8 product with a scale per token and per channel, and its quantiser.
+#include "buffer_lds.h"
 #include "kernels.h"
+
+#include <type_traits>
 
 namespace rsllm_hip {
 
@@ -105,6 +108,314 @@ __global__ __launch_bounds__(256) void k_i8_simple(I8Args a) {
     if (a.bias) y += a.bias[o];
     i8_store(a.out, (size_t)t * a.out_stride + o, y, a.dtype_out);
 }
+
+#ifndef I8_KEY
+#define I8_KEY(row) (((row) >> 1) & 7)
+#endif
+namespace {
+// ---- the product on the matrix cores -------------------------------------------
+
+typedef int i8_v4 __attribute__((ext_vector_type(4)));
+
+// A workgroup's tile: BM = 16 MF WM channels x BN = 16 NF WN tokens, each
+// wavefront 16 MF x 16 NF of it; with WK > 1 the K slices of 128 bytes go round
+// the WK groups of wavefronts, whose whole-number sums are added at the end.
+// Slices of both operands are copied to LDS ST deep.
+template <int WM_, int WN_, int WK_, int MF_, int NF_, int ST_> struct I8Tile {
+    static constexpr int WM = WM_, WN = WN_, WK = WK_, MF = MF_, NF = NF_, ST = ST_;
+    static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * WM * WN * WK;
+    static constexpr int kSlice = (BM + BN) * 128;          // bytes of one slice
+    static constexpr int kCopies = (BM + BN) / 8;           // of 1 KB (8 rows) each
+    static constexpr int D = (kCopies + WM * WN - 1) / (WM * WN);  // a wavefront's
+    static constexpr int kRed = WK > 1 ? WK * WM * WN * MF * NF * 1024 : 0;
+    static constexpr int kRing = WK * ST * kSlice;
+    static constexpr int kLds = kRing > kRed ? kRing : kRed;
+    static_assert(kLds <= 160 * 1024 && D * (ST - 2) <= 63, "tile");
+};
+
+// Four consecutive channels of one token.
+__device__ __forceinline__ void i8_finish(const I8Args &a, const i8_v4 &acc, int o, int t, bool vec) {
+    if (t >= a.n_tok || o >= a.out_dim) return;
+    const float xs = a.xscale[t];
+    const size_t at = (size_t)t * a.out_stride + o;
+    if (vec && o + 3 < a.out_dim) {
+        const float4 ws = *reinterpret_cast<const float4 *>(a.wscale + o);
+        float y[4] = {((float)acc[0] * xs) * ws.x, ((float)acc[1] * xs) * ws.y,
+                      ((float)acc[2] * xs) * ws.z, ((float)acc[3] * xs) * ws.w};
+        if (a.bias) {
+            const float4 b = *reinterpret_cast<const float4 *>(a.bias + o);
+            y[0] += b.x; y[1] += b.y; y[2] += b.z; y[3] += b.w;
+        }
+        if (a.dtype_out == T_F32) {
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) =
+                make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+            uint32_t lo, hi;
+            if (a.dtype_out == T_F16) {
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                lo = __builtin_bit_cast(uint32_t, h2{(_Float16)y[0], (_Float16)y[1]});
+                hi = __builtin_bit_cast(uint32_t, h2{(_Float16)y[2], (_Float16)y[3]});
+            } else {
+                typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+                lo = __builtin_bit_cast(uint32_t, b2{(__bf16)y[0], (__bf16)y[1]});
+                hi = __builtin_bit_cast(uint32_t, b2{(__bf16)y[2], (__bf16)y[3]});
+            }
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(lo, hi);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (o + i >= a.out_dim) return;
+        float y = ((float)acc[i] * xs) * a.wscale[o + i];
+        if (a.bias) y += a.bias[o + i];
+        i8_store(a.out, at + i, y, a.dtype_out);
+    }
+}
+
+template <class G>
+__global__ __launch_bounds__(G::kThreads) void k_i8_tile(I8Args a, int n_ct, int n_tt) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int MF = G::MF, NF = G::NF, ST = G::ST, D = G::D;
+    // Workgroups go round the 8 XCDs: each takes a run of tiles, token tiles
+    // fastest, so the tiles that share a weight row are behind one L2.
+    const int total = n_ct * n_tt, per = (total + 7) / 8;
+    const int L = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || L >= total) return;  // the whole workgroup
+    const int tt = L % n_tt, ct = L / n_tt;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wn = wv % G::WN, wm = wv / G::WN % G::WM, wk = wv / (G::WN * G::WM);
+    const int o0 = ct * G::BM, t0 = tt * G::BN, rb = a.row_bytes;
+
+    const int w_rows = min(G::BM, a.out_dim - o0), x_rows = min(G::BN, a.n_tok - t0);
+    const bl_rsrc rw = bl_make_rsrc(a.w + (size_t)o0 * rb, (uint32_t)w_rows * (uint32_t)rb);
+    const bl_rsrc rx = bl_make_rsrc(a.xq + (size_t)t0 * rb, (uint32_t)x_rows * (uint32_t)rb);
+    // Copy c of a slice: 8 rows of the channels (c < BM / 8) or the tokens;
+    // lane i brings row i / 8, and to place i % 8 of it the 16 bytes that the
+    // operand reads look for there: (i % 8) ^ key(row).
+    const uint32_t lds0 = bl_lds(smem) + (uint32_t)(wk * ST * G::kSlice);
+    const int me = wm * G::WN + wn;  // among the wavefronts of one K group
+    const int steps = ((rb + 127) / 128 + G::WK - 1) / G::WK;
+    auto copy = [&](int i, int buf) {
+        const int k0 = (wk + G::WK * i) * 128;
+#pragma unroll
+        for (int p = 0; p < D; p++) {
+            const int c = min(me + G::WM * G::WN * p, G::kCopies - 1);
+            const bool is_w = c < G::BM / 8;
+            const int row = (is_w ? 8 * c : 8 * c - G::BM) + (lane >> 3);
+            const int k = k0 + 16 * ((lane & 7) ^ I8_KEY(row));
+            // behind the row's end: an offset past any resource, which brings zeros
+            const uint32_t off = k < rb ? (uint32_t)row * (uint32_t)rb + (uint32_t)k : 0xFFFFFFF0u;
+            const uint32_t dst = lds0 + (uint32_t)(buf * G::kSlice + c * 1024);
+            if (is_w) bl_dma16(rw, off, 0, dst);
+            else bl_dma16(rx, off, 0, dst);
+        }
+    };
+    i8_v4 acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[m][n] = i8_v4{0, 0, 0, 0};
+
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint8_t *const lw = smem + wk * ST * G::kSlice + (wm * 16 * MF + r16) * 128;
+    const uint8_t *const lx = smem + wk * ST * G::kSlice + (G::BM + wn * 16 * NF + r16) * 128;
+    const int s0 = 16 * (q ^ I8_KEY(r16)), s1 = 16 * ((4 + q) ^ I8_KEY(r16));
+
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++) copy(i, i);
+    int buf = 0, nbuf = ST - 1;
+    for (int i = 0; i < steps; i++) {
+        // slice i has landed everywhere, and everyone has read slice i - 1
+        if constexpr (G::WM * G::WN * G::WK > G::WK) bl_barrier<D *(ST - 2)>();
+        else bl_wait<D *(ST - 2)>();
+        copy(i + ST - 1, nbuf);
+        const uint8_t *const bw = lw + buf * G::kSlice, *const bx = lx + buf * G::kSlice;
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            const int so = kk ? s1 : s0;
+            i8_v4 fw[MF], fx[NF];
+#pragma unroll
+            for (int n = 0; n < NF; n++) fx[n] = *reinterpret_cast<const i8_v4 *>(bx + n * 2048 + so);
+#pragma unroll
+            for (int m = 0; m < MF; m++) fw[m] = *reinterpret_cast<const i8_v4 *>(bw + m * 2048 + so);
+#pragma unroll
+            for (int m = 0; m < MF; m++)
+#pragma unroll
+                for (int n = 0; n < NF; n++)
+                    acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[m], fx[n], acc[m][n], 0, 0, 0);
+        }
+        buf = buf + 1 == ST ? 0 : buf + 1;
+        nbuf = nbuf + 1 == ST ? 0 : nbuf + 1;
+    }
+    bl_wait<0>();  // (the copies past the last slice, zeros, land in the ring too)
+    const uint32_t esz = a.dtype_out == T_F32 ? 4u : 2u;
+    const bool vec = ((uintptr_t)a.out % (4 * esz)) == 0 && a.out_stride % 4 == 0 &&
+                     ((uintptr_t)a.wscale % 16) == 0 && ((uintptr_t)a.bias % 16) == 0;
+    if constexpr (G::WK == 1) {
+#pragma unroll
+        for (int n = 0; n < NF; n++)
+#pragma unroll
+            for (int m = 0; m < MF; m++)
+                i8_finish(a, acc[m][n], o0 + 16 * (wm * MF + m) + 4 * q, t0 + 16 * (wn * NF + n) + r16, vec);
+    } else {
+        bl_barrier<0>();
+        i8_v4 *red = reinterpret_cast<i8_v4 *>(smem);
+        constexpr int F = G::WM * G::WN * MF * NF;  // 16 x 16 pieces of the tile
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+            for (int n = 0; n < NF; n++)
+                red[(wk * F + (me * MF + m) * NF + n) * 64 + lane] = acc[m][n];
+        __syncthreads();
+        for (int f = wv; f < F; f += G::WM * G::WN * G::WK) {
+            i8_v4 s = red[f * 64 + lane];
+#pragma unroll
+            for (int k = 1; k < G::WK; k++) s += red[(k * F + f) * 64 + lane];
+            const int n = f % NF, m = f / NF % MF, w = f / (NF * MF), fn = w % G::WN, fm = w / G::WN;
+            i8_finish(a, s, o0 + 16 * (fm * MF + m) + 4 * q, t0 + 16 * (fn * NF + n) + r16, vec);
+        }
+    }
+}
+
+template <class G> hipError_t i8_tile_go(const I8Args &a, hipStream_t s) {
+    static const hipError_t attr = hipFuncSetAttribute(
+        reinterpret_cast<const void *>(&k_i8_tile<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+    if (attr != hipSuccess) return attr;
+    const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
+    const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
+    k_i8_tile<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);
+    return hipGetLastError();
+}
+
+// The same product for many tokens: WM x WN wavefronts, two slices in LDS, and
+// the operands of the next half slice read into registers while the matrix
+// cores work on this one. One barrier a slice, in its middle: behind it the
+// next slice has landed, and every wavefront holds what is left of this one in
+// registers, so the slice after the next can be copied over it.
+template <int WM_, int WN_, int MF_, int NF_, int ST_ = 2> struct I8Big {
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, ST = ST_;
+    static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * WM * WN;
+    static constexpr int kSlice = (BM + BN) * 128, kCopies = (BM + BN) / 8;
+    static constexpr int D = (kCopies + WM * WN - 1) / (WM * WN);
+    static constexpr int kLds = ST * kSlice;
+    static_assert(kLds <= 160 * 1024 && D * (ST - 1) <= 63, "tile");
+};
+
+template <class G>
+__global__ __launch_bounds__(G::kThreads) void k_i8_big(I8Args a, int n_ct, int n_tt) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int MF = G::MF, NF = G::NF, D = G::D, NW = G::WM * G::WN, ST = G::ST;
+    const int total = n_ct * n_tt, per = (total + 7) / 8;
+    const int L = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || L >= total) return;  // the whole workgroup
+    const int tt = L % n_tt, ct = L / n_tt;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wn = wv % G::WN, wm = wv / G::WN;
+    const int o0 = ct * G::BM, t0 = tt * G::BN, rb = a.row_bytes;
+
+    const int w_rows = min(G::BM, a.out_dim - o0), x_rows = min(G::BN, a.n_tok - t0);
+    const bl_rsrc rw = bl_make_rsrc(a.w + (size_t)o0 * rb, (uint32_t)w_rows * (uint32_t)rb);
+    const bl_rsrc rx = bl_make_rsrc(a.xq + (size_t)t0 * rb, (uint32_t)x_rows * (uint32_t)rb);
+    const uint32_t lds0 = bl_lds(smem);
+    // copy c: 8 rows of channels (c < BM / 8) or tokens; rows behind the last
+    // repeat it (their products are not stored)
+    uint32_t off[D];
+#pragma unroll
+    for (int p = 0; p < D; p++) {
+        const int c = min(wv + NW * p, G::kCopies - 1);
+        const bool is_w = c < G::BM / 8;
+        const int row = (is_w ? 8 * c : 8 * c - G::BM) + (lane >> 3);
+        off[p] = (uint32_t)min(row, (is_w ? w_rows : x_rows) - 1) * (uint32_t)rb +
+                 16u * (uint32_t)((lane & 7) ^ I8_KEY(row));
+    }
+    const int n_sl = (rb + 127) / 128;
+    auto copy1 = [&](int i, int buf, int p) {
+        const int c = min(wv + NW * p, G::kCopies - 1);
+        const bool is_w = c < G::BM / 8;
+        uint32_t o = off[p] + 128u * (uint32_t)i;
+        if (128 * i + 128 > rb) {  // half a slice: zeros behind the row
+            const int row = (is_w ? 8 * c : 8 * c - G::BM) + (lane >> 3);
+            if (((lane & 7) ^ I8_KEY(row)) >= 4) o = 0xFFFFFFF0u;
+        }
+        const bl_rsrc r = is_w ? rw : rx;
+        bl_dma16(bl_rsrc{r[0], r[1], i < n_sl ? r[2] : 0u, r[3]}, o, 0,
+                 lds0 + (uint32_t)(buf * G::kSlice + c * 1024));
+    };
+    i8_v4 acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[m][n] = i8_v4{0, 0, 0, 0};
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint8_t *const lw = smem + (wm * 16 * MF + r16) * 128;
+    const uint8_t *const lx = smem + (G::BM + wn * 16 * NF + r16) * 128;
+    const int s0 = 16 * (q ^ I8_KEY(r16)), s1 = s0 ^ 64;
+    i8_v4 f[2][MF + NF];  // operands of a half slice: NF of tokens, MF of channels
+    auto read1 = [&](int h, int buf, int j) {
+        const int so = (h ? s1 : s0) + buf * G::kSlice;
+        f[h][j] = j < NF ? *reinterpret_cast<const i8_v4 *>(lx + j * 2048 + so)
+                         : *reinterpret_cast<const i8_v4 *>(lw + (j - NF) * 2048 + so);
+    };
+    // the MFMAs of half h; between them the reads of the other half's next
+    // operands (from slice buffer rbuf) and, with `cp`, the copies of slice i
+    auto phase = [&](auto h_c, int rbuf, bool rd, int i, int cbuf, bool cp) __attribute__((always_inline)) {
+        constexpr int h = decltype(h_c)::value;
+#pragma unroll
+        for (int m = 0; m < MF; m++) {
+            if (rd) {
+#pragma unroll
+                for (int j = m * (MF + NF) / MF; j < (m + 1) * (MF + NF) / MF; j++) read1(h ^ 1, rbuf, j);
+            }
+            if (cp) {
+#pragma unroll
+                for (int p = m * D / MF; p < (m + 1) * D / MF; p++) copy1(i, cbuf, p);
+            }
+#pragma unroll
+            for (int n = 0; n < NF; n++)
+                acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h][NF + m], f[h][n], acc[m][n], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < ST; i++)
+#pragma unroll
+        for (int p = 0; p < D; p++) copy1(i, i, p);
+    bl_barrier<D *(ST - 1)>();
+#pragma unroll
+    for (int j = 0; j < MF + NF; j++) read1(0, 0, j);
+    int buf = 0;
+    for (int i = 0; i < n_sl; i++) {
+        const int next = buf + 1 == ST ? 0 : buf + 1;
+        phase(std::integral_constant<int, 0>{}, buf, true, 0, 0, false);
+        bl_barrier<D *(ST - 2)>();
+        phase(std::integral_constant<int, 1>{}, next, true, i + ST, buf, true);
+        buf = next;
+    }
+    bl_wait<0>();  // (the copies past the last slice, zeros, land in the ring too)
+    const uint32_t esz = a.dtype_out == T_F32 ? 4u : 2u;
+    const bool vec = ((uintptr_t)a.out % (4 * esz)) == 0 && a.out_stride % 4 == 0 &&
+                     ((uintptr_t)a.wscale % 16) == 0 && ((uintptr_t)a.bias % 16) == 0;
+#pragma unroll
+    for (int n = 0; n < NF; n++)
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+            i8_finish(a, acc[m][n], o0 + 16 * (wm * MF + m) + 4 * q, t0 + 16 * (wn * NF + n) + r16, vec);
+}
+
+template <class G> hipError_t i8_big_go(const I8Args &a, hipStream_t s) {
+    static const hipError_t attr = hipFuncSetAttribute(
+        reinterpret_cast<const void *>(&k_i8_big<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+    if (attr != hipSuccess) return attr;
+    const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
+    const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
+    k_i8_big<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);
+    return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_i8_quantize(const void *x, size_t stride, int8_t *xq, float *scale, int n_tok,
                               int in_dim, uint32_t dtype, hipStream_t s) {

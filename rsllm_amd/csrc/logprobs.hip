@@ -1,138 +1,336 @@
 // Log-probability, rank, entropy and most likely alternatives of each row of
-// vocabulary logits.
+// vocabulary logits, in one pass over them.
 //   m = max l, S = sum exp(l - m), D = sum exp(l - m) (l - m)
 //   logprob = l_tok - m - log S,  entropy = log S - D / S
+// Every lane keeps m, S and D of what it has seen (S and D rescaled when m
+// rises: S' = r S, D' = r (D + (m - m') S), r = exp(m - m')), so a row is read
+// once; parts meet by the same rule. What bounds it: the read of the logits for
+// prompts, a chain of dependent loads and two launches for one row.
+// Alternatives: a wavefront keeps its n_top best in order, one a lane. A logit
+// is only looked at where it beats the last of them, which in rows of no
+// particular order soon is rare (n_top (1 + log(n / n_top)) times in n).
 #include "kernels.h"
 
 namespace rsllm_hip {
 
 namespace {
 
-__device__ __forceinline__ float lp_load(const void *p, size_t i, uint32_t dtype) {
+constexpr float kInf = __builtin_inff();
+constexpr int kLpWaves = 4;         // wavefronts a workgroup
+constexpr int kLpTurn = 16 * 64 * kLpWaves;  // elements of a turn: 16 a lane
+constexpr int kLpNoId = -2147483647 - 1;
+
+__device__ __forceinline__ float lp_one(const void *p, size_t i, uint32_t dtype) {
     if (dtype == T_F32) return static_cast<const float *>(p)[i];
     const uint16_t b = static_cast<const uint16_t *>(p)[i];
     return dtype == T_F16 ? f16_to_f32(b) : __builtin_bit_cast(float, (uint32_t)b << 16);
 }
 
-constexpr float kInf = __builtin_inff();
-
-// l - m; the limit 0 where both are +inf.
-__device__ __forceinline__ float lp_diff(float l, float m) { return l == m ? 0.0f : l - m; }
-
-}  // namespace
-
-// One workgroup per row; every listed alternative is one more look through the
-// row.
-__global__ __launch_bounds__(256) void k_logprobs_row(LogprobArgs a) {
-    __shared__ float red[4][3];
-    __shared__ int red_i[4][2];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const size_t row = (size_t)t * a.stride;
-    const int tok = a.tokens ? a.tokens[t] : -1;
-    const bool has = tok >= 0 && tok < a.vocab;
-    const float mine = has ? lp_load(a.logits, row + tok, a.dtype) : 0.0f;
-
-    auto best = [&](float v, int i, float &bv, int &bi) {
+template <uint32_t DT> struct LpVec {
+    static constexpr int N = DT == T_F32 ? 4 : 8;  // of 16 bytes
+    static constexpr int L = 16 / N;               // loads of a turn
+    static __device__ __forceinline__ void unpack(const uint4 &u, float *v) {
+        const uint32_t d[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
-            const float v2 = __shfl_xor(v, off, 64);
-            const int i2 = __shfl_xor(i, off, 64);
-            if (v2 > v || (v2 == v && i2 < i)) {
-                v = v2;
-                i = i2;
+        for (int i = 0; i < 4; i++) {
+            if constexpr (DT == T_F32) {
+                v[i] = __builtin_bit_cast(float, d[i]);
+            } else if constexpr (DT == T_BF16) {
+                v[2 * i] = __builtin_bit_cast(float, d[i] << 16);
+                v[2 * i + 1] = __builtin_bit_cast(float, d[i] & 0xFFFF0000u);
+            } else {
+                v[2 * i] = f16_to_f32(d[i] & 0xFFFFu);
+                v[2 * i + 1] = f16_to_f32(d[i] >> 16);
             }
         }
-        __syncthreads();
-        if (lane == 0) {
-            red[wv][0] = v;
-            red_i[wv][0] = i;
-        }
-        __syncthreads();
-        bv = red[0][0];
-        bi = red_i[0][0];
-        for (int w = 1; w < 4; w++)
-            if (red[w][0] > bv || (red[w][0] == bv && red_i[w][0] < bi)) {
-                bv = red[w][0];
-                bi = red_i[w][0];
-            }
-    };
+    }
+};
 
-    float v = -kInf, m;
-    int above = 0, bad = 0, unused;
-    for (int i = tid; i < a.vocab; i += 256) {
-        const float l = lp_load(a.logits, row + i, a.dtype);
-        if (l > v) v = l;
-        above += has && l > mine ? 1 : 0;
-        bad |= l != l ? 1 : 0;
-    }
-    best(v, 0, m, unused);
-    float s = 0.0f, d = 0.0f;
-    for (int i = tid; i < a.vocab; i += 256) {
-        const float l = lp_load(a.logits, row + i, a.dtype);
-        if (l > -kInf) {
-            const float x = lp_diff(l, m), e = __expf(x);
-            s += e;
-            if (e > 0.0f) d += e * x;
+// Running sums of some logits; m -inf: none but -inf so far. NaN in s: a NaN seen.
+struct LpSums {
+    float m, s, d;
+};
+// exp(x), x <= 0. (e x is wanted with e = 0 at x = -inf: hence the floor, far
+// below where e vanishes.)
+__device__ __forceinline__ float lp_exp(float x) { return __expf(x); }
+__device__ __forceinline__ float lp_floor(float x) { return fmaxf(x, -200.0f); }
+
+// What `a` and `b` saw together. +inf: the limit, in which only +inf counts (s
+// their number).
+__device__ __forceinline__ LpSums lp_join(const LpSums &a, const LpSums &b) {
+    const float m = fmaxf(a.m, b.m);
+    const float xa = a.m == m ? 0.0f : a.m - m, xb = b.m == m ? 0.0f : b.m - m;
+    const float ra = lp_exp(xa), rb = lp_exp(xb);
+    return LpSums{m, ra * a.s + rb * b.s,
+                  ra * (a.d + lp_floor(xa) * a.s) + rb * (b.d + lp_floor(xb) * b.s)};
+}
+
+// The best (value, id) seen by a wavefront, the i-th at lane i; -inf, kLpNoId
+// behind the last.
+struct LpTop {
+    float v;
+    int i;
+};
+__device__ __forceinline__ int lp_shift(int x) {  // lane l gets lane l - 1's
+    return __builtin_amdgcn_update_dpp(x, x, 0x138, 0xf, 0xf, false);  // wave_shr:1
+}
+__device__ __forceinline__ float lp_lane(float v, int l) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+// Takes every lane's candidate (v, i) that is among the n best into the list.
+// edge_v, edge_i: the list's n-th (uniform).
+__device__ __forceinline__ void lp_take(LpTop &top, int n, float &edge_v, int &edge_i, float v, int i) {
+    const int lane = threadIdx.x & 63;
+    auto beats = [&]() { return v > edge_v || (v == edge_v && i < edge_i); };
+    unsigned long long todo = __ballot(beats());
+    while (todo) {
+        const int who = __ffsll(todo) - 1;
+        todo &= todo - 1;
+        const float cv = lp_lane(v, who);
+        const int ci = __builtin_amdgcn_readlane(i, who);
+        const bool before = top.v > cv || (top.v == cv && top.i < ci);
+        const int at = __popcll(__ballot(before));
+        const float pv = __builtin_bit_cast(float, lp_shift(__builtin_bit_cast(int, top.v)));
+        const int pi = lp_shift(top.i);
+        if (lane > at) {
+            top.v = pv;
+            top.i = pi;
+        } else if (lane == at) {
+            top.v = cv;
+            top.i = ci;
         }
-    }
-    s = wave_sum(s);
-    d = wave_sum(d);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-        above += __shfl_xor(above, off, 64);
-        bad |= __shfl_xor(bad, off, 64);
-    }
-    __syncthreads();
-    if (lane == 0) {
-        red[wv][1] = s;
-        red[wv][2] = d;
-        red_i[wv][0] = above;
-        red_i[wv][1] = bad;
-    }
-    __syncthreads();
-    s = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
-    d = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
-    above = red_i[0][0] + red_i[1][0] + red_i[2][0] + red_i[3][0];
-    bad = red_i[0][1] | red_i[1][1] | red_i[2][1] | red_i[3][1];
-    __syncthreads();
-    const bool none = m == -kInf;  // nothing but -inf (and NaN)
-    const float log_s = none ? 0.0f : logf(s), nan = __builtin_nanf("");
-    auto logprob = [&](float l) { return bad ? nan : none ? -kInf : lp_diff(l, m) - log_s; };
-    if (tid == 0) {
-        if (a.tokens) {
-            a.logprob[t] = has ? logprob(mine) : nan;
-            if (a.rank) a.rank[t] = has && mine == mine ? above + 1 : 0;
-        }
-        if (a.entropy) a.entropy[t] = bad ? nan : none ? 0.0f : log_s - d / s;
-    }
-    float last = kInf;
-    int last_i = -1;
-    for (int r = 0; r < a.n_top; r++) {
-        float bv = -kInf, cv;
-        int bi = a.vocab, ci;
-        for (int i = tid; i < a.vocab; i += 256) {
-            const float l = lp_load(a.logits, row + i, a.dtype);
-            if ((l < last || (l == last && i > last_i)) && l > bv) {
-                bv = l;
-                bi = i;
-            }
-        }
-        best(bv, bi, cv, ci);
-        const bool empty = !(cv > -kInf);
-        if (tid == 0) {
-            a.top_ids[(size_t)t * a.n_top + r] = empty ? -1 : ci;
-            a.top_logprobs[(size_t)t * a.n_top + r] = empty ? (bad ? nan : -kInf) : logprob(cv);
-        }
-        last = cv;
-        last_i = ci;
+        edge_v = lp_lane(top.v, n - 1);
+        edge_i = __builtin_amdgcn_readlane(top.i, n - 1);
+        todo &= __ballot(beats());
     }
 }
 
-size_t logprobs_scratch_bytes(int n_tok, int vocab, int n_top) { return 0; }
+// One part of a row: sums, the number of logits above the token's, and its list.
+struct LpPart {
+    LpSums sums;
+    int above;
+};
+
+__device__ __forceinline__ LpPart lp_wave_join(LpPart p) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+        const LpSums o{__shfl_xor(p.sums.m, off, 64), __shfl_xor(p.sums.s, off, 64),
+                       __shfl_xor(p.sums.d, off, 64)};
+        p.sums = lp_join(p.sums, o);
+        p.above += __shfl_xor(p.above, off, 64);
+    }
+    return p;
+}
+
+// A row's outputs, by one wavefront that holds its sums and list.
+__device__ __forceinline__ void lp_finish(const LogprobArgs &a, int t, const LpPart &p, const LpTop &top) {
+    const int lane = threadIdx.x & 63;
+    const float m = p.sums.m, nan = __builtin_nanf("");
+    const bool bad = p.sums.s != p.sums.s, empty = m == -kInf;
+    const float log_s = empty ? 0.0f : logf(p.sums.s);
+    auto logprob = [&](float l) {
+        return bad ? nan : empty ? -kInf : (l == m ? 0.0f : l - m) - log_s;
+    };
+    if (lane == 0) {
+        if (a.tokens) {
+            const int tok = a.tokens[t];
+            const bool has = tok >= 0 && tok < a.vocab;
+            const float l = has ? lp_one(a.logits, (size_t)t * a.stride + tok, a.dtype) : nan;
+            a.logprob[t] = has ? logprob(l) : nan;
+            if (a.rank) a.rank[t] = l == l ? p.above + 1 : 0;
+        }
+        if (a.entropy) a.entropy[t] = bad ? nan : empty ? 0.0f : log_s - p.sums.d / p.sums.s;
+    }
+    if (lane < a.n_top) {
+        const size_t at = (size_t)t * a.n_top + lane;
+        a.top_ids[at] = top.v > -kInf ? top.i : -1;
+        a.top_logprobs[at] = top.v > -kInf ? logprob(top.v) : bad ? nan : -kInf;
+    }
+}
+
+}  // namespace
+
+// Where the parts of a row lie in the caller's workspace.
+struct LpWork {
+    LpPart *parts;  // [n_tok x chunks]
+    LpTop *tops;    // [n_tok x chunks x n_top]
+};
+
+// Workgroup (chunk, row): `turns` turns, each kLpWaves * L pieces of 64 lanes x
+// 16 bytes of the row, counted from the 16 bytes that the row starts in. With one chunk a row it
+// writes the row's outputs, else its part.
+template <uint32_t DT>
+__global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWork w, int chunks,
+                                                            int turns) {
+    using V = LpVec<DT>;
+    constexpr int N = V::N, L = V::L, M = N * L;
+    __shared__ LpPart part[kLpWaves];
+    __shared__ LpTop list[kLpWaves][64];
+    const int t = blockIdx.x / chunks, c = blockIdx.x - t * chunks;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const size_t row = (size_t)t * a.stride;
+    const uint8_t *const p = static_cast<const uint8_t *>(a.logits) + row * (16 / N);
+    const int head = (int)((uintptr_t)p & 15) / (16 / N);  // elements of the first line before the row
+
+    const int tok = a.tokens ? a.tokens[t] : -1;
+    // (NaN: nothing is above)
+    const float mine = tok >= 0 && tok < a.vocab ? lp_one(a.logits, row + tok, DT) : __builtin_nanf("");
+    LpSums sum{-kInf, 0.0f, 0.0f};
+    int above = 0;
+    LpTop top{-kInf, kLpNoId};
+    float edge_v = -kInf;
+    int edge_i = kLpNoId;
+
+    const int pieces = turns * (kLpWaves * L);
+    const int all = (int)(((long long)head + a.vocab + 64 * N - 1) / (64 * N));
+    const int p1 = min(all, (c + 1) * pieces);
+    for (int q0 = c * pieces + wv * L; q0 < p1; q0 += kLpWaves * L) {
+        float v[M];
+        // (piece q0's first element may be before the row: only in its first piece)
+        const long long e0 = (long long)q0 * (64 * N) - head;
+        if (e0 >= 0 && q0 + L <= p1 && e0 + 64 * M <= a.vocab) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(p + e0 * (16 / N)) + lane;
+            uint4 u[L];
+#pragma unroll
+            for (int k = 0; k < L; k++) u[k] = src[64 * k];
+#pragma unroll
+            for (int k = 0; k < L; k++) V::unpack(u[k], v + N * k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < L; k++)
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const long long e = e0 + 64 * N * k + N * lane + i;
+                    const bool in = q0 + k < p1 && e >= 0 && e < a.vocab;
+                    v[N * k + i] = in ? lp_one(a.logits, row + (size_t)e, DT) : -kInf;
+                }
+        }
+        float big = v[0];
+#pragma unroll
+        for (int i = 1; i < M; i++) big = fmaxf(big, v[i]);  // (a NaN is passed over)
+        const float m = fmaxf(sum.m, big);
+        if (__builtin_expect(__ballot(m == kInf) != 0, 0)) {
+            // +inf - +inf is no number: the limit, one element at a time
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+                above += v[i] > mine ? 1 : 0;
+                sum = lp_join(sum, v[i] != v[i] ? LpSums{-kInf, v[i], 0.0f}
+                                                : LpSums{v[i], v[i] > -kInf ? 1.0f : 0.0f, 0.0f});
+            }
+        } else {
+            const float base = m == -kInf ? 0.0f : m;  // (-inf - -inf is none either)
+            const float x = sum.m - base, r = lp_exp(x);
+            float s = 0.0f, d = 0.0f;
+#pragma unroll
+            for (int i = 0; i < M; i++) {
+                above += v[i] > mine ? 1 : 0;
+                const float y = v[i] - base, e = lp_exp(y);
+                s += e;
+                d = fmaf(e, lp_floor(y), d);
+            }
+            sum.d = r * (sum.d + lp_floor(x) * sum.s) + d;
+            sum.s = r * sum.s + s;
+            sum.m = m;
+        }
+        if (a.n_top && __ballot(big >= edge_v && big > -kInf)) {
+#pragma unroll
+            for (int k = 0; k < L; k++)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                    lp_take(top, a.n_top, edge_v, edge_i, v[N * k + i], (int)(e0 + 64 * N * k + N * lane + i));
+        }
+    }
+    const LpPart mypart = lp_wave_join(LpPart{sum, above});
+    if (lane == 0) part[wv] = mypart;
+    if (a.n_top) list[wv][lane] = top;
+    __syncthreads();
+    if (wv != 0) return;
+    LpPart all_part = part[0];
+#pragma unroll
+    for (int k = 1; k < kLpWaves; k++) {
+        all_part.sums = lp_join(all_part.sums, part[k].sums);
+        all_part.above += part[k].above;
+        if (a.n_top) {
+            const LpTop o = list[k][lane];
+            lp_take(top, a.n_top, edge_v, edge_i, lane < a.n_top ? o.v : -kInf, lane < a.n_top ? o.i : kLpNoId);
+        }
+    }
+    if (chunks == 1) {
+        lp_finish(a, t, all_part, top);
+    } else {
+        const size_t at = (size_t)t * chunks + c;
+        if (lane == 0) w.parts[at] = all_part;
+        if (lane < a.n_top) w.tops[at * a.n_top + lane] = top;
+    }
+}
+
+// One wavefront per row: its chunks' parts and lists.
+__global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, LpWork w, int chunks) {
+    const int t = blockIdx.x, lane = threadIdx.x;
+    const size_t at = (size_t)t * chunks;
+    LpPart p{{-kInf, 0.0f, 0.0f}, 0};
+    for (int c = lane; c < chunks; c += 64) {
+        const LpPart o = w.parts[at + c];
+        p.sums = lp_join(p.sums, o.sums);
+        p.above += o.above;
+    }
+    p = lp_wave_join(p);
+    LpTop top{-kInf, kLpNoId};
+    float edge_v = -kInf;
+    int edge_i = kLpNoId;
+    const int n = chunks * a.n_top;
+    for (int e = lane; e - lane < n; e += 64) {
+        const LpTop o = e < n ? w.tops[at * a.n_top + e] : LpTop{-kInf, kLpNoId};
+        lp_take(top, a.n_top, edge_v, edge_i, o.v, o.i);
+    }
+    lp_finish(a, t, p, top);
+}
+
+namespace {
+
+// Chunks of a row. A workgroup takes a whole row where the rows alone keep the
+// CUs busy (four workgroups each); fewer rows are cut up to that many, but no
+// finer than one turn of a workgroup's loads.
+struct LpPlan {
+    int chunks, turns;  // turns of a chunk
+};
+LpPlan lp_plan(int n_tok, int vocab) {
+    // (8: the elements before the row in its first 16 bytes at most, so that the
+    // plan depends on n_tok and vocab alone)
+    const long long turns = ((long long)vocab + 8 + kLpTurn - 1) / kLpTurn;
+    const long long want = std::min<long long>(turns, std::max(1, 1024 / std::max(n_tok, 1)));
+    const long long per = (turns + want - 1) / want;
+    return {(int)((turns + per - 1) / per), (int)per};
+}
+size_t lp_round(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t logprobs_scratch_bytes(int n_tok, int vocab, int n_top) {
+    const LpPlan p = lp_plan(n_tok, vocab);
+    if (p.chunks == 1 || n_tok == 0) return 0;
+    const size_t n = (size_t)n_tok * p.chunks;
+    return lp_round(n * sizeof(LpPart)) + lp_round(n * n_top * sizeof(LpTop));
+}
 
 hipError_t launch_logprobs(const LogprobArgs &a, uint8_t *work, int n_tok, hipStream_t s) {
     if (n_tok <= 0) return hipSuccess;
-    k_logprobs_row<<<(unsigned)n_tok, 256, 0, s>>>(a);
+    const LpPlan p = lp_plan(n_tok, a.vocab);
+    LpWork w{};
+    if (p.chunks > 1) {
+        w.parts = reinterpret_cast<LpPart *>(work);
+        w.tops = reinterpret_cast<LpTop *>(work + lp_round((size_t)n_tok * p.chunks * sizeof(LpPart)));
+    }
+    const long long wgs = (long long)n_tok * p.chunks;
+    if (wgs > 0x7FFFFFFFll) return hipErrorInvalidValue;
+    const dim3 g((unsigned)wgs);
+    if (a.dtype == T_F32) k_logprobs<T_F32><<<g, 64 * kLpWaves, 0, s>>>(a, w, p.chunks, p.turns);
+    else if (a.dtype == T_F16) k_logprobs<T_F16><<<g, 64 * kLpWaves, 0, s>>>(a, w, p.chunks, p.turns);
+    else k_logprobs<T_BF16><<<g, 64 * kLpWaves, 0, s>>>(a, w, p.chunks, p.turns);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.chunks == 1) return e;
+    k_logprobs_join<<<(unsigned)n_tok, 64, 0, s>>>(a, w, p.chunks);
     return hipGetLastError();
 }
 
