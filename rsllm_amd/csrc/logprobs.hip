@@ -8,7 +8,8 @@
 // prompts, a chain of dependent loads and two launches for one row.
 // Alternatives: a wavefront keeps its n_top best in order, one a lane. A logit
 // is only looked at where it beats the last of them, which in rows of no
-// particular order soon is rare (n_top (1 + log(n / n_top)) times in n).
+// particular order soon is rare (n_top (1 + log(n / n_top)) times in n); many
+// that do at once are sorted and merged in.
 #include "kernels.h"
 
 namespace rsllm_hip {
@@ -77,33 +78,105 @@ __device__ __forceinline__ int lp_shift(int x) {  // lane l gets lane l - 1's
 __device__ __forceinline__ float lp_lane(float v, int l) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
 }
-// Takes every lane's candidate (v, i) that is among the n best into the list.
-// edge_v, edge_i: the list's n-th (uniform).
-__device__ __forceinline__ void lp_take(LpTop &top, int n, float &edge_v, int &edge_i, float v, int i) {
-    const int lane = threadIdx.x & 63;
-    auto beats = [&]() { return v > edge_v || (v == edge_v && i < edge_i); };
-    unsigned long long todo = __ballot(beats());
-    while (todo) {
-        const int who = __ffsll(todo) - 1;
-        todo &= todo - 1;
-        const float cv = lp_lane(v, who);
-        const int ci = __builtin_amdgcn_readlane(i, who);
-        const bool before = top.v > cv || (top.v == cv && top.i < ci);
-        const int at = __popcll(__ballot(before));
-        const float pv = __builtin_bit_cast(float, lp_shift(__builtin_bit_cast(int, top.v)));
-        const int pi = lp_shift(top.i);
-        if (lane > at) {
-            top.v = pv;
-            top.i = pi;
-        } else if (lane == at) {
-            top.v = cv;
-            top.i = ci;
-        }
-        edge_v = lp_lane(top.v, n - 1);
-        edge_i = __builtin_amdgcn_readlane(top.i, n - 1);
-        todo &= __ballot(beats());
+// (av, ai) comes before (bv, bi): the larger, then the lower id.
+__device__ __forceinline__ bool lp_before(float av, int ai, float bv, int bi) {
+    return av > bv || (av == bv && ai < bi);
+}
+// Lane l gets lane l ^ X's: within rows of 16 lanes by DPP, across by a shuffle.
+template <int X> __device__ __forceinline__ int lp_xor(int x) {
+    if constexpr (X == 1) return __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xf, 0xf, false);  // quad_perm
+    if constexpr (X == 2) return __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xf, 0xf, false);
+    if constexpr (X == 4) {  // ^ 7 (row_half_mirror), then ^ 3
+        const int y = __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false);
+        return __builtin_amdgcn_update_dpp(y, y, 0x1B, 0xf, 0xf, false);
+    }
+    if constexpr (X == 8) return __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, false);  // row_ror:8
+    return __shfl_xor(x, X, 64);
+}
+// One step of a bitonic network: lanes l and l ^ X keep the one before at the
+// lane where `first` says so.
+template <int X> __device__ __forceinline__ void lp_step(LpTop &t, bool first) {
+    const float v = __builtin_bit_cast(float, lp_xor<X>(__builtin_bit_cast(int, t.v)));
+    const int i = lp_xor<X>(t.i);
+    if (lp_before(v, i, t.v, t.i) == first) {
+        t.v = v;
+        t.i = i;
     }
 }
+// 64 lanes whose order rises and then falls (or the reverse), into order; down: the
+// first at lane 0 of each run of 2 X lanes.
+template <int X> __device__ __forceinline__ void lp_merge_from(LpTop &t, bool down) {
+    const int lane = threadIdx.x & 63;
+    lp_step<X>(t, ((lane & X) == 0) == down);
+    if constexpr (X > 1) lp_merge_from<X / 2>(t, down);
+}
+__device__ __forceinline__ void lp_sort(LpTop &t) {
+    const int lane = threadIdx.x & 63;
+    lp_merge_from<1>(t, (lane & 2) == 0);
+    lp_merge_from<2>(t, (lane & 4) == 0);
+    lp_merge_from<4>(t, (lane & 8) == 0);
+    lp_merge_from<8>(t, (lane & 16) == 0);
+    lp_merge_from<16>(t, (lane & 32) == 0);
+    lp_merge_from<32>(t, true);
+}
+// The 64 best of two lists in order: the better of a's i-th and b's 63 - i-th
+// falls and rises once.
+__device__ __forceinline__ void lp_merge(LpTop &top, const LpTop &o) {
+    const float v = __builtin_bit_cast(float, lp_xor<63>(__builtin_bit_cast(int, o.v)));
+    const int i = lp_xor<63>(o.i);
+    if (lp_before(v, i, top.v, top.i)) {
+        top.v = v;
+        top.i = i;
+    }
+    lp_merge_from<32>(top, true);
+}
+
+// A wavefront's list and its n-th (uniform).
+struct LpList {
+    LpTop top{-kInf, kLpNoId};
+    float edge_v = -kInf;
+    int edge_i = kLpNoId;
+    __device__ __forceinline__ void edge(int n) {
+        edge_v = lp_lane(top.v, n - 1);
+        edge_i = __builtin_amdgcn_readlane(top.i, n - 1);
+    }
+    // Takes every lane's candidate that is among the n best, and says whether
+    // there was one: a few one by one, more of them sorted (kSorted: they come so)
+    // and merged. An insertion is some 25 dependent instructions, a sort 21 steps
+    // of 8 and a merge 7.
+    template <bool kSorted> __device__ __forceinline__ bool take(int n, float v, int i) {
+        const int lane = threadIdx.x & 63;
+        bool beats = lp_before(v, i, edge_v, edge_i);
+        unsigned long long todo = __ballot(beats);
+        if (!todo) return false;
+        if (__popcll(todo) > (kSorted ? 3 : 10)) {
+            LpTop o{beats ? v : -kInf, beats ? i : kLpNoId};
+            if (!kSorted) lp_sort(o);
+            lp_merge(top, o);
+            edge(n);
+            return true;
+        }
+        do {
+            const int who = __ffsll(todo) - 1;
+            todo &= todo - 1;
+            const float cv = lp_lane(v, who);
+            const int ci = __builtin_amdgcn_readlane(i, who);
+            const int at = __popcll(__ballot(lp_before(top.v, top.i, cv, ci)));
+            const float pv = __builtin_bit_cast(float, lp_shift(__builtin_bit_cast(int, top.v)));
+            const int pi = lp_shift(top.i);
+            if (lane > at) {
+                top.v = pv;
+                top.i = pi;
+            } else if (lane == at) {
+                top.v = cv;
+                top.i = ci;
+            }
+            edge(n);
+            todo &= __ballot(lp_before(v, i, edge_v, edge_i));
+        } while (todo);
+        return true;
+    }
+};
 
 // One part of a row: sums, the number of logits above the token's, and its list.
 struct LpPart {
@@ -178,9 +251,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
     const float mine = tok >= 0 && tok < a.vocab ? lp_one(a.logits, row + tok, DT) : __builtin_nanf("");
     LpSums sum{-kInf, 0.0f, 0.0f};
     int above = 0;
-    LpTop top{-kInf, kLpNoId};
-    float edge_v = -kInf;
-    int edge_i = kLpNoId;
+    LpList best;
 
     const int pieces = turns * (kLpWaves * L);
     const int all = (int)(((long long)head + a.vocab + 64 * N - 1) / (64 * N));
@@ -233,17 +304,30 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
             sum.s = r * sum.s + s;
             sum.m = m;
         }
-        if (a.n_top && __ballot(big >= edge_v && big > -kInf)) {
+        if (a.n_top && __ballot(big >= best.edge_v && big > -kInf)) {
+            const int i0 = (int)(e0 + N * lane);
+            if (best.edge_v == -kInf) {
+                // the first turns: every lane's largest first, which leaves
+                // little of the rest to take
+                int at = 0;
+                float one = -kInf;
 #pragma unroll
-            for (int k = 0; k < L; k++)
+                for (int j = 0; j < M; j++) {
+                    at = v[j] > one ? j : at;
+                    one = fmaxf(one, v[j]);
+                }
+                best.take<false>(a.n_top, one, i0 + at / N * (64 * N) + at % N);
 #pragma unroll
-                for (int i = 0; i < N; i++)
-                    lp_take(top, a.n_top, edge_v, edge_i, v[N * k + i], (int)(e0 + 64 * N * k + N * lane + i));
+                for (int j = 0; j < M; j++) v[j] = j == at ? -kInf : v[j];
+            }
+#pragma unroll
+            for (int j = 0; j < M; j++)
+                best.take<false>(a.n_top, v[j], i0 + j / N * (64 * N) + j % N);
         }
     }
     const LpPart mypart = lp_wave_join(LpPart{sum, above});
     if (lane == 0) part[wv] = mypart;
-    if (a.n_top) list[wv][lane] = top;
+    if (a.n_top) list[wv][lane] = lane < a.n_top ? best.top : LpTop{-kInf, kLpNoId};
     __syncthreads();
     if (wv != 0) return;
     LpPart all_part = part[0];
@@ -253,15 +337,15 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
         all_part.above += part[k].above;
         if (a.n_top) {
             const LpTop o = list[k][lane];
-            lp_take(top, a.n_top, edge_v, edge_i, lane < a.n_top ? o.v : -kInf, lane < a.n_top ? o.i : kLpNoId);
+            best.take<true>(a.n_top, o.v, o.i);
         }
     }
     if (chunks == 1) {
-        lp_finish(a, t, all_part, top);
+        lp_finish(a, t, all_part, best.top);
     } else {
         const size_t at = (size_t)t * chunks + c;
         if (lane == 0) w.parts[at] = all_part;
-        if (lane < a.n_top) w.tops[at * a.n_top + lane] = top;
+        if (lane < a.n_top) w.tops[at * a.n_top + lane] = best.top;
     }
 }
 
@@ -276,15 +360,20 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, LpWork w, i
         p.above += o.above;
     }
     p = lp_wave_join(p);
-    LpTop top{-kInf, kLpNoId};
-    float edge_v = -kInf;
-    int edge_i = kLpNoId;
-    const int n = chunks * a.n_top;
-    for (int e = lane; e - lane < n; e += 64) {
-        const LpTop o = e < n ? w.tops[at * a.n_top + e] : LpTop{-kInf, kLpNoId};
-        lp_take(top, a.n_top, edge_v, edge_i, o.v, o.i);
+    // a chunk's list a lane, their i-th entries together: as soon as none of those
+    // is among the best, none behind them is
+    LpList best;
+    for (int c0 = 0; c0 < chunks && a.n_top; c0 += 64) {
+        const bool in = c0 + lane < chunks;
+        const LpTop *src = w.tops + (at + min(c0 + lane, chunks - 1)) * a.n_top;
+        LpTop next = src[0];
+        for (int r = 0; r < a.n_top; r++) {
+            const LpTop o = next;
+            next = src[min(r + 1, a.n_top - 1)];
+            if (!best.take<false>(a.n_top, in ? o.v : -kInf, in ? o.i : kLpNoId)) break;
+        }
     }
-    lp_finish(a, t, p, top);
+    lp_finish(a, t, p, best.top);
 }
 
 namespace {
