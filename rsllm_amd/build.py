@@ -51,6 +51,7 @@ EXTRA_FLAGS = {
     "gemv_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gemm_exact.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "moe_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "int8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

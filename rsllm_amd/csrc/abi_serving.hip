@@ -46,16 +46,14 @@ constexpr size_t kI8MaxIn = 131071;  // 128 * 128 * 131071 < 2^31
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// The caller's work of an int8 product: codes, scales, then the product's own.
+// The caller's work of an int8 product: codes, then scales.
 struct I8Work {
-    size_t codes = 0, scales = 0, split = 0, total = 0;
+    size_t codes = 0, total = 0;
 };
 bool i8_work(size_t n_tok, size_t in_dim, size_t out_dim, I8Work *w) {
     if (!counts_ok(n_tok) || !counts_ok(out_dim) || in_dim == 0 || in_dim > kI8MaxIn) return false;
     w->codes = round256(n_tok * i8_row_bytes(in_dim));
-    w->scales = round256(n_tok * sizeof(float));
-    w->split = round256(i8_split_bytes((int)n_tok, (int)in_dim, (int)out_dim));
-    w->total = w->codes + w->scales + w->split;
+    w->total = w->codes + round256(n_tok * sizeof(float));
     return true;
 }
 
@@ -193,8 +191,7 @@ int rsllm_hip_matmul_int8_prequant_dev(void *out, size_t out_len, size_t out_str
     if (const int rc = abi::make_device_current()) return rc;
     const I8Args a{weights, xq, wscale, xscale, bias_len ? bias : nullptr, out, out_stride,
                    (int)n_tok, (int)out_dim, (int)i8_row_bytes(in_dim), dtype_out};
-    HIP_TRY(launch_i8_matmul(a, work + parts.codes + parts.scales, (hipStream_t)stream),
-            "matmul_int8");
+    HIP_TRY(launch_i8_matmul(a, (hipStream_t)stream), "matmul_int8");
     return abi::ok_status();
 }
 
@@ -216,13 +213,16 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
     if (const int rc = abi::make_device_current()) return rc;
     int8_t *xq = reinterpret_cast<int8_t *>(work);
     float *xscale = reinterpret_cast<float *>(work + parts.codes);
+    const I8Args a{weights, xq, wscale, xscale, bias_len ? bias : nullptr, out, out_stride,
+                   (int)n_tok, (int)out_dim, (int)i8_row_bytes(in_dim), dtype_out};
+    if (i8_few_supported((int)n_tok, (int)in_dim)) {
+        HIP_TRY(launch_i8_few(a, x, x_stride, (int)in_dim, dtype_x, (hipStream_t)stream), "matmul_int8");
+        return abi::ok_status();
+    }
     HIP_TRY(launch_i8_quantize(x, x_stride, xq, xscale, (int)n_tok, (int)in_dim, dtype_x,
                                (hipStream_t)stream),
             "quantize_int8");
-    const I8Args a{weights, xq, wscale, xscale, bias_len ? bias : nullptr, out, out_stride,
-                   (int)n_tok, (int)out_dim, (int)i8_row_bytes(in_dim), dtype_out};
-    HIP_TRY(launch_i8_matmul(a, work + parts.codes + parts.scales, (hipStream_t)stream),
-            "matmul_int8");
+    HIP_TRY(launch_i8_matmul(a, (hipStream_t)stream), "matmul_int8");
     return abi::ok_status();
 }
 

@@ -294,9 +294,13 @@ struct I8Args {
     int n_tok, out_dim, row_bytes;
     uint32_t dtype_out;
 };
-// `split` holds i8_split_bytes(n_tok, in_dim, out_dim) bytes.
-size_t i8_split_bytes(int n_tok, int in_dim, int out_dim);
-hipError_t launch_i8_matmul(const I8Args &a, uint8_t *split, hipStream_t s);
+hipError_t launch_i8_matmul(const I8Args &a, hipStream_t s);
+// The same from the floats x themselves (dtype, x_stride elements apart; a.xq and
+// a.xscale are not used), in one launch; hipErrorNotSupported where
+// i8_few_supported says no.
+bool i8_few_supported(int n_tok, int in_dim);
+hipError_t launch_i8_few(const I8Args &a, const void *x, size_t x_stride, int in_dim, uint32_t dtype,
+                         hipStream_t s);
 
 // logprobs.hip: per row of logits (dtype F32, F16 or BF16, `stride` elements
 // apart) what rsllm_hip_token_logprobs_dev gives. tokens may be null (logprob
