@@ -29,7 +29,7 @@ __device__ __forceinline__ void i8_store(void *p, size_t i, float v, uint32_t dt
 // near its code. Scales below 2^-100 are worked with 2^64 times as large, values
 // too (both exactly), where 1 / d still fits.
 struct I8Scale {
-    float d, up, d_up, inv;
+    float d, up, d_up, inv, quick;  // quick: 1 / d, or 0 where up is not 1
 };
 __device__ __forceinline__ I8Scale i8_scale(float amax) {
     I8Scale s;
@@ -37,6 +37,7 @@ __device__ __forceinline__ I8Scale i8_scale(float amax) {
     s.up = s.d < 0x1p-100f ? 0x1p64f : 1.0f;
     s.d_up = s.d * s.up;
     s.inv = s.d > 0.0f ? 1.0f / s.d_up : 0.0f;
+    s.quick = s.up == 1.0f ? s.inv : 0.0f;
     return s;
 }
 // v / d to the nearest integer, halves to even: the product with 1 / d is off by
@@ -81,15 +82,28 @@ __device__ __forceinline__ void i8_load_vec(const void *x, size_t row, int i, in
         for (int k = 0; k < N; k++) v[k] = i + k < in_dim ? i8_load(x, row + i + k, DT) : 0.0f;
     }
 }
-// The N codes of v, packed, to 4-byte aligned memory.
+// The N codes of v, packed, to 4-byte aligned memory. Adding 1.5 * 2^23 to v / d
+// leaves the nearest integer in the low bits of the sum; what is left over is
+// below d / 2 for all of them but once in some 2^17, and then v is taken one by
+// one (as in rows of tiny scales, whose `quick` is 0).
 template <int N> __device__ __forceinline__ void i8_store_codes(int8_t *dst, const float *v, const I8Scale &s) {
-    uint32_t w[N / 4];
+#pragma clang fp contract(off)
+    uint32_t b[N], w[N / 4];
+    float left = 0.0f;
 #pragma unroll
-    for (int k = 0; k < N / 4; k++) {
-        w[k] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[k] |= (uint32_t)(uint8_t)(int8_t)i8_code(v[4 * k + j], s) << (8 * j);
+    for (int k = 0; k < N; k++) {
+        const float sum = __builtin_fmaf(v[k], s.quick, 0x1.8p23f), r = sum - 0x1.8p23f;
+        left = fmaxf(left, fabsf(__builtin_fmaf(-r, s.d, v[k])));
+        b[k] = __builtin_bit_cast(uint32_t, sum);
     }
+    if (!(2.0f * left < s.d)) {
+#pragma unroll
+        for (int k = 0; k < N; k++) b[k] = (uint32_t)i8_code(v[k], s);
+    }
+#pragma unroll
+    for (int k = 0; k < N / 4; k++)  // the low bytes of four
+        w[k] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * k + 3], b[4 * k + 2], 0x0C0C0400u),
+                                     __builtin_amdgcn_perm(b[4 * k + 1], b[4 * k], 0x0C0C0400u), 0x05040100u);
     if constexpr (N == 4) *reinterpret_cast<uint32_t *>(dst) = w[0];
     else *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
 }
@@ -182,19 +196,35 @@ __global__ __launch_bounds__(256) void k_i8_few(I8Args a, const void *__restrict
                     w[r][p] = bload16(rw, (uint32_t)((wv * R + r) * rb + k0 + 1024 * p + 16 * lane), 0);
             }
     };
-    load(0);
+    // x, then the first weights behind it: loads return in order
+    constexpr int kHeld = 16 / (N * (T > 2 ? 2 : 1));
+    float held[T][kHeld][N];
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+        for (int h = 0; h < kHeld; h++) {
+            const int i = (h * 256 + tid) * N;
+#pragma unroll
+            for (int k = 0; k < N; k++) held[t][h][k] = 0.0f;
+            if (i < in_dim) i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, held[t][h]);
+        }
+    if (in_dim <= kHeld * 256 * N) load(0);
     uint32_t big[T];
 #pragma unroll
-    for (int t = 0; t < T; t++) big[t] = 0;
-    for (int i = tid * N; i < in_dim; i += 256 * N) {
-        float v[T][N];
+    for (int t = 0; t < T; t++) {
+        big[t] = 0;
 #pragma unroll
-        for (int t = 0; t < T; t++) i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, v[t]);
+        for (int h = 0; h < kHeld; h++)
 #pragma unroll
-        for (int t = 0; t < T; t++)
+            for (int k = 0; k < N; k++) big[t] = max(big[t], i8_abs_bits(held[t][h][k]));
+        for (int i = (kHeld * 256 + tid) * N; i < in_dim; i += 256 * N) {
+            float v[N];
+            i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, v);
 #pragma unroll
-            for (int k = 0; k < N; k++) big[t] = max(big[t], i8_abs_bits(v[t][k]));
+            for (int k = 0; k < N; k++) big[t] = max(big[t], i8_abs_bits(v[k]));
+        }
     }
+    if (in_dim > kHeld * 256 * N) load(0);
 #pragma unroll
     for (int t = 0; t < T; t++) {
 #pragma unroll
@@ -209,13 +239,16 @@ __global__ __launch_bounds__(256) void k_i8_few(I8Args a, const void *__restrict
         big[t] = max(max(red[t][0], red[t][1]), max(red[t][2], red[t][3]));
         ok[t] = i8_finite_bits(big[t]);
         sc[t] = i8_scale(ok[t] ? __builtin_bit_cast(float, big[t]) : 0.0f);
-    }
-    for (int i = tid * N; i < kp; i += 256 * N) {
-        float v[T][N];
 #pragma unroll
-        for (int t = 0; t < T; t++) i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, v[t]);
-#pragma unroll
-        for (int t = 0; t < T; t++) i8_store_codes<N>(codes + t * kp + i, v[t], sc[t]);
+        for (int h = 0; h < kHeld; h++) {
+            const int i = (h * 256 + tid) * N;
+            if (i < kp) i8_store_codes<N>(codes + t * kp + i, held[t][h], sc[t]);
+        }
+        for (int i = (kHeld * 256 + tid) * N; i < kp; i += 256 * N) {
+            float v[N];
+            i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, v);
+            i8_store_codes<N>(codes + t * kp + i, v, sc[t]);
+        }
     }
     __syncthreads();
     constexpr int NV = R * (T == 3 ? 4 : T);
@@ -579,6 +612,132 @@ template <class G> hipError_t i8_big_go(const I8Args &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// The same with the ring cut finer: five units of one operand's slice, so that
+// the channels, which come from memory, are copied two slices ahead and the
+// tokens, which other workgroups read as well, one.
+template <int WM_, int WN_, int MF_, int NF_> struct I8Wide {
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_;
+    static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * WM * WN;
+    static constexpr int kUnit = (BM > BN ? BM : BN) * 128, kLds = 5 * kUnit;
+    static constexpr int DW = (BM / 8 + WM * WN - 1) / (WM * WN), DX = (BN / 8 + WM * WN - 1) / (WM * WN);
+    static_assert(kLds <= 160 * 1024, "tile");
+};
+
+template <class G>
+__global__ __launch_bounds__(G::kThreads) void k_i8_wide(I8Args a, int n_ct, int n_tt) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int MF = G::MF, NF = G::NF, NW = G::WM * G::WN, DW = G::DW, DX = G::DX;
+    const int total = n_ct * n_tt, per = (total + 7) / 8;
+    const int L = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || L >= total) return;  // the whole workgroup
+    const int tt = L % n_tt, ct = L / n_tt;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wn = wv % G::WN, wm = wv / G::WN;
+    const int o0 = ct * G::BM, t0 = tt * G::BN, rb = a.row_bytes;
+
+    const int w_rows = min(G::BM, a.out_dim - o0), x_rows = min(G::BN, a.n_tok - t0);
+    const bl_rsrc rw = bl_make_rsrc(a.w + (size_t)o0 * rb, (uint32_t)w_rows * (uint32_t)rb);
+    const bl_rsrc rx = bl_make_rsrc(a.xq + (size_t)t0 * rb, (uint32_t)x_rows * (uint32_t)rb);
+    const uint32_t lds0 = bl_lds(smem);
+    // copy p of an operand: 8 rows; rows behind the last repeat it (their
+    // products are not stored)
+    uint32_t ow[DW], ox[DX];
+    auto at = [&](int p, int copies, int rows) {
+        const int row = 8 * min(wv + NW * p, copies - 1) + (lane >> 3);
+        return (uint32_t)min(row, rows - 1) * (uint32_t)rb + 16u * (uint32_t)((lane & 7) ^ i8_key(row));
+    };
+#pragma unroll
+    for (int p = 0; p < DW; p++) ow[p] = at(p, G::BM / 8, w_rows);
+#pragma unroll
+    for (int p = 0; p < DX; p++) ox[p] = at(p, G::BN / 8, x_rows);
+    const int n_sl = (rb + 127) / 128;
+    auto copy1 = [&](const bl_rsrc &r, uint32_t o, int copies, int i, int unit, int p) {
+        const int c = min(wv + NW * p, copies - 1);
+        o += 128u * (uint32_t)i;
+        if (128 * i + 128 > rb && ((lane & 7) ^ i8_key(8 * c + (lane >> 3))) >= 4) o = 0xFFFFFFF0u;
+        bl_dma16(bl_rsrc{r[0], r[1], i < n_sl ? r[2] : 0u, r[3]}, o, 0, lds0 + (uint32_t)(unit * G::kUnit + c * 1024));
+    };
+    auto copy_w = [&](int i, int unit, int p) { copy1(rw, ow[p], G::BM / 8, i, unit, p); };
+    auto copy_x = [&](int i, int unit, int p) { copy1(rx, ox[p], G::BN / 8, i, unit, p); };
+    i8_v4 acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[m][n] = i8_v4{0, 0, 0, 0};
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint8_t *const lw = smem + (wm * 16 * MF + r16) * 128;
+    const uint8_t *const lx = smem + (wn * 16 * NF + r16) * 128;
+    const int s0 = 16 * (q ^ i8_key(r16)), s1 = s0 ^ 64;
+    i8_v4 f[2][MF + NF];  // operands of a half slice: NF of tokens, MF of channels
+    auto read1 = [&](int h, int uw, int ux, int j) {
+        const int so = h ? s1 : s0;
+        f[h][j] = j < NF ? *reinterpret_cast<const i8_v4 *>(lx + j * 2048 + so + ux * G::kUnit)
+                         : *reinterpret_cast<const i8_v4 *>(lw + (j - NF) * 2048 + so + uw * G::kUnit);
+    };
+    // phase h: its MFMAs, the other half's next operands read from (uw, ux), and
+    // behind the barrier (h = 1) the copies of tokens i + 2 and channels i + 3
+    auto phase = [&](auto h_c, int uw, int ux, int i, int fx, int fw) __attribute__((always_inline)) {
+        constexpr int h = decltype(h_c)::value;
+#pragma unroll
+        for (int m = 0; m < MF; m++) {
+#pragma unroll
+            for (int j = m * (MF + NF) / MF; j < (m + 1) * (MF + NF) / MF; j++) read1(h ^ 1, uw, ux, j);
+            if constexpr (h == 1) {
+#pragma unroll
+                for (int p = m * (DW + DX) / MF; p < (m + 1) * (DW + DX) / MF; p++) {
+                    if (p < DX) copy_x(i + 2, fx, p);
+                    else copy_w(i + 3, fw, p - DX);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NF; n++)
+                acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h][NF + m], f[h][n], acc[m][n], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+#pragma unroll
+        for (int p = 0; p < DW; p++) copy_w(i, 2 * i, p);
+        if (i < 2) {
+#pragma unroll
+            for (int p = 0; p < DX; p++) copy_x(i, 2 * i + 1, p);
+        }
+    }
+    bl_barrier<2 * DW + DX>();
+#pragma unroll
+    for (int j = 0; j < MF + NF; j++) read1(0, 0, 1, j);
+    int uw = 0, ux = 1;
+    for (int i = 0; i < n_sl; i++) {
+        const int nw = uw >= 3 ? uw - 3 : uw + 2, nx = ux >= 3 ? ux - 3 : ux + 2;
+        phase(std::integral_constant<int, 0>{}, uw, ux, 0, 0, 0);
+        bl_barrier<DW>();
+        phase(std::integral_constant<int, 1>{}, nw, nx, i, uw, ux);
+        uw = nw;
+        ux = nx;
+    }
+    bl_wait<0>();  // (the copies past the last slice, zeros, land in the ring too)
+    const uint32_t esz = a.dtype_out == T_F32 ? 4u : 2u;
+    const bool vec = ((uintptr_t)a.out % (4 * esz)) == 0 && a.out_stride % 4 == 0 &&
+                     ((uintptr_t)a.wscale % 16) == 0 && ((uintptr_t)a.bias % 16) == 0;
+#pragma unroll
+    for (int n = 0; n < NF; n++)
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+            i8_finish(a, acc[m][n], o0 + 16 * (wm * MF + m) + 4 * q, t0 + 16 * (wn * NF + n) + r16, vec);
+}
+
+template <class G> hipError_t i8_wide_go(const I8Args &a, hipStream_t s) {
+    static const hipError_t attr = hipFuncSetAttribute(
+        reinterpret_cast<const void *>(&k_i8_wide<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+    if (attr != hipSuccess) return attr;
+    const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
+    const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
+    k_i8_wide<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 namespace {
@@ -660,6 +819,11 @@ constexpr I8Kernel i8_tile(int occ, float c0, float c1, float c2) {
     using G = I8Tile<WM, WN, WK, MF, NF, ST>;
     return {&i8_tile_go<G>, G::BM, G::BN, WK, occ, c0, c1, c2};
 }
+template <int WM, int WN, int MF, int NF>
+constexpr I8Kernel i8_wide(int occ, float c0, float c1, float c2) {
+    using G = I8Wide<WM, WN, MF, NF>;
+    return {&i8_wide_go<G>, G::BM, G::BN, 1, occ, c0, c1, c2};
+}
 template <int WM, int WN, int MF, int NF, int ST>
 constexpr I8Kernel i8_big(int occ, float c0, float c1, float c2) {
     using G = I8Big<WM, WN, MF, NF, ST>;
@@ -677,7 +841,8 @@ const I8Kernel kI8Kernels[] = {
     i8_big<4, 2, 3, 4, 3>(1, 0.0f, 5.14f, 0.562f),       // 192 x 128
     i8_big<2, 4, 8, 2, 3>(1, 0.0f, 6.81f, 0.696f),       // 256 x 128
     i8_big<2, 4, 6, 3, 3>(1, 0.0f, 6.48f, 0.727f),       // 192 x 192
-    i8_big<2, 4, 8, 4, 2>(1, 0.0f, 6.77f, 1.215f),       // 256 x 256
+    i8_wide<2, 4, 7, 4>(1, 0.0f, 6.4f, 1.08f),           // 224 x 256
+    i8_wide<2, 4, 8, 4>(1, 0.0f, 6.7f, 1.18f),           // 256 x 256
 };
 
 }  // namespace
