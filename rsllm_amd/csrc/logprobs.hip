@@ -19,7 +19,6 @@ namespace {
 constexpr float kInf = __builtin_inff();
 constexpr int kLpWaves = 4;         // wavefronts a workgroup
 constexpr int kLpTurn = 16 * 64 * kLpWaves;  // elements of a turn: 16 a lane
-constexpr int kLpNoId = -2147483647 - 1;
 
 __device__ __forceinline__ float lp_one(const void *p, size_t i, uint32_t dtype) {
     if (dtype == T_F32) return static_cast<const float *>(p)[i];
@@ -66,51 +65,45 @@ __device__ __forceinline__ LpSums lp_join(const LpSums &a, const LpSums &b) {
                   ra * (a.d + lp_floor(xa) * a.s) + rb * (b.d + lp_floor(xb) * b.s)};
 }
 
-// The best (value, id) seen by a wavefront, the i-th at lane i; -inf, kLpNoId
-// behind the last.
-struct LpTop {
-    float v;
-    int i;
+// A listed logit as one number: the value's place in the order of all floats
+// above the complement of its id, so that the larger comes before, and of equals
+// the lower id; 0: none. A wavefront's list stands in order, the i-th at lane i.
+struct LpKey {
+    uint32_t hi, lo;
+    __device__ __forceinline__ uint64_t n() const { return (uint64_t)hi << 32 | lo; }
 };
-__device__ __forceinline__ int lp_shift(int x) {  // lane l gets lane l - 1's
-    return __builtin_amdgcn_update_dpp(x, x, 0x138, 0xf, 0xf, false);  // wave_shr:1
+__device__ __forceinline__ LpKey lp_key(float v, int i) {
+    const int b = __builtin_bit_cast(int, v + 0.0f);  // (-0 and 0 are equal)
+    return LpKey{(uint32_t)b ^ ((uint32_t)(b >> 31) | 0x80000000u), ~(uint32_t)i};
 }
-__device__ __forceinline__ float lp_lane(float v, int l) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+__device__ __forceinline__ float lp_value(uint32_t hi) {
+    return __builtin_bit_cast(float, hi & 0x80000000u ? hi ^ 0x80000000u : ~hi);
 }
-// (av, ai) comes before (bv, bi): the larger, then the lower id.
-__device__ __forceinline__ bool lp_before(float av, int ai, float bv, int bi) {
-    return av > bv || (av == bv && ai < bi);
+template <int CTRL> __device__ __forceinline__ uint32_t lp_dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false);
 }
 // Lane l gets lane l ^ X's: within rows of 16 lanes by DPP, across by a shuffle.
-template <int X> __device__ __forceinline__ int lp_xor(int x) {
-    if constexpr (X == 1) return __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xf, 0xf, false);  // quad_perm
-    if constexpr (X == 2) return __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xf, 0xf, false);
-    if constexpr (X == 4) {  // ^ 7 (row_half_mirror), then ^ 3
-        const int y = __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false);
-        return __builtin_amdgcn_update_dpp(y, y, 0x1B, 0xf, 0xf, false);
-    }
-    if constexpr (X == 8) return __builtin_amdgcn_update_dpp(x, x, 0x128, 0xf, 0xf, false);  // row_ror:8
-    return __shfl_xor(x, X, 64);
+template <int X> __device__ __forceinline__ uint32_t lp_xor(uint32_t x) {
+    if constexpr (X == 1) return lp_dpp<0xB1>(x);                  // quad_perm
+    else if constexpr (X == 2) return lp_dpp<0x4E>(x);
+    else if constexpr (X == 4) return lp_dpp<0x1B>(lp_dpp<0x141>(x));  // row_half_mirror (^ 7), ^ 3
+    else if constexpr (X == 8) return lp_dpp<0x128>(x);            // row_ror:8
+    else return (uint32_t)__shfl_xor((int)x, X, 64);
 }
-// One step of a bitonic network: lanes l and l ^ X keep the one before at the
-// lane where `first` says so.
-template <int X> __device__ __forceinline__ void lp_step(LpTop &t, bool first) {
-    const float v = __builtin_bit_cast(float, lp_xor<X>(__builtin_bit_cast(int, t.v)));
-    const int i = lp_xor<X>(t.i);
-    if (lp_before(v, i, t.v, t.i) == first) {
-        t.v = v;
-        t.i = i;
-    }
+// One step of a bitonic network: of lanes l and l ^ X, those where `first` says
+// so keep the one that comes before.
+template <int X> __device__ __forceinline__ void lp_step(LpKey &t, bool first) {
+    const LpKey o{lp_xor<X>(t.hi), lp_xor<X>(t.lo)};
+    if ((o.n() > t.n()) == first) t = o;
 }
-// 64 lanes whose order rises and then falls (or the reverse), into order; down: the
-// first at lane 0 of each run of 2 X lanes.
-template <int X> __device__ __forceinline__ void lp_merge_from(LpTop &t, bool down) {
+// Runs of 2 X lanes that fall and then rise (or the reverse), into order: falling
+// where `down`.
+template <int X> __device__ __forceinline__ void lp_merge_from(LpKey &t, bool down) {
     const int lane = threadIdx.x & 63;
     lp_step<X>(t, ((lane & X) == 0) == down);
     if constexpr (X > 1) lp_merge_from<X / 2>(t, down);
 }
-__device__ __forceinline__ void lp_sort(LpTop &t) {
+__device__ __forceinline__ void lp_sort(LpKey &t) {
     const int lane = threadIdx.x & 63;
     lp_merge_from<1>(t, (lane & 2) == 0);
     lp_merge_from<2>(t, (lane & 4) == 0);
@@ -120,59 +113,50 @@ __device__ __forceinline__ void lp_sort(LpTop &t) {
     lp_merge_from<32>(t, true);
 }
 // The 64 best of two lists in order: the better of a's i-th and b's 63 - i-th
-// falls and rises once.
-__device__ __forceinline__ void lp_merge(LpTop &top, const LpTop &o) {
-    const float v = __builtin_bit_cast(float, lp_xor<63>(__builtin_bit_cast(int, o.v)));
-    const int i = lp_xor<63>(o.i);
-    if (lp_before(v, i, top.v, top.i)) {
-        top.v = v;
-        top.i = i;
-    }
+// fall and rise once.
+__device__ __forceinline__ void lp_merge(LpKey &top, const LpKey &b) {
+    const LpKey o{lp_xor<63>(b.hi), lp_xor<63>(b.lo)};
+    if (o.n() > top.n()) top = o;
     lp_merge_from<32>(top, true);
 }
 
 // A wavefront's list and its n-th (uniform).
 struct LpList {
-    LpTop top{-kInf, kLpNoId};
-    float edge_v = -kInf;
-    int edge_i = kLpNoId;
-    __device__ __forceinline__ void edge(int n) {
-        edge_v = lp_lane(top.v, n - 1);
-        edge_i = __builtin_amdgcn_readlane(top.i, n - 1);
+    LpKey top{0, 0}, edge{0, 0};
+    __device__ __forceinline__ void set_edge(int n) {
+        edge.hi = (uint32_t)__builtin_amdgcn_readlane((int)top.hi, n - 1);
+        edge.lo = (uint32_t)__builtin_amdgcn_readlane((int)top.lo, n - 1);
     }
     // Takes every lane's candidate that is among the n best, and says whether
     // there was one: a few one by one, more of them sorted (kSorted: they come so)
-    // and merged. An insertion is some 25 dependent instructions, a sort 21 steps
-    // of 8 and a merge 7.
-    template <bool kSorted> __device__ __forceinline__ bool take(int n, float v, int i) {
+    // and merged.
+    template <bool kSorted> __device__ __forceinline__ bool take(int n, const LpKey &c) {
         const int lane = threadIdx.x & 63;
-        bool beats = lp_before(v, i, edge_v, edge_i);
+        const bool beats = c.n() > edge.n();
         unsigned long long todo = __ballot(beats);
         if (!todo) return false;
-        if (__popcll(todo) > (kSorted ? 3 : 10)) {
-            LpTop o{beats ? v : -kInf, beats ? i : kLpNoId};
-            if (!kSorted) lp_sort(o);
-            lp_merge(top, o);
-            edge(n);
+        if (__popcll(todo) > (kSorted ? 3 : 8)) {
+            if (!kSorted && edge.n() == 0 && __ballot(top.n() != 0) == 0) {
+                top = c;  // the first candidates
+                lp_sort(top);
+            } else {
+                LpKey o{beats ? c.hi : 0, beats ? c.lo : 0};
+                if (!kSorted) lp_sort(o);
+                lp_merge(top, o);
+            }
+            set_edge(n);
             return true;
         }
         do {
             const int who = __ffsll(todo) - 1;
             todo &= todo - 1;
-            const float cv = lp_lane(v, who);
-            const int ci = __builtin_amdgcn_readlane(i, who);
-            const int at = __popcll(__ballot(lp_before(top.v, top.i, cv, ci)));
-            const float pv = __builtin_bit_cast(float, lp_shift(__builtin_bit_cast(int, top.v)));
-            const int pi = lp_shift(top.i);
-            if (lane > at) {
-                top.v = pv;
-                top.i = pi;
-            } else if (lane == at) {
-                top.v = cv;
-                top.i = ci;
-            }
-            edge(n);
-            todo &= __ballot(lp_before(v, i, edge_v, edge_i));
+            const LpKey w{(uint32_t)__builtin_amdgcn_readlane((int)c.hi, who),
+                          (uint32_t)__builtin_amdgcn_readlane((int)c.lo, who)};
+            const int at = __popcll(__ballot(top.n() > w.n()));
+            const LpKey prev{lp_dpp<0x138>(top.hi), lp_dpp<0x138>(top.lo)};  // wave_shr:1
+            top = lane < at ? top : lane == at ? w : prev;
+            set_edge(n);
+            todo &= __ballot(c.n() > edge.n());
         } while (todo);
         return true;
     }
@@ -196,7 +180,7 @@ __device__ __forceinline__ LpPart lp_wave_join(LpPart p) {
 }
 
 // A row's outputs, by one wavefront that holds its sums and list.
-__device__ __forceinline__ void lp_finish(const LogprobArgs &a, int t, const LpPart &p, const LpTop &top) {
+__device__ __forceinline__ void lp_finish(const LogprobArgs &a, int t, const LpPart &p, const LpKey &top) {
     const int lane = threadIdx.x & 63;
     const float m = p.sums.m, nan = __builtin_nanf("");
     const bool bad = p.sums.s != p.sums.s, empty = m == -kInf;
@@ -216,8 +200,8 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs &a, int t, const LpP
     }
     if (lane < a.n_top) {
         const size_t at = (size_t)t * a.n_top + lane;
-        a.top_ids[at] = top.v > -kInf ? top.i : -1;
-        a.top_logprobs[at] = top.v > -kInf ? logprob(top.v) : bad ? nan : -kInf;
+        a.top_ids[at] = top.hi ? (int)~top.lo : -1;
+        a.top_logprobs[at] = top.hi ? logprob(lp_value(top.hi)) : bad ? nan : -kInf;
     }
 }
 
@@ -226,7 +210,7 @@ __device__ __forceinline__ void lp_finish(const LogprobArgs &a, int t, const LpP
 // Where the parts of a row lie in the caller's workspace.
 struct LpWork {
     LpPart *parts;  // [n_tok x chunks]
-    LpTop *tops;    // [n_tok x chunks x n_top]
+    LpKey *tops;    // [n_tok x chunks x n_top]
 };
 
 // Workgroup (chunk, row): `turns` turns, each kLpWaves * L pieces of 64 lanes x
@@ -238,7 +222,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
     using V = LpVec<DT>;
     constexpr int N = V::N, L = V::L, M = N * L;
     __shared__ LpPart part[kLpWaves];
-    __shared__ LpTop list[kLpWaves][64];
+    __shared__ LpKey list[kLpWaves][64];
     const int t = blockIdx.x / chunks, c = blockIdx.x - t * chunks;
     const int lane = threadIdx.x & 63;
     const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -252,6 +236,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
     LpSums sum{-kInf, 0.0f, 0.0f};
     int above = 0;
     LpList best;
+    float edge_v = -kInf;
 
     const int pieces = turns * (kLpWaves * L);
     const int all = (int)(((long long)head + a.vocab + 64 * N - 1) / (64 * N));
@@ -304,9 +289,13 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
             sum.s = r * sum.s + s;
             sum.m = m;
         }
-        if (a.n_top && __ballot(big >= best.edge_v && big > -kInf)) {
+        // (edge_v: the list's n-th value, -inf before there is one)
+        if (a.n_top && __ballot(big >= edge_v && big > -kInf)) {
             const int i0 = (int)(e0 + N * lane);
-            if (best.edge_v == -kInf) {
+            auto key = [&](float l, int j) {
+                return l > -kInf ? lp_key(l, i0 + j / N * (64 * N) + j % N) : LpKey{0, 0};
+            };
+            if (best.edge.hi == 0) {
                 // the first turns: every lane's largest first, which leaves
                 // little of the rest to take
                 int at = 0;
@@ -316,18 +305,22 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
                     at = v[j] > one ? j : at;
                     one = fmaxf(one, v[j]);
                 }
-                best.take<false>(a.n_top, one, i0 + at / N * (64 * N) + at % N);
+                best.take<false>(a.n_top, key(one, at));
 #pragma unroll
                 for (int j = 0; j < M; j++) v[j] = j == at ? -kInf : v[j];
+                edge_v = best.edge.hi ? lp_value(best.edge.hi) : -kInf;
             }
 #pragma unroll
             for (int j = 0; j < M; j++)
-                best.take<false>(a.n_top, v[j], i0 + j / N * (64 * N) + j % N);
+                if (__ballot(v[j] >= edge_v)) {
+                    best.take<false>(a.n_top, key(v[j], j));
+                    edge_v = best.edge.hi ? lp_value(best.edge.hi) : -kInf;
+                }
         }
     }
     const LpPart mypart = lp_wave_join(LpPart{sum, above});
     if (lane == 0) part[wv] = mypart;
-    if (a.n_top) list[wv][lane] = lane < a.n_top ? best.top : LpTop{-kInf, kLpNoId};
+    if (a.n_top) list[wv][lane] = lane < a.n_top ? best.top : LpKey{0, 0};
     __syncthreads();
     if (wv != 0) return;
     LpPart all_part = part[0];
@@ -336,8 +329,7 @@ __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWor
         all_part.sums = lp_join(all_part.sums, part[k].sums);
         all_part.above += part[k].above;
         if (a.n_top) {
-            const LpTop o = list[k][lane];
-            best.take<true>(a.n_top, o.v, o.i);
+            best.take<true>(a.n_top, list[k][lane]);
         }
     }
     if (chunks == 1) {
@@ -365,12 +357,12 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, LpWork w, i
     LpList best;
     for (int c0 = 0; c0 < chunks && a.n_top; c0 += 64) {
         const bool in = c0 + lane < chunks;
-        const LpTop *src = w.tops + (at + min(c0 + lane, chunks - 1)) * a.n_top;
-        LpTop next = src[0];
+        const LpKey *src = w.tops + (at + min(c0 + lane, chunks - 1)) * a.n_top;
+        LpKey next = src[0];
         for (int r = 0; r < a.n_top; r++) {
-            const LpTop o = next;
+            const LpKey o = next;
             next = src[min(r + 1, a.n_top - 1)];
-            if (!best.take<false>(a.n_top, in ? o.v : -kInf, in ? o.i : kLpNoId)) break;
+            if (!best.take<false>(a.n_top, in ? o : LpKey{0, 0})) break;
         }
     }
     lp_finish(a, t, p, best.top);
@@ -400,7 +392,7 @@ size_t logprobs_scratch_bytes(int n_tok, int vocab, int n_top) {
     const LpPlan p = lp_plan(n_tok, vocab);
     if (p.chunks == 1 || n_tok == 0) return 0;
     const size_t n = (size_t)n_tok * p.chunks;
-    return lp_round(n * sizeof(LpPart)) + lp_round(n * n_top * sizeof(LpTop));
+    return lp_round(n * sizeof(LpPart)) + lp_round(n * n_top * sizeof(LpKey));
 }
 
 hipError_t launch_logprobs(const LogprobArgs &a, uint8_t *work, int n_tok, hipStream_t s) {
@@ -409,7 +401,7 @@ hipError_t launch_logprobs(const LogprobArgs &a, uint8_t *work, int n_tok, hipSt
     LpWork w{};
     if (p.chunks > 1) {
         w.parts = reinterpret_cast<LpPart *>(work);
-        w.tops = reinterpret_cast<LpTop *>(work + lp_round((size_t)n_tok * p.chunks * sizeof(LpPart)));
+        w.tops = reinterpret_cast<LpKey *>(work + lp_round((size_t)n_tok * p.chunks * sizeof(LpPart)));
     }
     const long long wgs = (long long)n_tok * p.chunks;
     if (wgs > 0x7FFFFFFFll) return hipErrorInvalidValue;
