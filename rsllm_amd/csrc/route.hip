@@ -20,17 +20,63 @@ __device__ __forceinline__ float route_load(const void *p, size_t i, uint32_t dt
     return (dtype == T_F16 ? f16_to_f32(b) : __builtin_bit_cast(float, (uint32_t)b << 16)) + 0.0f;
 }
 
+// exp(x) to some 2^-52: x = n log 2 + r, |r| < 0.35, and the power series of exp(r)
+// up to r^12 / 12!, after Cody and Waite's reduction. (Short, where the library's is long: most calls of these
+// kernels pay for fetching their code.)
+__device__ __forceinline__ double route_exp64(double x) {
+    x = fmin(fmax(x, -1000.0), 1000.0);
+    const double n = rint(x * 0x1.71547652b82fep+0);  // log2 e
+    // log 2 in two parts, the first of few enough bits that n times it is exact
+    const double r = fma(n, -0x1.7f7d1cf79abcap-20, fma(n, -0x1.62e4p-1, x));
+    double p = 1.0 / 479001600.0;
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+// log(1 + e), 0 <= e <= 1: 2 atanh(z), z = e / (2 + e) <= 1/3, to z^33.
+__device__ __forceinline__ double route_log1p(double e) {
+    const double z = e / (2.0 + e), q = z * z;
+    double p = 2.0 / 33.0;
+    p = fma(p, q, 2.0 / 31.0);
+    p = fma(p, q, 2.0 / 29.0);
+    p = fma(p, q, 2.0 / 27.0);
+    p = fma(p, q, 2.0 / 25.0);
+    p = fma(p, q, 2.0 / 23.0);
+    p = fma(p, q, 2.0 / 21.0);
+    p = fma(p, q, 2.0 / 19.0);
+    p = fma(p, q, 2.0 / 17.0);
+    p = fma(p, q, 2.0 / 15.0);
+    p = fma(p, q, 2.0 / 13.0);
+    p = fma(p, q, 2.0 / 11.0);
+    p = fma(p, q, 2.0 / 9.0);
+    p = fma(p, q, 2.0 / 7.0);
+    p = fma(p, q, 2.0 / 5.0);
+    p = fma(p, q, 2.0 / 3.0);
+    p = fma(p, q, 2.0);
+    return p * z;
+}
+
 // exp(l - m) with m the largest logit: the limit where both are +inf.
 __device__ __forceinline__ double route_exp(float l, float m) {
-    return l == m ? 1.0 : exp((double)l - (double)m);
+    return l == m ? 1.0 : route_exp64((double)l - (double)m);
 }
 
 // The score of logit l; softmax: m the row's largest logit, sum its total.
 __device__ __forceinline__ double route_score(float l, int score, float m, double sum) {
     if (score == ROUTE_SOFTMAX) return route_exp(l, m) / sum;
-    if (score == ROUTE_SIGMOID) return 1.0 / (1.0 + exp(-(double)l));
-    const double x = (double)l;
-    return sqrt((x > 0.0 ? x : 0.0) + log1p(exp(-fabs(x))));
+    const double x = (double)l, e = route_exp64(score == ROUTE_SIGMOID ? -x : -fabs(x));
+    if (score == ROUTE_SIGMOID) return 1.0 / (1.0 + e);
+    return sqrt(fmax(x, 0.0) + route_log1p(e));
 }
 
 constexpr double kNever = -__builtin_inf();  // an expert that is not to be chosen
@@ -175,240 +221,554 @@ __global__ __launch_bounds__(256) void k_route_any(RouteArgs a) {
 
 namespace {
 
-// ---- one wavefront per token -----------------------------------------------
+// ---- W lanes per token --------------------------------------------------------
 //
-// Lane l holds R neighbouring experts of group l / LG (LG lanes a group), so
-// lanes, and a lane's own places, stand in the order of the ids. The choice is
-// made in f32 and certain wherever two neighbours in the order are further apart
-// than twice what f32 can be off (kRouteOff relative to the larger, or to 1), or
-// have the same logit and bias; a token with another close pair goes
-// through the same steps in 64 bits. 256 experts with biases of 0.05: about 1
-// token in 300 does.
+// Lane l of a token's W holds R neighbouring experts of group l / LG (LG lanes a
+// group), so lanes, and a lane's own places, stand in the order of the ids. A
+// lane keeps the three best of its R at hand; every round takes the best of the W
+// lanes' first ones, and only a lane that gave three looks through its R again.
+// The choice is made in f32. Which of two keys is larger is certain there when
+// they are further apart than f32 can be off (route_apart). The chosen experts'
+// scores are wanted in 64 bits for the weights anyhow: where two neighbours among
+// them are close, those settle their order. Where the last chosen is close to one
+// left out, or a kept group to one left out, and they are not the same logit and
+// bias, the token's choice is made again in 64 bits (256 experts, biases of 0.05:
+// about 1 token in 5000).
+// Several tokens a wavefront share its instructions, and the best of 16 lanes is
+// four steps within a DPP row; more experts a lane cost more looks through them.
 
-// How far an f32 key may be off, relative to max(1, |key|). exp(x) from v_exp_f32
-// is (|x| + 3) 2^-24 off; sigmoid'(x) |x| < 1/4 and exp(x) |x| < 0.4, so the two
-// scores within [0, 1] are within 2^-21 (the softmax's sum adds 16 roundings);
-// sqrt(log(1 + e)) with e >= 0.01 (below it a series) halves the relative error
-// of a logarithm that is within 2^-22 absolute, and is at least 0.1: 2^-19.7.
-constexpr float kRouteOff = 0x1p-19f;
-
-// The largest of 64 lanes' values, at every lane (uniform).
-__device__ __forceinline__ float route_wave_max(float v) {
-    auto step = [](float x, auto ctrl, auto rows) {
-        const int lo = __builtin_bit_cast(int, -__builtin_inff());
-        return fmaxf(x, __builtin_bit_cast(
-                            float, __builtin_amdgcn_update_dpp(lo, __builtin_bit_cast(int, x),
-                                                               decltype(ctrl)::value,
-                                                               decltype(rows)::value, 0xf, false)));
-    };
-    using std::integral_constant;
-    v = step(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1
-    v = step(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
-    v = step(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
-    v = step(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
-    v = step(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15
-    v = step(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+// A float's place in the order of all floats as a number (no NaN); 0, below that of
+// -inf: none.
+__device__ __forceinline__ uint32_t route_order(float v) {
+    const int b = __builtin_bit_cast(int, v);
+    return (uint32_t)b ^ ((uint32_t)(b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ double route_wave_max(double v) {
+__device__ __forceinline__ float route_value(uint32_t o) {
+    return __builtin_bit_cast(float, o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+// The largest of a token's W lanes' values, at each of them: rotations within the
+// DPP rows of 16 lanes, then rows exchanged.
+template <int W> __device__ __forceinline__ uint32_t route_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true));  // row_ror:8
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, true));
+    if constexpr (W >= 32) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max((uint32_t)s[0], (uint32_t)s[1]);
+    }
+    if constexpr (W >= 64) {
+        const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max((uint32_t)s[0], (uint32_t)s[1]);
+    }
+    return v;
+}
+// The first of a token's W lanes (0..W - 1) where `yes`, W or more if none.
+template <int W> __device__ __forceinline__ int route_first(bool yes) {
+    const unsigned long long all = __ballot(yes);
+    const int lane = threadIdx.x & 63;
+    if constexpr (W == 64) return all ? __ffsll(all) - 1 : 64;
+    uint32_t half = lane < 32 ? (uint32_t)all : (uint32_t)(all >> 32);
+    if constexpr (W == 16) half = lane & 16 ? half >> 16 : half & 0xFFFFu;
+    return half ? __ffs((int)half) - 1 : 64;
+}
+template <int W> __device__ __forceinline__ double route_sum(double v) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = fmax(v, __shfl_xor(v, off, 64));
+    for (int off = W / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
     return v;
 }
 
 __device__ __forceinline__ float route_score32(float l, int score, float m, float inv) {
     if (score == ROUTE_SOFTMAX) return (l == m ? 1.0f : __expf(l - m)) * inv;
     if (score == ROUTE_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + __expf(-l));
-    const float e = __expf(-fabsf(l));
-    const float g = e < 0.01f ? e * (1.0f - e * (0.5f - e * (1.0f / 3.0f))) : __logf(1.0f + e);
+    // log(1 + e) with what the sum 1 + e lost put back
+    const float e = __expf(-fabsf(l)), u = 1.0f + e;
+    const float g = e < 0.01f ? e * (1.0f - e * (0.5f - e * (1.0f / 3.0f)))
+                              : __logf(u) + (e - (u - 1.0f)) * __builtin_amdgcn_rcpf(u);
     return __builtin_amdgcn_sqrtf(fmaxf(l, 0.0f) + g);
 }
 
-// Whether a before b is certain in f32.
-__device__ __forceinline__ bool route_apart(float a, float b) {
-    return a - b > 2.0f * kRouteOff * fmaxf(1.0f, fmaxf(fabsf(a), fabsf(b)));
+// Whether f32 keys a >= b are certainly in that order. With u = 2^-24, exp(x) from
+// v_exp_f32 is (|x| + 2) u off (the product with log2 e, the instruction's step).
+//   sigmoid: s (1 - s) (|x| + 2) u < 0.73 u, and 3 u for 1 + e and v_rcp_f32
+//   sqrt(log(1 + e) + max(l, 0)): 1 + e is made good, so the logarithm is within
+//     (|l| + 5) u relative, its root within half of that and 2 u: s |l| < 1 where
+//     l < 0, so 5 u for s < 1, and 5 u relative above
+//   softmax: s <= 1 / S, and relative (|x| + 2) u, and 31 u for S (22 additions
+//     one after the other, its terms' own) and its inverse: 36 u / S
+// and the sum with the bias u relative. off: twice that and some more, for the two,
+// of the token's largest score (from its largest logit).
+__device__ __forceinline__ bool route_apart(float a, float b, float off) {
+    return a - b > off + 0x1p-22f * fmaxf(fabsf(a), fabsf(b));
+}
+__device__ __forceinline__ float route_off(int score, float top, float inv) {
+    if (score == ROUTE_SOFTMAX) return 0x1.4p-18f * inv;
+    if (score == ROUTE_SIGMOID) return 0x1p-21f;
+    return 0x1.8p-21f * fmaxf(1.0f, sqrtf(top + 0.7f));
 }
 
-// Lane `lane` of a token's wavefront: the R experts from id `first` on, live
-// where they exist and can be chosen.
+// Lane `sub` of a token's: the R experts from id `first` on, logits -inf where
+// there is none or it cannot be chosen.
 template <int R> struct RouteLane {
-    float l[R];  // logits; -inf where there is nothing to choose
+    float l[R], b[R];  // logits and biases
     int first;
 };
 
-// The k best of the token in the order of the keys (T: float or double; norm:
-// the softmax's divisor, or its inverse in float), lane i getting the i-th's id,
-// -1 behind the last. False where T cannot tell.
-template <class T, int R>
-__device__ __forceinline__ bool route_choose(const RouteArgs &a, size_t row, const RouteLane<R> &x,
-                                             int LG, float m, T norm, int &id) {
-    constexpr bool kFast = sizeof(T) == 4;
-    const int lane = threadIdx.x & 63;
-    const T never = -(T)__builtin_inff();
-    T key[R], place[R];
+// What the host works out of a call's sizes.
+struct RouteForm {
+    int per, LG;  // experts a group, lanes a group
+    int whole;    // every lane holds R experts, at 16-byte aligned addresses
+};
+// A token's chosen experts in LDS: id and f32 key (as route_order), the r-th at [r].
+struct RoutePick {
+    int id;
+    uint32_t key;
+};
+
+// The k best of each of the wavefront's tokens by their f32 keys (inv: the inverse of
+// the softmax's divisor; off: route_off) to `pick`, id -1 behind the last. False at the tokens where
+// f32 cannot tell which they are.
+template <int W, int R>
+__device__ __forceinline__ bool route_choose(const RouteArgs &a, const RouteForm &f, const RouteLane<R> &x,
+                                             int g, float m, float inv, float off, RoutePick *pick) {
+    const int lane = threadIdx.x & 63, sub = lane % W;
+    const float none = -__builtin_inff();
+    bool sure = true;
+    uint32_t place[R];
 #pragma unroll
-    for (int j = 0; j < R; j++) {
-        key[j] = never;
-        if (x.l[j] > -__builtin_inff()) {
-            if (a.bias || a.n_group > 1) {
-                if constexpr (kFast) key[j] = route_score32(x.l[j], a.score, m, norm);
-                else key[j] = route_score(x.l[j], a.score, m, norm);
-                if (a.bias) key[j] += (T)a.bias[x.first + j];
-                key[j] = key[j] > never ? key[j] : never;  // (a NaN is not)
-            }
-        }
-        place[j] = a.bias ? key[j] : (T)x.l[j];
-    }
-    if (a.n_group > 1) {
-        // the lane's two best keys, then those of the group at its first lane:
-        // every step adds the lanes behind those gathered so far
-        T b0 = never, b1 = never;
+    for (int j = 0; j < R; j++) place[j] = x.l[j] > none ? route_order(x.l[j]) : 0;
+    if (a.bias || a.n_group > 1) {
+        uint32_t key[R];
 #pragma unroll
         for (int j = 0; j < R; j++) {
-            b1 = key[j] > b0 ? b0 : key[j] > b1 ? key[j] : b1;
-            b0 = key[j] > b0 ? key[j] : b0;
+            const float s = route_score32(x.l[j], a.score, m, inv) + (a.bias ? x.b[j] : 0.0f);
+            // (+ 0.0: keys of -0; a NaN is not chosen)
+            key[j] = place[j] && s > none ? route_order(s + 0.0f) : 0;
+            place[j] = a.bias ? key[j] : place[j];
         }
-        const int in_group = lane % LG;
-        for (int off = 1; off < LG; off <<= 1) {
-            const T c0 = __shfl_down(b0, off, 64), c1 = __shfl_down(b1, off, 64);
-            if (in_group + off < LG) {
-                const T lo = b0 < c0 ? b0 : c0, hi = b1 > c1 ? b1 : c1;
-                b0 = b0 > c0 ? b0 : c0;
-                b1 = lo > hi ? lo : hi;
+        if (a.n_group > 1) {
+            // the lane's two best keys, then those of the group at its first
+            // lane: every step adds the lanes behind those gathered so far
+            uint32_t b0 = 0, b1 = 0;
+#pragma unroll
+            for (int j = 0; j < R; j++) {
+                b1 = max(b1, min(key[j], b0));
+                b0 = max(b0, key[j]);
             }
-        }
-        const bool head = in_group == 0 && lane < LG * a.n_group;
-        T sum = !head ? never : a.group_top == 2 && b1 > never ? b0 + b1 : b0;
-        unsigned long long kept = 0;
-        T last = never;
-        for (int r = 0; r < a.topk_group; r++) {
-            const T best = route_wave_max(sum);
-            if (!(best > never)) break;
-            const int who = __ffsll(__ballot(sum == best)) - 1;
-            kept |= 1ull << who;
-            last = best;
-            if (lane == who) sum = never;
-        }
-        if constexpr (kFast) {
-            const T next = route_wave_max(sum);
-            // (half the gap: sums of two)
-            if (next > never && !route_apart(0.5f * last, 0.5f * next)) return false;
-        }
-        if (!(kept >> (lane - in_group) & 1)) {
-#pragma unroll
-            for (int j = 0; j < R; j++) place[j] = never;
-        }
-    }
-    id = -1;
-    T last = never;
-    int last_id = 0;
-    const int rounds = kFast && a.bias ? a.k + 1 : a.k;  // the last against the next
-    for (int r = 0; r < rounds; r++) {
-        T top = place[0];
-        int at = 0;
-#pragma unroll
-        for (int j = 1; j < R; j++) {
-            at = place[j] > top ? j : at;
-            top = place[j] > top ? place[j] : top;
-        }
-        const T best = route_wave_max(top);
-        if (!(best > never)) break;
-        const int who = __ffsll(__ballot(top == best)) - 1;
-        const int won = __builtin_amdgcn_readlane(x.first + at, who);
-        if constexpr (kFast) {
-            // whatever is near the one before has to be its equal in 64 bits
-            // too: the same logit and bias
-            if (a.bias && r > 0 && !route_apart(last, best)) {
-                const float l = route_load(a.logits, row + last_id, a.dtype), b = a.bias[last_id];
-                bool unsure = false;
+            const int head = g * f.LG, in_group = sub - head;
+            for (int d = 1; d < f.LG; d <<= 1) {
+                const uint32_t c0 = (uint32_t)__shfl_down((int)b0, d, 64), c1 = (uint32_t)__shfl_down((int)b1, d, 64);
+                if (in_group + d < f.LG) {
+                    b1 = max(max(b1, c1), min(b0, c0));
+                    b0 = max(b0, c0);
+                }
+            }
+            uint32_t sum = a.group_top == 2 && b1 ? route_order(route_value(b0) + route_value(b1) + 0.0f) : b0;
+            if (in_group != 0 || g >= a.n_group) sum = 0;
+            uint32_t last = 0;
+            bool kept = false;
+            for (int r = 0; r < a.topk_group; r++) {
+                const uint32_t best = route_max<W>(sum);
+                const int who = route_first<W>(sum == best && best != 0);
+                kept |= who == head;
+                last = best ? best : last;
+                if (who == sub) sum = 0;
+            }
+            // the last kept against the best one left out (half the gap: sums of two)
+            const uint32_t next = route_max<W>(sum);
+            const bool near = next && !route_apart(0.5f * route_value(last), 0.5f * route_value(next), off);
+            if (__ballot(near)) {
+                // groups of one key each are equal where the logits and biases are
+                bool unsure = near && a.group_top == 2;
+                uint32_t l = 0, b = 0;
 #pragma unroll
                 for (int j = 0; j < R; j++)
-                    if (place[j] > never && !route_apart(last, place[j]))
-                        unsure |= !(x.l[j] == l && a.bias[x.first + j] == b);
-                if (__ballot(unsure)) return false;
+                    if (key[j] == last) {
+                        l = max(l, route_order(x.l[j]));
+                        b = max(b, a.bias ? route_order(x.b[j]) : 1u);
+                    }
+                l = route_max<W>(l);
+                b = route_max<W>(b);
+#pragma unroll
+                for (int j = 0; j < R; j++)
+                    if (near && key[j] && !route_apart(route_value(max(key[j], last)), route_value(min(key[j], last)), off))
+                        unsure |= !(route_order(x.l[j]) == l && (!a.bias || route_order(x.b[j]) == b));
+                sure = route_first<W>(unsure) >= W;
+            }
+#pragma unroll
+            for (int j = 0; j < R; j++) place[j] = kept ? place[j] : 0;
+        }
+    }
+    uint32_t h0, h1, h2;
+    int a0, a1, a2;
+    // the lane's three best of those below `under`, and behind j = from of those
+    // that equal it
+    auto scan = [&](uint32_t under, int from) __attribute__((always_inline)) {
+        h0 = h1 = h2 = 0;
+        a0 = a1 = a2 = 0;
+#pragma unroll
+        for (int j = 0; j < R; j++) {
+            const uint32_t v = place[j] < under || (place[j] == under && j > from) ? place[j] : 0;
+            const bool g0 = v > h0, g1 = v > h1, g2 = v > h2;
+            h2 = g1 ? h1 : g2 ? v : h2;
+            a2 = g1 ? a1 : g2 ? j : a2;
+            h1 = g0 ? h0 : g1 ? v : h1;
+            a1 = g0 ? a0 : g1 ? j : a1;
+            h0 = g0 ? v : h0;
+            a0 = g0 ? j : a0;
+        }
+    };
+    scan(0xFFFFFFFFu, -1);
+    for (int r = sub; r < a.k; r += W) pick[r] = RoutePick{-1, 0};
+    __builtin_amdgcn_wave_barrier();
+    int gave = 0;
+    uint32_t last = 0;
+    for (int r = 0; r < a.k; r++) {
+        const uint32_t best = route_max<W>(h0);
+        const int who = route_first<W>(h0 == best && best != 0);
+        last = best ? best : last;
+        const int from = a0;
+        if (who == sub) {
+            pick[r] = RoutePick{x.first + a0, best};
+            gave++;
+            h0 = h1;
+            a0 = a1;
+            h1 = h2;
+            a1 = a2;
+            h2 = 0;
+        }
+        if (R > 3 && __ballot(gave == 3)) {
+            const uint32_t k0 = h0, k1 = h1, k2 = h2;
+            const int i0 = a0, i1 = a1, i2 = a2;
+            scan(best, from);  // what comes after the one it just gave
+            if (gave == 3) {
+                gave = 0;
+            } else {
+                h0 = k0; h1 = k1; h2 = k2;
+                a0 = i0; a1 = i1; a2 = i2;
             }
         }
-        if (lane == r && r < a.k) id = won;
-        if (lane == who) {
+    }
+    if (a.bias) {
+        // the last chosen against the best one left out
+        const uint32_t next = route_max<W>(h0);
+        const bool near = next && !route_apart(route_value(last), route_value(next), off);
+        if (__ballot(near)) {
+            // chosen or not, whatever is close to the last chosen has to be its
+            // equal: the same logit and bias
+            bool unsure = false;
+            uint32_t l = 0, b = 0;
 #pragma unroll
             for (int j = 0; j < R; j++)
-                if (j == at) place[j] = never;
-        }
-        last = best;
-        last_id = won;
-    }
-    return true;
-}
-
-__device__ __forceinline__ double route_wave_sum(double v) {
+                if (place[j] == last) {
+                    l = max(l, route_order(x.l[j]));
+                    b = max(b, route_order(x.b[j]));
+                }
+            l = route_max<W>(l);
+            b = route_max<W>(b);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+            for (int j = 0; j < R; j++)
+                if (near && place[j] && !route_apart(route_value(max(place[j], last)), route_value(min(place[j], last)), off))
+                    unsure |= !(route_order(x.l[j]) == l && route_order(x.b[j]) == b);
+            sure = sure && route_first<W>(unsure) >= W;
+        }
+    }
+    return sure;
 }
 
-template <int R, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_route_wave(RouteArgs a, int n_tok, int LG) {
-    const int lane = threadIdx.x & 63;
-    const int t = blockIdx.x * WAVES + (int)(threadIdx.x >> 6);
-    if (t >= n_tok) return;  // the whole wavefront; no barriers
+// A double's place in the order of all doubles (no NaN).
+__device__ __forceinline__ uint64_t route_order64(double v) {
+    const long long b = __builtin_bit_cast(long long, v + 0.0);
+    return (uint64_t)b ^ ((uint64_t)(b >> 63) | 0x8000000000000000ull);
+}
+
+// One token's choice in 64 bits by a whole wavefront, the r-th's id at lane r. Rarely
+// run, so its code is kept short: what it costs is fetching it. keys, gsum: LDS for
+// n_expert and n_group values; keys are kept as places in the order, 0 for an
+// expert that is not to be chosen.
+__device__ __forceinline__ int route_exact(const RouteArgs &a, size_t row, double *keys, double *gsum) {
+    const int lane = threadIdx.x & 63, per = a.n_expert / a.n_group;
+    float m = -__builtin_inff();
+    double sum = 0.0;
+    if (a.score == ROUTE_SOFTMAX) {
+#pragma unroll 1
+        for (int e = lane; e < a.n_expert; e += 64) {
+            const float l = route_load(a.logits, row + e, a.dtype);
+            m = l > m ? l : m;
+        }
+        m = route_value(route_max<64>(route_order(m)));
+#pragma unroll 1
+        for (int e = lane; e < a.n_expert; e += 64) {
+            const float l = route_load(a.logits, row + e, a.dtype);
+            if (l > -__builtin_inff()) sum += route_exp(l, m);
+        }
+        sum = route_sum<64>(sum);
+    }
+#pragma unroll 1
+    for (int e = lane; e < a.n_expert; e += 64) {
+        const float l = route_load(a.logits, row + e, a.dtype);
+        double k = kNever;
+        if (l > -__builtin_inff()) {
+            k = route_score(l, a.score, m, sum) + (a.bias ? (double)a.bias[e] : 0.0);
+            k = k > kNever ? k : kNever;
+        }
+        keys[e] = k;
+    }
+    __syncthreads();  // (one wavefront a workgroup)
+    if (a.n_group > 1) {
+        // (at most 64 groups, a lane each)
+        double b0 = kNever, b1 = kNever;
+        if (lane < a.n_group) {
+#pragma unroll 4
+            for (int e = lane * per; e < (lane + 1) * per; e++) {
+                const double k = keys[e];
+                b1 = k > b0 ? b0 : k > b1 ? k : b1;
+                b0 = k > b0 ? k : b0;
+            }
+            b0 = a.group_top == 2 && b1 > kNever ? b0 + b1 : b0;
+            gsum[lane] = b0;
+        }
+        __syncthreads();
+        int before = 0;
+#pragma unroll 4
+        for (int g = 0; g < a.n_group; g++) before += route_before(gsum[g], g, b0, lane);
+        if (lane < a.n_group && before >= a.topk_group) {
+#pragma unroll 1
+            for (int e = lane * per; e < (lane + 1) * per; e++) keys[e] = kNever;
+        }
+        __syncthreads();
+    }
+    int id = -1;
+    uint64_t *const place = reinterpret_cast<uint64_t *>(keys);
+#pragma unroll 1
+    for (int e = lane; e < a.n_expert; e += 64) {
+        // without a bias the logits are the order
+        double k = keys[e];
+        if (!a.bias && k > kNever) k = (double)route_load(a.logits, row + e, a.dtype);
+        place[e] = k > kNever ? route_order64(k) : 0;
+    }
+#pragma unroll 1
+    for (int r = 0; r < a.k; r++) {
+        uint64_t v = 0;
+        int i = 0;
+#pragma unroll 4
+        for (int e = lane; e < a.n_expert; e += 64) {
+            const uint64_t k = place[e];
+            i = k > v ? e : i;
+            v = k > v ? k : v;
+        }
+        // the upper halves first, then the lower among those, then the ids
+        const uint32_t hi = route_max<64>((uint32_t)(v >> 32));
+        bool in = (uint32_t)(v >> 32) == hi;
+        const uint32_t lo = route_max<64>(in ? (uint32_t)v : 0);
+        if (hi == 0) break;
+        in = in && (uint32_t)v == lo;
+        const int won = (int)~route_max<64>(in ? ~(uint32_t)i : 0);
+        if (lane == r) id = won;
+        if (in && i == won) place[won] = 0;
+    }
+    __syncthreads();
+    return id;
+}
+
+template <int W, int R>
+__global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_tok) {
+    constexpr int KS = 64 / W;  // chosen experts a lane
+    __shared__ double keys[W * R], gsum[64];
+    __shared__ RoutePick picks[KS][64];
+    const int lane = threadIdx.x & 63, sub = lane % W;
+    const int t = min((int)blockIdx.x * KS + lane / W, n_tok - 1);
+    const bool mine = (int)blockIdx.x * KS + lane / W < n_tok;
     const size_t row = (size_t)t * a.stride;
     const float none = -__builtin_inff();
-    const int per = a.n_expert / a.n_group, g = lane / LG, e0 = (lane - g * LG) * R;
+    const int g = a.n_group == 1 ? 0 : sub / f.LG, e0 = (sub - g * f.LG) * R;
+    RoutePick *const pick = picks[lane / W];
     RouteLane<R> x;
-    x.first = g * per + e0;
-    float top = none;
+    x.first = g * f.per + e0;
+    // all loads before the first use
+    if (f.whole) {
+        float4 b[R / 4];
+        if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < R / 4; j++) b[j] = reinterpret_cast<const float4 *>(a.bias + x.first)[j];
+        }
+        if (a.dtype == T_F32) {
+            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(a.logits) + row + x.first);
+            float4 v[R / 4];
+#pragma unroll
+            for (int j = 0; j < R / 4; j++) v[j] = p[j];
+#pragma unroll
+            for (int j = 0; j < R / 4; j++) {
+                x.l[4 * j] = v[j].x; x.l[4 * j + 1] = v[j].y; x.l[4 * j + 2] = v[j].z; x.l[4 * j + 3] = v[j].w;
+            }
+        } else {
+            const uint2 *p = reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.logits) + row + x.first);
+            uint2 v[R / 4];
+#pragma unroll
+            for (int j = 0; j < R / 4; j++) v[j] = p[j];
+#pragma unroll
+            for (int j = 0; j < R; j++) {
+                const uint32_t w = j & 2 ? v[j / 4].y : v[j / 4].x;
+                x.l[j] = a.dtype == T_F16 ? f16_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu)
+                                          : __builtin_bit_cast(float, j & 1 ? w & 0xFFFF0000u : w << 16);
+            }
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < R / 4; j++) {
+                x.b[4 * j] = b[j].x; x.b[4 * j + 1] = b[j].y; x.b[4 * j + 2] = b[j].z; x.b[4 * j + 3] = b[j].w;
+            }
+        }
+    } else {
+        // past the end the row's last expert
+        auto at = [&](int j) { return min(x.first + j, a.n_expert - 1); };
+        if (a.dtype == T_F32) {
+            const float *p = static_cast<const float *>(a.logits) + row;
+#pragma unroll
+            for (int j = 0; j < R; j++) x.l[j] = p[at(j)];
+        } else {
+            const uint16_t *p = static_cast<const uint16_t *>(a.logits) + row;
+            uint32_t b[R];
+#pragma unroll
+            for (int j = 0; j < R; j++) b[j] = p[at(j)];
+#pragma unroll
+            for (int j = 0; j < R; j++)
+                x.l[j] = a.dtype == T_F16 ? f16_to_f32(b[j]) : __builtin_bit_cast(float, b[j] << 16);
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int j = 0; j < R; j++) x.b[j] = a.bias[at(j)];
+        }
+#pragma unroll
+        for (int j = 0; j < R; j++) x.l[j] = g < a.n_group && e0 + j < f.per ? x.l[j] : none;
+    }
+    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < R; j++) {
-        x.l[j] = g < a.n_group && e0 + j < per ? route_load(a.logits, row + x.first + j, a.dtype) : none;
-        x.l[j] = x.l[j] > none ? x.l[j] : none;  // (a NaN is not)
-        top = fmaxf(top, x.l[j]);
+        // (+ 0.0: -0 and 0 are one place; a NaN is not to be chosen)
+        x.l[j] = x.l[j] > none ? x.l[j] + 0.0f : none;
+        top = max(top, route_order(x.l[j]));
     }
-    const bool softmax = a.score == ROUTE_SOFTMAX, keys = a.bias || a.n_group > 1;
+    const bool softmax = a.score == ROUTE_SOFTMAX, keyed = a.bias || a.n_group > 1;
     float m = none, inv = 1.0f;
-    if (softmax) {
-        m = route_wave_max(top);
-        if (keys) {
+    if (softmax || keyed) {
+        m = route_value(route_max<W>(top));
+        if (softmax && keyed) {
             float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < R; j++)
                 if (x.l[j] > none) s += x.l[j] == m ? 1.0f : __expf(x.l[j] - m);
-            inv = 1.0f / wave_sum(s);
+#pragma unroll
+            for (int off = W / 2; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+            inv = 1.0f / s;
         }
     }
     auto sum64 = [&]() {
         double s = 0.0;
-#pragma unroll
-        for (int j = 0; j < R; j++)
-            if (x.l[j] > none) s += route_exp(x.l[j], m);
-        return route_wave_sum(s);
+#pragma unroll 2
+        for (int e = sub; e < a.n_expert; e += W) {
+            const float l = route_load(a.logits, row + e, a.dtype);
+            const double v = route_exp(l, m);
+            s += l > none ? v : 0.0;
+        }
+        return route_sum<W>(s);
     };
     double sum = 1.0;
     if (softmax && !a.renormalise) sum = sum64();
-    int id;
-    if (!route_choose<float, R>(a, row, x, LG, m, inv, id)) {
-        const double total = softmax ? sum64() : 1.0;
-        (void)route_choose<double, R>(a, row, x, LG, m, total, id);
+    const float off = route_off(a.score, m, inv);
+    const bool sure = route_choose<W, R>(a, f, x, g, m, inv, off, pick);
+    bool settled = false;  // by 64-bit keys
+    unsigned long long todo = __ballot(!sure);
+    while (todo) {
+        const int first = (__ffsll(todo) - 1) & ~(W - 1);  // the token's first lane
+        todo &= ~(~0ull >> (64 - W) << first);
+        const size_t its = ((size_t)__builtin_amdgcn_readlane((int)(row >> 32), first) << 32) |
+                           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)row, first);
+        const int exact = route_exact(a, its, keys, gsum);
+        if (lane < a.k) picks[first / W][lane].id = exact;
+        settled |= (lane & ~(W - 1)) == first;
     }
-    // the weights in 64 bits, a lane each (renormalised, the softmax's divisor
-    // leaves them as they are)
-    double w = id >= 0 ? route_score(route_load(a.logits, row + max(id, 0), a.dtype), a.score, m, sum) : 0.0;
-    if (a.renormalise) {
-        const double total = route_wave_sum(w);
-        w = total == 0.0 ? 0.0 : w * (double)a.scale / total;
-    } else {
-        w *= (double)a.scale;
+    __syncthreads();
+    int id[KS];
+    uint32_t place[KS];
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+        const RoutePick p = i * W + sub < a.k ? pick[i * W + sub] : RoutePick{-1, 0};
+        id[i] = p.id;
+        place[i] = settled ? 0 : p.key;
     }
-    if (lane < a.k) {
-        const size_t at = (size_t)t * a.k + lane;
-        a.ids[at] = id;
-        a.weights[at] = (float)w;
+    // the weights in 64 bits (renormalised, the softmax's divisor leaves them as
+    // they are)
+    double w[KS], total = 0.0;
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+        w[i] = 0.0;
+        if (i * W < a.k) {
+            const float l = route_load(a.logits, row + max(id[i], 0), a.dtype);
+            const double s = route_score(l, a.score, m, sum);
+            w[i] = id[i] >= 0 ? s : 0.0;
+            total += w[i];
+        }
+    }
+    if (a.renormalise) total = route_sum<W>(total);
+    int rank[KS];
+#pragma unroll
+    for (int i = 0; i < KS; i++) rank[i] = i * W + sub;
+    if (a.bias) {
+        // neighbours in the order that f32 cannot tell apart
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int r = i * W + sub;
+            if (r + 1 < a.k && place[i]) {
+                const uint32_t next = pick[r + 1].key;
+                near |= next && !route_apart(route_value(place[i]), route_value(next), off);
+            }
+        }
+        if (__ballot(near)) {
+            // all by their keys in 64 bits (the softmax's with its divisor)
+            const double norm = softmax && a.renormalise ? sum64() : 1.0;
+            double key[KS];
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                key[i] = id[i] >= 0 ? w[i] / norm + (double)a.bias[max(id[i], 0)] : kNever;
+                rank[i] = 0;
+            }
+            for (int r = 0; r < a.k; r++) {
+                const int from = (lane & ~(W - 1)) + r % W;
+                double o = key[0];
+                int oi = id[0];
+#pragma unroll
+                for (int i = 1; i < KS; i++) {
+                    o = r / W == i ? key[i] : o;
+                    oi = r / W == i ? id[i] : oi;
+                }
+                o = __shfl(o, from, 64);
+                oi = __shfl(oi, from, 64);
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+                    rank[i] += id[i] >= 0 ? (oi >= 0 && route_before(o, oi, key[i], id[i])) : i * W + sub > r;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+        if (i * W + sub >= a.k || !mine) continue;
+        double v = w[i] * (double)a.scale;
+        if (a.renormalise) v = total == 0.0 ? 0.0 : v / total;
+        const size_t at = (size_t)t * a.k + rank[i];
+        a.ids[at] = id[i];
+        a.weights[at] = (float)v;
     }
 }
 
-template <int R> static hipError_t route_wave_go(const RouteArgs &a, int n_tok, int LG, hipStream_t s) {
-    // a wavefront a workgroup while that leaves CUs to fill
-    if (n_tok <= 2048) k_route_wave<R, 1><<<(unsigned)n_tok, 64, 0, s>>>(a, n_tok, LG);
-    else k_route_wave<R, 4><<<(unsigned)((n_tok + 3) / 4), 256, 0, s>>>(a, n_tok, LG);
+template <int W, int R> hipError_t route_go(const RouteArgs &a, int n_tok, int LG, hipStream_t s) {
+    constexpr int per_wg = 64 / W;
+    const int per = a.n_expert / a.n_group;
+    const size_t piece = 4 * (a.dtype == T_F32 ? 4 : 2);  // bytes of a load
+    const bool whole = LG * R == per && LG * a.n_group == W && (uintptr_t)a.logits % piece == 0 &&
+                       a.stride % 4 == 0 && (uintptr_t)a.bias % 16 == 0;
+    k_route<W, R><<<(unsigned)((n_tok + per_wg - 1) / per_wg), 64, 0, s>>>(a, RouteForm{per, LG, whole}, n_tok);
     return hipGetLastError();
 }
 
@@ -416,18 +776,20 @@ template <int R> static hipError_t route_wave_go(const RouteArgs &a, int n_tok, 
 
 hipError_t launch_moe_route(const RouteArgs &a, int n_tok, hipStream_t s) {
     if (n_tok <= 0) return hipSuccess;
-    // the fewest experts a lane that bring every group's lanes into a wavefront
+    // the fewest lanes a token that hold its groups with 4, then 8 experts each
+    // (256 experts, 8 of them, no bias, us at 512 / 4095 / 16384 tokens: 32 lanes
+    // of 8 6.4 / 7.7 / 15.6, 64 of 4 6.2 / 7.5 / 21.6, 16 of 16 9.2 / 9.1 / 18.3;
+    // 64 experts at 16384: 16 lanes of 4 9.8, 32 of 8 21.7)
     const int per = a.n_expert / a.n_group;
-    for (int r = 1; r <= 16; r *= 2) {
-        const int LG = (per + r - 1) / r;
-        if ((long long)LG * a.n_group > 64) continue;
-        switch (r) {
-        case 1: return route_wave_go<1>(a, n_tok, LG, s);
-        case 2: return route_wave_go<2>(a, n_tok, LG, s);
-        case 4: return route_wave_go<4>(a, n_tok, LG, s);
-        case 8: return route_wave_go<8>(a, n_tok, LG, s);
-        default: return route_wave_go<16>(a, n_tok, LG, s);
-        }
+    struct Form {
+        int w, r;
+        hipError_t (*go)(const RouteArgs &, int, int, hipStream_t);
+    };
+    static const Form forms[] = {{16, 4, route_go<16, 4>}, {16, 8, route_go<16, 8>}, {32, 8, route_go<32, 8>},
+                                 {64, 8, route_go<64, 8>}, {64, 16, route_go<64, 16>}};
+    for (const Form &f : forms) {
+        const int LG = (per + f.r - 1) / f.r;
+        if ((long long)LG * a.n_group <= f.w) return f.go(a, n_tok, LG, s);
     }
     k_route_any<<<(unsigned)n_tok, 256, (size_t)a.n_group * sizeof(double), s>>>(a);
     return hipGetLastError();

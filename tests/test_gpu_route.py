@@ -91,6 +91,52 @@ def test_keys_that_differ_by_less_than_a_32_bit_rounding(hip):
 
 
 @pytest.mark.parametrize("score", [0, 1, 2])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (8, 4, 2), (8, 4, 1)])
+@pytest.mark.parametrize("n,k", [(64, 8), (256, 8), (256, 20), (384, 8), (1000, 64)])
+def test_close_keys(hip, score, groups, n, k):
+    """Rows whose logits are a few f32 steps apart, and rows of few values among
+    which such pairs are: neighbours in the order, the last chosen and the first
+    left out, and groups are settled by the 64-bit keys."""
+    rng = np.random.default_rng(n + k + score)
+    step = np.float32(2.0 ** -23)
+    rows = []
+    for base in (1.0, -1.5, 3.0):
+        rows.append(np.float32(base) + step * rng.integers(0, 40, n).astype(np.float32) * 2)
+        rows.append(np.float32(base) + step * rng.permutation(n).astype(np.float32) * 4)
+        x = rng.normal(0, 1.5, n).astype(np.float32)
+        x[rng.permutation(n)[:n // 2]] = np.float32(base) + step * rng.integers(0, 3, n // 2) * 2
+        rows.append(x)
+    x = np.stack(rows)
+    for bias in (np.zeros(n), rng.integers(-2, 3, n) * 2.0 ** -12, rng.integers(0, 2, n) * 1e-7,
+                 -2.0 + rng.integers(0, 3, n) * 2.0 ** -22, None):
+        b = None if bias is None else bias.astype(np.float32).astype(np.float64)
+        keep = groups_settled(x.astype(np.float64), b, *groups, score)
+        assert keep.sum() >= len(x) // 2
+        run(hip, x[keep], bias, k, *groups, score=score)
+
+
+def groups_settled(x, bias, n_group, topk_group, group_top, score):
+    """Rows whose kept groups 64-bit arithmetic settles. A group's count (s_a + b_1)
+    + (s_b + b_2) and another's (s_a + b_2) + (s_b + b_1) are equal numbers, but
+    each of the three additions may round by half of 2^-52 of a value below 4, so
+    two such counts can come out up to 6 * 2^-52 * 4 / 2 < 2^-48 apart, in either
+    order, by the last bits of s alone. Rows with counts that near at the border
+    and not of the same logits and biases are left out."""
+    keep = np.ones(len(x), bool)
+    for t, l in enumerate(x):
+        key = R.scores(l, score) + (0 if bias is None else bias)
+        counts = []
+        for g in np.arange(len(l)).reshape(n_group, -1):
+            top = sorted(g, key=lambda e: (-key[e], e))[:group_top]
+            counts.append((key[top].sum(), tuple(sorted((l[e], 0 if bias is None else bias[e]) for e in top))))
+        counts.sort(key=lambda c: -c[0])
+        if topk_group < n_group:
+            edge = counts[topk_group - 1]
+            keep[t] = all(c[1] == edge[1] or abs(c[0] - edge[0]) > 2.0 ** -48 for c in counts)
+    return keep
+
+
+@pytest.mark.parametrize("score", [0, 1, 2])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("groups", [(1, 1, 1), (8, 3, 2), (8, 3, 1)])
 def test_masked_experts(hip, score, bias, groups):
