@@ -230,10 +230,9 @@ namespace {
 // The choice is made in f32. Which of two keys is larger is certain there when
 // they are further apart than f32 can be off (route_apart). The chosen experts'
 // scores are wanted in 64 bits for the weights anyhow: where two neighbours among
-// them are close, those settle their order. Where the last chosen is close to one
-// left out, or a kept group to one left out, and they are not the same logit and
-// bias, the token's choice is made again in 64 bits (256 experts, biases of 0.05:
-// about 1 token in 5000).
+// them, or the last of them and up to four behind it, are close, those settle it.
+// More that are close there, or a kept group close to one left out, and not the
+// same logit and bias: the token's choice is made again in 64 bits.
 // Several tokens a wavefront share its instructions, and the best of 16 lanes is
 // four steps within a DPP row; more experts a lane cost more looks through them.
 
@@ -325,12 +324,13 @@ struct RoutePick {
     uint32_t key;
 };
 
-// The k best of each of the wavefront's tokens by their f32 keys (inv: the inverse of
+// The k best (and what is close behind them: `taken` in all) of each of the
+// wavefront's tokens by their f32 keys (inv: the inverse of
 // the softmax's divisor; off: route_off) to `pick`, id -1 behind the last. False at the tokens where
 // f32 cannot tell which they are.
 template <int W, int R>
 __device__ __forceinline__ bool route_choose(const RouteArgs &a, const RouteForm &f, const RouteLane<R> &x,
-                                             int g, float m, float inv, float off, RoutePick *pick) {
+                                             int g, float m, float inv, float off, RoutePick *pick, int &taken) {
     const int lane = threadIdx.x & 63, sub = lane % W;
     const float none = -__builtin_inff();
     bool sure = true;
@@ -419,14 +419,14 @@ __device__ __forceinline__ bool route_choose(const RouteArgs &a, const RouteForm
         }
     };
     scan(0xFFFFFFFFu, -1);
-    for (int r = sub; r < a.k; r += W) pick[r] = RoutePick{-1, 0};
+    for (int r = sub; r < min(a.k + 4, 64); r += W) pick[r] = RoutePick{-1, 0};
     __builtin_amdgcn_wave_barrier();
     int gave = 0;
-    uint32_t last = 0;
-    for (int r = 0; r < a.k; r++) {
+    // the best one left, as pick[r], at the tokens where `take` lets it
+    auto round = [&](int r, auto take) __attribute__((always_inline)) {
         const uint32_t best = route_max<W>(h0);
-        const int who = route_first<W>(h0 == best && best != 0);
-        last = best ? best : last;
+        const bool in = best != 0 && take(best);
+        const int who = route_first<W>(h0 == best && in);
         const int from = a0;
         if (who == sub) {
             pick[r] = RoutePick{x.first + a0, best};
@@ -448,14 +448,25 @@ __device__ __forceinline__ bool route_choose(const RouteArgs &a, const RouteForm
                 a0 = i0; a1 = i1; a2 = i2;
             }
         }
+        return best;
+    };
+    uint32_t last = 0;
+    for (int r = 0; r < a.k; r++) {
+        const uint32_t best = round(r, [](uint32_t) { return true; });
+        last = best ? best : last;
     }
+    taken = a.k;
     if (a.bias) {
-        // the last chosen against the best one left out
-        const uint32_t next = route_max<W>(h0);
-        const bool near = next && !route_apart(route_value(last), route_value(next), off);
+        // up to four more that are close to the last chosen, for the 64-bit keys
+        auto close = [&](uint32_t k) { return k && !route_apart(route_value(last), route_value(k), off); };
+        while (__ballot(close(route_max<W>(h0))) && taken < a.k + 4 && taken < 64) {
+            (void)round(taken, close);
+            taken++;
+        }
+        const bool near = close(route_max<W>(h0));
         if (__ballot(near)) {
-            // chosen or not, whatever is close to the last chosen has to be its
-            // equal: the same logit and bias
+            // still more: chosen or not, whatever is close to the last chosen has
+            // to be its equal then, the same logit and bias
             bool unsure = false;
             uint32_t l = 0, b = 0;
 #pragma unroll
@@ -676,7 +687,8 @@ __global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_to
     double sum = 1.0;
     if (softmax && !a.renormalise) sum = sum64();
     const float off = route_off(a.score, m, inv);
-    const bool sure = route_choose<W, R>(a, f, x, g, m, inv, off, pick);
+    int taken;
+    const bool sure = route_choose<W, R>(a, f, x, g, m, inv, off, pick, taken);
     bool settled = false;  // by 64-bit keys
     unsigned long long todo = __ballot(!sure);
     while (todo) {
@@ -685,7 +697,7 @@ __global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_to
         const size_t its = ((size_t)__builtin_amdgcn_readlane((int)(row >> 32), first) << 32) |
                            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)row, first);
         const int exact = route_exact(a, its, keys, gsum);
-        if (lane < a.k) picks[first / W][lane].id = exact;
+        if (lane < taken) picks[first / W][lane].id = lane < a.k ? exact : -1;
         settled |= (lane & ~(W - 1)) == first;
     }
     __syncthreads();
@@ -693,24 +705,22 @@ __global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_to
     uint32_t place[KS];
 #pragma unroll
     for (int i = 0; i < KS; i++) {
-        const RoutePick p = i * W + sub < a.k ? pick[i * W + sub] : RoutePick{-1, 0};
+        const RoutePick p = i * W + sub < taken ? pick[i * W + sub] : RoutePick{-1, 0};
         id[i] = p.id;
         place[i] = settled ? 0 : p.key;
     }
-    // the weights in 64 bits (renormalised, the softmax's divisor leaves them as
-    // they are)
-    double w[KS], total = 0.0;
+    // their scores in 64 bits (renormalised, the softmax's divisor leaves the
+    // weights as they are)
+    double w[KS];
 #pragma unroll
     for (int i = 0; i < KS; i++) {
         w[i] = 0.0;
-        if (i * W < a.k) {
+        if (i * W < taken) {
             const float l = route_load(a.logits, row + max(id[i], 0), a.dtype);
             const double s = route_score(l, a.score, m, sum);
             w[i] = id[i] >= 0 ? s : 0.0;
-            total += w[i];
         }
     }
-    if (a.renormalise) total = route_sum<W>(total);
     int rank[KS];
 #pragma unroll
     for (int i = 0; i < KS; i++) rank[i] = i * W + sub;
@@ -720,7 +730,7 @@ __global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_to
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             const int r = i * W + sub;
-            if (r + 1 < a.k && place[i]) {
+            if (r + 1 < taken && place[i]) {
                 const uint32_t next = pick[r + 1].key;
                 near |= next && !route_apart(route_value(place[i]), route_value(next), off);
             }
@@ -734,7 +744,7 @@ __global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_to
                 key[i] = id[i] >= 0 ? w[i] / norm + (double)a.bias[max(id[i], 0)] : kNever;
                 rank[i] = 0;
             }
-            for (int r = 0; r < a.k; r++) {
+            for (int r = 0; r < taken; r++) {
                 const int from = (lane & ~(W - 1)) + r % W;
                 double o = key[0];
                 int oi = id[0];
@@ -751,9 +761,15 @@ __global__ __launch_bounds__(64) void k_route(RouteArgs a, RouteForm f, int n_to
             }
         }
     }
+    double total = 0.0;
+    if (a.renormalise) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) total += rank[i] < a.k ? w[i] : 0.0;
+        total = route_sum<W>(total);
+    }
 #pragma unroll
     for (int i = 0; i < KS; i++) {
-        if (i * W + sub >= a.k || !mine) continue;
+        if (rank[i] >= a.k || !mine) continue;
         double v = w[i] * (double)a.scale;
         if (a.renormalise) v = total == 0.0 ? 0.0 : v / total;
         const size_t at = (size_t)t * a.k + rank[i];
