@@ -512,7 +512,8 @@ int rsllm_hip_matmul_q8_0_batch_dev(float *out, size_t out_len, const uint8_t *w
  * the same results, bit for bit. `work`: rsllm_hip_int8_work_bytes(n_tok,
  * in_dim, out_dim) bytes of the caller's (it never falls as n_tok grows),
  * 256-byte aligned, used by this call alone until it has run: calls that may
- * overlap, and graphs that may replay at once, get one each.
+ * overlap, and graphs that may replay at once, get one each. The prequant form
+ * also takes NULL with work_len 0 (its products leave nothing between launches).
  * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for in_dim 0 or
  * above 131071 (where the sum could leave 32 bits), out_dim 0, NULL or
  * misaligned pointers; SHAPE_MISMATCH for a stride below its row, x_len or

@@ -60,8 +60,7 @@ bool i8_work(size_t n_tok, size_t in_dim, size_t out_dim, I8Work *w) {
 // Checks of the product that both forms share.
 int check_i8(const void *out, size_t out_len, size_t out_stride, const int8_t *w, size_t w_len,
              const float *wscale, size_t wscale_len, const float *bias, size_t bias_len,
-             const uint8_t *work, size_t work_len, size_t n_tok, size_t in_dim, size_t out_dim,
-             uint32_t dtype_out, I8Work *parts) {
+             const uint8_t *work, size_t n_tok, size_t in_dim, size_t out_dim, uint32_t dtype_out) {
     if (!float_type(dtype_out))
         return set_error(RSLLM_HIP_ERR_UNIMPLEMENTED, "matmul_int8: output dtype not implemented");
     if (in_dim == 0 || in_dim > kI8MaxIn)
@@ -76,10 +75,7 @@ int check_i8(const void *out, size_t out_len, size_t out_stride, const int8_t *w
         return mismatch("matmul_int8: bias must be out_dim or absent");
     if (out_stride < out_dim || !span_ok(n_tok, out_dim, out_stride, out_len))
         return mismatch("matmul_int8: out must hold n_tok rows of out_dim, out_stride apart");
-    (void)i8_work(n_tok, in_dim, out_dim, parts);
-    if (work_len < parts->total)
-        return mismatch("matmul_int8: work must be int8_work_bytes");
-    if (!w || !wscale || (n_tok && !out) || (bias_len && !bias) || (parts->total && !work))
+    if (!w || !wscale || (n_tok && !out) || (bias_len && !bias))
         return invalid("NULL pointer with a nonzero length");
     if (!aligned(w, 16) || !aligned(wscale, 4) || !aligned(bias, 4) || !aligned(work, 256) ||
         !aligned(out, elem_bytes(dtype_out)))
@@ -177,10 +173,9 @@ int rsllm_hip_matmul_int8_prequant_dev(void *out, size_t out_len, size_t out_str
                                        size_t work_len, size_t n_tok, size_t in_dim,
                                        size_t out_dim, uint32_t dtype_out,
                                        rsllm_hip_stream_t stream) {
-    I8Work parts;
+    (void)work_len;  // (these products leave nothing between launches)
     if (const int rc = check_i8(out, out_len, out_stride, weights, weights_len, wscale, wscale_len,
-                                bias, bias_len, work, work_len, n_tok, in_dim, out_dim, dtype_out,
-                                &parts))
+                                bias, bias_len, work, n_tok, in_dim, out_dim, dtype_out))
         return rc;
     if (!product_is(n_tok, i8_row_bytes(in_dim), xq_len))
         return mismatch("matmul_int8: xq must be n_tok * int8_row_bytes(in_dim)");
@@ -201,11 +196,13 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
                               size_t x_stride, uint8_t *work, size_t work_len, size_t n_tok,
                               size_t in_dim, size_t out_dim, uint32_t dtype_x, uint32_t dtype_out,
                               rsllm_hip_stream_t stream) {
-    I8Work parts;
     if (const int rc = check_i8(out, out_len, out_stride, weights, weights_len, wscale, wscale_len,
-                                bias, bias_len, work, work_len, n_tok, in_dim, out_dim, dtype_out,
-                                &parts))
+                                bias, bias_len, work, n_tok, in_dim, out_dim, dtype_out))
         return rc;
+    I8Work parts;
+    (void)i8_work(n_tok, in_dim, out_dim, &parts);
+    if (work_len < parts.total) return mismatch("matmul_int8: work must be int8_work_bytes");
+    if (parts.total && !work) return invalid("NULL pointer with a nonzero length");
     if (const int rc = check_x("matmul_int8: x must hold n_tok rows of in_dim, x_stride apart", x,
                                x_len, x_stride, n_tok, in_dim, dtype_x))
         return rc;

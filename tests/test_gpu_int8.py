@@ -200,6 +200,56 @@ def test_non_finite_tokens_stay_alone(hip, n_tok):
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("n_tok", [1, 4, 20, 70, 300])
+@pytest.mark.parametrize("dtype_out", KINDS)
+def test_scales_and_outputs_aligned_to_their_elements_alone(hip, n_tok, dtype_out):
+    """wscale, bias and out one element into an allocation, so on no 16-byte
+    border; work of the halves' product left out."""
+    rng = np.random.default_rng(n_tok)
+    n, out_dim = 192, 132
+    w, ws = weights(rng, out_dim, n)
+    bias = rng.normal(0, 1, out_dim).astype(np.float32)
+    codes, scales = R.quantize(rng.normal(0, 1, (n_tok, n)).astype(np.float32).astype(np.float64))
+    want, p = R.int8_product(codes, scales, w[:, :n], ws, bias)
+
+    def shifted(a):
+        return torch.cat([torch.full((1,), 9.0), torch.from_numpy(a)]).cuda()
+    wd, xq, sc = torch.from_numpy(w).cuda(), torch.from_numpy(codes).cuda(), torch.from_numpy(scales).cuda()
+    wsd, bd = shifted(ws), shifted(bias)
+    y = torch.full((1 + n_tok * out_dim,), -7.0, dtype=R.TORCH[dtype_out], device="cuda")
+    hip.matmul_int8_prequant_dev(y.data_ptr() + y.element_size(), n_tok * out_dim, out_dim, wd.data_ptr(),
+                                 wd.numel(), wsd.data_ptr() + 4, out_dim, bd.data_ptr() + 4, out_dim,
+                                 xq.data_ptr(), xq.numel(), sc.data_ptr(), n_tok, 0, 0, n_tok, n, out_dim,
+                                 R.GGML[dtype_out], torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    got = y.cpu().double().numpy()
+    assert got[0] == -7.0
+    got = got[1:].reshape(n_tok, out_dim)
+    bound = 3.001 * 2.0 ** -24 * np.abs(p) + 2.0 ** -24 * np.abs(want) \
+        + 1.001 * R.HALF_STEP[dtype_out] * np.abs(want) * (dtype_out != "f32") + R.TINY_STEP[dtype_out]
+    assert not (np.abs(got - want) > bound).any()
+
+
+@pytest.mark.parametrize("n_tok", [1, 3, 20, 70])
+def test_weights_beyond_32_bit_offsets(hip, n_tok):
+    """A matrix of 5.2 GB: the last rows against their own products."""
+    n, out_dim, tail = 131071, 40000, 50
+    w = torch.randint(-127, 128, (out_dim, 131072), dtype=torch.int8, device="cuda")
+    ws = torch.full((out_dim,), 1e-6, device="cuda")
+    x = torch.randn(n_tok, n, device="cuda")
+    y = torch.full((n_tok, out_dim), NAN, device="cuda")
+    work = torch.empty(hip.int8_work_bytes(n_tok, n, out_dim), dtype=torch.uint8, device="cuda")
+    hip.matmul_int8_dev(y.data_ptr(), y.numel(), out_dim, w.data_ptr(), w.numel(), ws.data_ptr(), out_dim,
+                        0, 0, x.data_ptr(), x.numel(), n, work.data_ptr(), work.numel(), n_tok, n, out_dim,
+                        stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    codes, scales = R.quantize(x.cpu().double().numpy())
+    want, p = R.int8_product(codes, scales, w[-tail:, :n].cpu().numpy(), ws[-tail:].cpu().numpy(), None)
+    got = y.cpu().double().numpy()
+    assert np.isfinite(got).all()
+    assert not (np.abs(got[:, -tail:] - want) > 3.001 * 2.0 ** -24 * np.abs(p)).any()
+
+
 def test_overflow_to_the_output_type(hip):
     """A product above f16's largest is inf, as a rounding gives."""
     w = np.full((4, 64), 127, np.int8)

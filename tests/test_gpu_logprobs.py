@@ -38,7 +38,7 @@ def bounds(values, lp, ent, top):
 
 def near(got, want, bound):
     got = got.astype(np.float64)
-    want = np.where(np.abs(want) > 3.4028236e38, np.sign(want) * INF, want)  # f32's largest
+    want = np.where(np.abs(want) > 3.4028236e38, np.copysign(INF, want), want)  # f32's largest
     same = (got == want) | (np.isnan(got) & np.isnan(want))
     with np.errstate(invalid="ignore"):
         ok = same | (np.abs(got - want) <= bound)
@@ -245,3 +245,27 @@ def test_on_another_stream_and_captured(hip):
             near(top.cpu().numpy(), want_top, b_top)
             np.testing.assert_array_equal(rank.cpu().numpy(), r)
             np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
+
+
+def test_rows_beyond_32_bit_offsets(hip):
+    """4.7 GB of logits: the first and the last rows."""
+    n_tok, v = 9100, 129280
+    d = torch.randn(n_tok, v, device="cuda")
+    tok = torch.randint(0, v, (n_tok,), dtype=torch.int32, device="cuda")
+    o, rank = torch.full((2, n_tok), NAN, device="cuda"), torch.zeros(n_tok, dtype=torch.int32, device="cuda")
+    ids, top = torch.zeros(n_tok, 5, dtype=torch.int32, device="cuda"), torch.zeros(n_tok, 5, device="cuda")
+    work = torch.empty(256 + hip.token_logprobs_work_bytes(n_tok, v, 5), dtype=torch.uint8, device="cuda")
+    hip.token_logprobs_dev(o[0].data_ptr(), o[1].data_ptr(), rank.data_ptr(), n_tok, ids.data_ptr(),
+                           top.data_ptr(), n_tok * 5, d.data_ptr(), d.numel(), v, tok.data_ptr(), n_tok,
+                           work.data_ptr(), work.numel(), n_tok, v, 5,
+                           stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for at in (slice(0, 2), slice(n_tok - 2, n_tok)):
+        x = d[at].cpu().double().numpy()
+        lp, r, ent, want_ids, want_top = R.logprobs(x, tok[at].cpu().tolist(), 5)
+        b_lp, b_ent, b_top = bounds(x, lp, ent, want_top)
+        near(o[0, at].cpu().numpy(), lp, b_lp)
+        near(o[1, at].cpu().numpy(), ent, b_ent)
+        near(top[at].cpu().numpy(), want_top, b_top)
+        np.testing.assert_array_equal(rank[at].cpu().numpy(), r)
+        np.testing.assert_array_equal(ids[at].cpu().numpy(), want_ids)

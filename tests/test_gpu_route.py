@@ -223,3 +223,20 @@ def test_on_another_stream_and_captured(hip):
         np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
         np.testing.assert_allclose(w.cpu().numpy(), want_w, rtol=2.0 ** -23)
         ids.fill_(-5)
+
+
+def test_rows_beyond_32_bit_offsets(hip):
+    """4.6 GB of logits: the first and the last tokens."""
+    n_tok, n, k = 4_500_001, 256, 8
+    d = torch.randn(n_tok, n, device="cuda")
+    b = torch.randn(n, device="cuda") * 0.05
+    ids = torch.full((n_tok, k), -5, dtype=torch.int32, device="cuda")
+    w = torch.zeros(n_tok, k, device="cuda")
+    hip.moe_route_dev(ids.data_ptr(), w.data_ptr(), n_tok * k, d.data_ptr(), d.numel(), n, b.data_ptr(), n,
+                      n_tok, n, k, 8, 4, 2, score=1, stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert (ids >= 0).all()
+    for at in (slice(0, 9), slice(n_tok - 9, n_tok)):
+        want_ids, want_w = R.route(d[at].cpu().double().numpy(), b.cpu().double().numpy(), k, 8, 4, 2, 1, True, 1.0)
+        np.testing.assert_array_equal(ids[at].cpu().numpy(), want_ids)
+        np.testing.assert_allclose(w[at].cpu().numpy(), want_w, rtol=2.0 ** -23)
