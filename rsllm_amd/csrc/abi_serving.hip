@@ -212,8 +212,8 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
     float *xscale = reinterpret_cast<float *>(work + parts.codes);
     const I8Args a{weights, xq, wscale, xscale, bias_len ? bias : nullptr, out, out_stride,
                    (int)n_tok, (int)out_dim, (int)i8_row_bytes(in_dim), dtype_out};
-    if (i8_few_supported((int)n_tok, (int)in_dim)) {
-        HIP_TRY(launch_i8_few(a, x, x_stride, (int)in_dim, dtype_x, (hipStream_t)stream), "matmul_int8");
+    if (n_tok == 1 && i8_one_supported((int)in_dim)) {
+        HIP_TRY(launch_i8_one(a, x, (int)in_dim, dtype_x, (hipStream_t)stream), "matmul_int8");
         return abi::ok_status();
     }
     HIP_TRY(launch_i8_quantize(x, x_stride, xq, xscale, (int)n_tok, (int)in_dim, dtype_x,

@@ -79,6 +79,19 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// The largest of the 64 lanes' values, at every lane: rotations within the DPP rows
+// of 16 lanes, then rows and halves exchanged.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true));  // row_ror:8
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, true));
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max((uint32_t)r[0], (uint32_t)r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max((uint32_t)h[0], (uint32_t)h[1]);
+}
+
 // Byte b (0..3) of a dword as float: one v_cvt_f32_ubyte{b}.
 __device__ __forceinline__ float ubyte_f(uint32_t v, int b) {
     return (float)((v >> (8 * b)) & 0xFFu);

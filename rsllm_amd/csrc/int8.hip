@@ -145,8 +145,7 @@ __global__ __launch_bounds__(THREADS) void k_i8_quantize(const void *__restrict_
 #pragma unroll
         for (int k = 0; k < N; k++) big = max(big, i8_abs_bits(v[k]));
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, off, 64));
+    big = wave_max_u32(big);
     if constexpr (W > 1) {
         if ((tid & 63) == 0) red[tid >> 6] = big;
         __syncthreads();
@@ -169,138 +168,106 @@ __global__ __launch_bounds__(THREADS) void k_i8_quantize(const void *__restrict_
     if (tid == 0) scale[t] = ok ? s.d : __builtin_nanf("");
 }
 
-// ---- few tokens: one launch, the weights streamed through dot products -----------
+// ---- one token: one launch, the weights streamed through dot products -----------
 //
-// A wavefront multiplies R rows with all T tokens: a lane holds 16 bytes of every
-// KB of a row, so the weights are read in whole lines, and its sums of all rows
-// and tokens are added across the wavefront at the end, each step halving what a
-// lane keeps. The workgroup quantises x itself (x is small and in L2), its first
-// weights already on the way. Bound by the weight stream.
-template <int T, uint32_t DT>
-__global__ __launch_bounds__(256) void k_i8_few(I8Args a, const void *__restrict__ x, size_t x_stride,
-                                                int in_dim, int kp, int vec) {
-    constexpr int R = 4, P = 4, N = I8Vec<DT>::N;  // P: 1 KB pieces of a row in flight
-    extern __shared__ __align__(16) int8_t codes[];  // [T][kp], zero behind in_dim
-    __shared__ uint32_t red[T][4];
+// A wavefront multiplies R rows: a lane holds 16 bytes of every KB of a row, so the
+// weights are read in whole lines, and its R sums are added across the wavefront at
+// the end. The workgroup quantises x itself (x is small and in L2), its first
+// weights already on the way. Bound by the weight stream (14336 x 4096: see the
+// launcher). From two tokens on, every workgroup's quantising costs more than the
+// launch it saves (4096 x 4096 f32, us, one launch against two: 1 token 6.9 / 7.9;
+// with a form of this kernel for more, 2 tokens 10.2 / 8.2, 4 tokens 15.1 / 8.4).
+template <uint32_t DT>
+__global__ __launch_bounds__(256) void k_i8_one(I8Args a, const void *__restrict__ x, int in_dim, int kp,
+                                                int vec) {
+    constexpr int R = 4, P = 4, N = I8Vec<DT>::N, kHeld = 16 / N;  // P: 1 KB pieces of a row in flight
+    extern __shared__ __align__(16) int8_t codes[];  // [kp], zero behind in_dim
+    __shared__ uint32_t red[4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int o0 = blockIdx.x * (4 * R), rb = a.row_bytes;
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(a.w + (size_t)o0 * rb, (uint32_t)min(4 * R, a.out_dim - o0) * (uint32_t)rb);
-    uint4 w[R][P];
-    auto load = [&](int k0) {
+    uint4 w[P][R];
+    // piece k0 of the rows (behind a row's end the next row's bytes or, past the
+    // last, zeros: the codes there are zero)
+    auto load = [&](uint4 (&d)[R], int k0) {
+        if (k0 < rb) {
 #pragma unroll
-        for (int p = 0; p < P; p++)
-            if (k0 + 1024 * p < rb) {
-#pragma unroll
-                for (int r = 0; r < R; r++)
-                    w[r][p] = bload16(rw, (uint32_t)((wv * R + r) * rb + k0 + 1024 * p + 16 * lane), 0);
-            }
+            for (int r = 0; r < R; r++) d[r] = bload16(rw, (uint32_t)((wv * R + r) * rb + k0 + 16 * lane), 0);
+        }
     };
     // x, then the first weights behind it: loads return in order
-    constexpr int kHeld = 16 / (N * (T > 2 ? 2 : 1));
-    float held[T][kHeld][N];
+    float held[kHeld][N];
 #pragma unroll
-    for (int t = 0; t < T; t++)
+    for (int h = 0; h < kHeld; h++) {
+        const int i = (h * 256 + tid) * N;
 #pragma unroll
-        for (int h = 0; h < kHeld; h++) {
-            const int i = (h * 256 + tid) * N;
-#pragma unroll
-            for (int k = 0; k < N; k++) held[t][h][k] = 0.0f;
-            if (i < in_dim) i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, held[t][h]);
-        }
-    if (in_dim <= kHeld * 256 * N) load(0);
-    uint32_t big[T];
-#pragma unroll
-    for (int t = 0; t < T; t++) {
-        big[t] = 0;
-#pragma unroll
-        for (int h = 0; h < kHeld; h++)
-#pragma unroll
-            for (int k = 0; k < N; k++) big[t] = max(big[t], i8_abs_bits(held[t][h][k]));
+        for (int k = 0; k < N; k++) held[h][k] = 0.0f;
+        if (i < in_dim) i8_load_vec<DT>(x, 0, i, in_dim, vec, held[h]);
+    }
+    uint32_t big = 0;
+    if (in_dim > kHeld * 256 * N) {
         for (int i = (kHeld * 256 + tid) * N; i < in_dim; i += 256 * N) {
             float v[N];
-            i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, v);
+            i8_load_vec<DT>(x, 0, i, in_dim, vec, v);
 #pragma unroll
-            for (int k = 0; k < N; k++) big[t] = max(big[t], i8_abs_bits(v[k]));
+            for (int k = 0; k < N; k++) big = max(big, i8_abs_bits(v[k]));
         }
     }
-    if (in_dim > kHeld * 256 * N) load(0);
 #pragma unroll
-    for (int t = 0; t < T; t++) {
+    for (int p = 0; p < P; p++) load(w[p], 1024 * p);
 #pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) big[t] = max(big[t], (uint32_t)__shfl_xor((int)big[t], off, 64));
-        if (lane == 0) red[t][wv] = big[t];
+    for (int h = 0; h < kHeld; h++)
+#pragma unroll
+        for (int k = 0; k < N; k++) big = max(big, i8_abs_bits(held[h][k]));
+    big = wave_max_u32(big);
+    if (lane == 0) red[wv] = big;
+    __syncthreads();
+    big = max(max(red[0], red[1]), max(red[2], red[3]));
+    const bool ok = i8_finite_bits(big);
+    const I8Scale sc = i8_scale(ok ? __builtin_bit_cast(float, big) : 0.0f);
+#pragma unroll
+    for (int h = 0; h < kHeld; h++) {
+        const int i = (h * 256 + tid) * N;
+        if (i < kp) i8_store_codes<N>(codes + i, held[h], sc);
+    }
+    for (int i = (kHeld * 256 + tid) * N; i < kp; i += 256 * N) {
+        float v[N];
+        i8_load_vec<DT>(x, 0, i, in_dim, vec, v);
+        i8_store_codes<N>(codes + i, v, sc);
     }
     __syncthreads();
-    I8Scale sc[T];
-    bool ok[T];
+    int acc[R] = {0, 0, 0, 0};
+    for (int k0 = 0; k0 < rb; k0 += 1024 * P) {
 #pragma unroll
-    for (int t = 0; t < T; t++) {
-        big[t] = max(max(red[t][0], red[t][1]), max(red[t][2], red[t][3]));
-        ok[t] = i8_finite_bits(big[t]);
-        sc[t] = i8_scale(ok[t] ? __builtin_bit_cast(float, big[t]) : 0.0f);
+        for (int p = 0; p < P; p++) {
+            const int k = k0 + 1024 * p;
+            if (k >= rb) break;
+            const uint4 c = *reinterpret_cast<const uint4 *>(codes + k + 16 * lane);
 #pragma unroll
-        for (int h = 0; h < kHeld; h++) {
-            const int i = (h * 256 + tid) * N;
-            if (i < kp) i8_store_codes<N>(codes + t * kp + i, held[t][h], sc[t]);
-        }
-        for (int i = (kHeld * 256 + tid) * N; i < kp; i += 256 * N) {
-            float v[N];
-            i8_load_vec<DT>(x, (size_t)t * x_stride, i, in_dim, vec, v);
-            i8_store_codes<N>(codes + t * kp + i, v, sc[t]);
-        }
-    }
-    __syncthreads();
-    constexpr int NV = R * (T == 3 ? 4 : T);
-    int acc[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) acc[i] = 0;
-    for (int k0 = 0;; k0 += 1024 * P) {
-#pragma unroll
-        for (int p = 0; p < P; p++)
-            if (k0 + 1024 * p < rb) {
-#pragma unroll
-                for (int t = 0; t < T; t++) {
-                    const uint4 c = *reinterpret_cast<const uint4 *>(codes + t * kp + k0 + 1024 * p + 16 * lane);
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        int d = acc[t * R + r];
-                        d = __builtin_amdgcn_sdot4((int)w[r][p].x, (int)c.x, d, false);
-                        d = __builtin_amdgcn_sdot4((int)w[r][p].y, (int)c.y, d, false);
-                        d = __builtin_amdgcn_sdot4((int)w[r][p].z, (int)c.z, d, false);
-                        acc[t * R + r] = __builtin_amdgcn_sdot4((int)w[r][p].w, (int)c.w, d, false);
-                    }
-                }
+            for (int r = 0; r < R; r++) {
+                acc[r] = __builtin_amdgcn_sdot4((int)w[p][r].x, (int)c.x, acc[r], false);
+                acc[r] = __builtin_amdgcn_sdot4((int)w[p][r].y, (int)c.y, acc[r], false);
+                acc[r] = __builtin_amdgcn_sdot4((int)w[p][r].z, (int)c.z, acc[r], false);
+                acc[r] = __builtin_amdgcn_sdot4((int)w[p][r].w, (int)c.w, acc[r], false);
             }
-        if (k0 + 1024 * P >= rb) break;
-        load(k0 + 1024 * P);
-    }
-    // lane bits 5, 4, ... pick the half of the sums that the lane goes on with
-    int off = 32;
-#pragma unroll
-    for (int n = NV / 2; n >= 1; n /= 2, off /= 2) {
-        const bool upper = (lane & off) != 0;
-#pragma unroll
-        for (int i = 0; i < n; i++) {
-            const int send = upper ? acc[i] : acc[i + n], keep = upper ? acc[i + n] : acc[i];
-            acc[i] = keep + __shfl_xor(send, off, 64);
+            load(w[p], k + 1024 * P);
         }
     }
-    for (; off >= 1; off /= 2) acc[0] += __shfl_xor(acc[0], off, 64);
-    constexpr int kRep = 64 / NV;  // lanes with the same sum
-    const int v = lane / kRep, t = v / R, o = o0 + wv * R + v % R;
-    if (lane % kRep == 0 && t < T && o < a.out_dim) {
-        float xs = sc[0].d;
-        bool fine = ok[0];
-#pragma unroll
-        for (int i = 1; i < T; i++) {
-            xs = t == i ? sc[i].d : xs;
-            fine = t == i ? ok[i] : fine;
-        }
-        if (!fine) xs = __builtin_nanf("");
-        float y = ((float)acc[0] * xs) * a.wscale[o];
+    // the upper 32 lanes go on with rows 2 and 3, the odd DPP rows with 1 and 3
+    const auto s0 = __builtin_amdgcn_permlane32_swap((uint32_t)acc[0], (uint32_t)acc[2], false, false);
+    const auto s1 = __builtin_amdgcn_permlane32_swap((uint32_t)acc[1], (uint32_t)acc[3], false, false);
+    const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)(s0[0] + s0[1]), (uint32_t)(s1[0] + s1[1]), false, false);
+    int sum = (int)(s[0] + s[1]);
+    sum += __builtin_amdgcn_mov_dpp(sum, 0x128, 0xf, 0xf, true);  // row_ror:8
+    sum += __builtin_amdgcn_mov_dpp(sum, 0x124, 0xf, 0xf, true);
+    sum += __builtin_amdgcn_mov_dpp(sum, 0x122, 0xf, 0xf, true);
+    sum += __builtin_amdgcn_mov_dpp(sum, 0x121, 0xf, 0xf, true);
+    const int o = o0 + wv * R + (lane >> 4);
+    if ((lane & 15) == 0 && o < a.out_dim) {
+        float y = ((float)sum * (ok ? sc.d : __builtin_nanf(""))) * a.wscale[o];
         if (a.bias) y += a.bias[o];
-        i8_store(a.out, (size_t)t * a.out_stride + o, y, a.dtype_out);
+        i8_store(a.out, (size_t)o, y, a.dtype_out);
     }
 }
 
@@ -758,17 +725,6 @@ hipError_t i8_quantize_go(const void *x, size_t stride, int8_t *xq, float *scale
     return hipGetLastError();
 }
 
-template <int T>
-hipError_t i8_few_go(const I8Args &a, const void *x, size_t stride, int in_dim, uint32_t dtype, hipStream_t s) {
-    const int kp = (in_dim + 1023) / 1024 * 1024, vec = i8_vec_ok(x, stride, dtype);
-    const dim3 g((unsigned)((a.out_dim + 15) / 16));
-    const size_t lds = (size_t)T * kp;
-    if (dtype == T_F32) k_i8_few<T, T_F32><<<g, 256, lds, s>>>(a, x, stride, in_dim, kp, vec);
-    else if (dtype == T_F16) k_i8_few<T, T_F16><<<g, 256, lds, s>>>(a, x, stride, in_dim, kp, vec);
-    else k_i8_few<T, T_BF16><<<g, 256, lds, s>>>(a, x, stride, in_dim, kp, vec);
-    return hipGetLastError();
-}
-
 }  // namespace
 
 hipError_t launch_i8_quantize(const void *x, size_t stride, int8_t *xq, float *scale, int n_tok,
@@ -780,19 +736,19 @@ hipError_t launch_i8_quantize(const void *x, size_t stride, int8_t *xq, float *s
     return i8_quantize_go<512>(x, stride, xq, scale, n_tok, in_dim, dtype, s);
 }
 
-bool i8_few_supported(int n_tok, int in_dim) {
-    return n_tok >= 1 && n_tok <= 4 && (size_t)n_tok * ((in_dim + 1023) / 1024 * 1024) <= 60 * 1024;
-}
+bool i8_one_supported(int in_dim) { return in_dim <= 60 * 1024; }  // its codes in LDS
 
-hipError_t launch_i8_few(const I8Args &a, const void *x, size_t stride, int in_dim, uint32_t dtype,
-                         hipStream_t s) {
-    if (!i8_few_supported(a.n_tok, in_dim)) return hipErrorNotSupported;
-    switch (a.n_tok) {
-    case 1: return i8_few_go<1>(a, x, stride, in_dim, dtype, s);
-    case 2: return i8_few_go<2>(a, x, stride, in_dim, dtype, s);
-    case 3: return i8_few_go<3>(a, x, stride, in_dim, dtype, s);
-    default: return i8_few_go<4>(a, x, stride, in_dim, dtype, s);
-    }
+// One token, us, against the quantiser and a tile product: 14336 x 4096 f32 14.4 /
+// 17.1 (59 MB: 4.1 TB/s), 4096 x 14336 18.4 / 18.7 (bf16 15.7 / 17.4), 4096 x 4096
+// bf16 5.7 / 7.5, 1024 x 1024 2.9 / 5.3.
+hipError_t launch_i8_one(const I8Args &a, const void *x, int in_dim, uint32_t dtype, hipStream_t s) {
+    if (!i8_one_supported(in_dim) || a.n_tok != 1) return hipErrorNotSupported;
+    const int kp = (in_dim + 1023) / 1024 * 1024, vec = i8_vec_ok(x, 0, dtype);
+    const dim3 g((unsigned)((a.out_dim + 15) / 16));
+    if (dtype == T_F32) k_i8_one<T_F32><<<g, 256, kp, s>>>(a, x, in_dim, kp, vec);
+    else if (dtype == T_F16) k_i8_one<T_F16><<<g, 256, kp, s>>>(a, x, in_dim, kp, vec);
+    else k_i8_one<T_BF16><<<g, 256, kp, s>>>(a, x, in_dim, kp, vec);
+    return hipGetLastError();
 }
 
 namespace {

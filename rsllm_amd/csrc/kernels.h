@@ -295,12 +295,10 @@ struct I8Args {
     uint32_t dtype_out;
 };
 hipError_t launch_i8_matmul(const I8Args &a, hipStream_t s);
-// The same from the floats x themselves (dtype, x_stride elements apart; a.xq and
-// a.xscale are not used), in one launch; hipErrorNotSupported where
-// i8_few_supported says no.
-bool i8_few_supported(int n_tok, int in_dim);
-hipError_t launch_i8_few(const I8Args &a, const void *x, size_t x_stride, int in_dim, uint32_t dtype,
-                         hipStream_t s);
+// One token (a.n_tok 1) from its floats x (dtype; a.xq and a.xscale are not used), in
+// one launch; hipErrorNotSupported where i8_one_supported says no.
+bool i8_one_supported(int in_dim);
+hipError_t launch_i8_one(const I8Args &a, const void *x, int in_dim, uint32_t dtype, hipStream_t s);
 
 // logprobs.hip: per row of logits (dtype F32, F16 or BF16, `stride` elements
 // apart) what rsllm_hip_token_logprobs_dev gives. tokens may be null (logprob
