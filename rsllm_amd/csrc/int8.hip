@@ -116,7 +116,7 @@ __device__ __forceinline__ bool i8_finite_bits(uint32_t b) { return b < 0x7F8000
 
 // A workgroup per row; the first kHeld vectors of a lane stay in registers
 // between the search for the largest magnitude and the codes, longer rows are
-// read again. Bound by reading x (2048 x 4096 bf16: see the launcher).
+// read again. Bound by reading x (2048 x 4096 bf16: 8.2 us for 25 MB, 3.1 TB/s).
 template <uint32_t DT, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_i8_quantize(const void *__restrict__ x, size_t stride,
                                                          int8_t *__restrict__ xq,
@@ -284,7 +284,9 @@ typedef int i8_v4 __attribute__((ext_vector_type(4)));
 // A workgroup's tile: BM = 16 MF WM channels x BN = 16 NF WN tokens, each
 // wavefront 16 MF x 16 NF of it; with WK > 1 the K slices of 128 bytes go round
 // the WK groups of wavefronts, whose whole-number sums are added at the end.
-// Slices of both operands are copied to LDS ST deep.
+// Slices of both operands are copied to LDS ST deep. For few tokens, where the
+// weights' stream is the floor (32 x 16 tiles, 32 tokens of 4096 x 4096: 6.0 us for
+// 17 MB, 2.8 TB/s).
 template <int WM_, int WN_, int WK_, int MF_, int NF_, int ST_> struct I8Tile {
     static constexpr int WM = WM_, WN = WN_, WK = WK_, MF = MF_, NF = NF_, ST = ST_;
     static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * WM * WN * WK;
@@ -457,7 +459,8 @@ template <class G> hipError_t i8_tile_go(const I8Args &a, hipStream_t s) {
 // the operands of the next half slice read into registers while the matrix
 // cores work on this one. One barrier a slice, in its middle: behind it the
 // next slice has landed, and every wavefront holds what is left of this one in
-// registers, so the slice after the next can be copied over it.
+// registers, so the slice after the next can be copied over it. (64 x 64 tiles, 300
+// tokens of 2048 x 4096: 9.4 us, 530 TOP/s: 160 tiles leave 96 CUs idle.)
 template <int WM_, int WN_, int MF_, int NF_, int ST_ = 2> struct I8Big {
     static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, ST = ST_;
     static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * WM * WN;
@@ -581,7 +584,10 @@ template <class G> hipError_t i8_big_go(const I8Args &a, hipStream_t s) {
 
 // The same with the ring cut finer: five units of one operand's slice, so that
 // the channels, which come from memory, are copied two slices ahead and the
-// tokens, which other workgroups read as well, one.
+// tokens, which other workgroups read as well, one. (224 x 256, 2048 tokens of
+// 14336 x 4096: 117 us with bf16 outputs, 2.06 POP/s; matrix cores busy in 47% of
+// the cycles. With two slices of 256 x 256 and f32 outputs, 28 of 133 us went with
+// the stores and another 18 with the copies to LDS.)
 template <int WM_, int WN_, int MF_, int NF_> struct I8Wide {
     static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_;
     static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * WM * WN;
@@ -753,12 +759,14 @@ hipError_t launch_i8_one(const I8Args &a, const void *x, int in_dim, uint32_t dt
 
 namespace {
 
-// A kernel of the product and what it takes, as fitted to 122 sizes (5 to 2048
-// tokens, rows of 256 to 14336, 128 to 16384 channels, weights from memory):
+// A kernel of the product and what it takes, by an estimate in us:
 //   us = c0 + r c1 + (L per CU or r) slices c2
 // with L workgroups a CU, r of them one after the other (at most `occ` run at
-// once), `slices` of 128 bytes a wavefront. The best of them by this estimate is
-// 1.3% slower on average than the fastest, and at most 24%.
+// once), `slices` of 128 bytes a wavefront. The constants are fitted to 122 sizes (3
+// to 2048 tokens, weights from memory), those of the two widest tiles set by hand
+// from a few products. Slower than the fastest of the thirteen: 1.4% on average and
+// 12% at most at those sizes; at sizes that no constant was taken from, 1.7% and 15%
+// (70 sizes, 2 to 3000 tokens) and 0.2% and 3% (40 products of 20 to 900 GOP).
 struct I8Kernel {
     hipError_t (*go)(const I8Args &, hipStream_t);
     int bm, bn, wk, occ;

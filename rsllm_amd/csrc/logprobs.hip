@@ -5,7 +5,9 @@
 // Every lane keeps m, S and D of what it has seen (S and D rescaled when m
 // rises: S' = r S, D' = r (D + (m - m') S), r = exp(m - m')), so a row is read
 // once; parts meet by the same rule. What bounds it: the read of the logits for
-// prompts, a chain of dependent loads and two launches for one row.
+// prompts (1000 x 129280 f32, 5 best: 94 us, 5.5 TB/s), two launches and the
+// lists' sorting and merging for few rows (1 x 129280, 8 best: 10.8 us; 32 x 32000
+// bf16, 20 best: 15.1, without a list 6.9).
 // Alternatives: a wavefront keeps its n_top best in order, one a lane. A logit
 // is only looked at where it beats the last of them, which in rows of no
 // particular order soon is rare (n_top (1 + log(n / n_top)) times in n); many
@@ -214,8 +216,8 @@ struct LpWork {
 };
 
 // Workgroup (chunk, row): `turns` turns, each kLpWaves * L pieces of 64 lanes x
-// 16 bytes of the row, counted from the 16 bytes that the row starts in. With one chunk a row it
-// writes the row's outputs, else its part.
+// 16 bytes of the row, counted from the 16 bytes that the row starts in. With one
+// chunk a row it writes the row's outputs, else its part.
 template <uint32_t DT>
 __global__ __launch_bounds__(64 * kLpWaves) void k_logprobs(LogprobArgs a, LpWork w, int chunks,
                                                             int turns) {
@@ -403,9 +405,7 @@ hipError_t launch_logprobs(const LogprobArgs &a, uint8_t *work, int n_tok, hipSt
         w.parts = reinterpret_cast<LpPart *>(work);
         w.tops = reinterpret_cast<LpKey *>(work + lp_round((size_t)n_tok * p.chunks * sizeof(LpPart)));
     }
-    const long long wgs = (long long)n_tok * p.chunks;
-    if (wgs > 0x7FFFFFFFll) return hipErrorInvalidValue;
-    const dim3 g((unsigned)wgs);
+    const dim3 g((unsigned)n_tok * (unsigned)p.chunks);
     if (a.dtype == T_F32) k_logprobs<T_F32><<<g, 64 * kLpWaves, 0, s>>>(a, w, p.chunks, p.turns);
     else if (a.dtype == T_F16) k_logprobs<T_F16><<<g, 64 * kLpWaves, 0, s>>>(a, w, p.chunks, p.turns);
     else k_logprobs<T_BF16><<<g, 64 * kLpWaves, 0, s>>>(a, w, p.chunks, p.turns);

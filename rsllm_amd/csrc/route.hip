@@ -1,10 +1,15 @@
 // Expert routing: router logits -> the ids and weights of each token's experts.
 //
-// Scores, keys and group sums are 64-bit, so which of two near experts is
-// chosen does not hang on a 32-bit rounding of exp; the weights are rounded
-// once at the end. An expert's place in the order is its key (score + bias), or
-// its logit itself where there is no bias (the scores rise with the logits);
-// equal places go to the lower id.
+// An expert's place in the order is its key (score + bias), or its logit itself
+// where there is no bias (the scores rise with the logits); equal places go to
+// the lower id. Which of two near experts is chosen is settled by 64-bit scores,
+// and the weights are 64-bit until their one rounding. Keys are looked at in 32
+// bits first, with a bound on their error: only what lies closer together than
+// that is worked out again.
+// Bound by its instructions for many tokens (16384 x 256 bf16, 8 of 4 of 8 groups:
+// 17.7 to 21.6 us by the logits, 1005 vector instructions a wavefront of two
+// tokens; reading 8.4 MB would take 2), by the launch and one chain of loads,
+// reductions and 64-bit scores for few (1 x 256: 5.7 us).
 #include "kernels.h"
 
 #include <type_traits>
@@ -21,8 +26,8 @@ __device__ __forceinline__ float route_load(const void *p, size_t i, uint32_t dt
 }
 
 // exp(x) to some 2^-52: x = n log 2 + r, |r| < 0.35, and the power series of exp(r)
-// up to r^12 / 12!, after Cody and Waite's reduction. (Short, where the library's is long: most calls of these
-// kernels pay for fetching their code.)
+// up to r^12 / 12!, after Cody and Waite's reduction. (Short, where the library's
+// is long: most calls of these kernels pay for fetching their code.)
 __device__ __forceinline__ double route_exp64(double x) {
     x = fmin(fmax(x, -1000.0), 1000.0);
     const double n = rint(x * 0x1.71547652b82fep+0);  // log2 e
