@@ -7,7 +7,7 @@
 // once; parts meet by the same rule. What bounds it: the read of the logits for
 // prompts (1000 x 129280 f32, 5 best: 94 us, 5.5 TB/s), two launches and the
 // lists' sorting and merging for few rows (1 x 129280, 8 best: 10.8 us; 32 x 32000
-// bf16, 20 best: 15.1, without a list 6.9).
+// bf16, 20 best: 14.3, without a list 7.0).
 // Alternatives: a wavefront keeps its n_top best in order, one a lane. A logit
 // is only looked at where it beats the last of them, which in rows of no
 // particular order soon is rare (n_top (1 + log(n / n_top)) times in n); many
@@ -20,6 +20,7 @@ namespace {
 
 constexpr float kInf = __builtin_inff();
 constexpr int kLpWaves = 4;         // wavefronts a workgroup
+constexpr int kLpFew = 8;           // chunks whose lists are merged one after another
 constexpr int kLpTurn = 16 * 64 * kLpWaves;  // elements of a turn: 16 a lane
 
 __device__ __forceinline__ float lp_one(const void *p, size_t i, uint32_t dtype) {
@@ -354,9 +355,26 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, LpWork w, i
         p.above += o.above;
     }
     p = lp_wave_join(p);
+    LpList best;
+    if (chunks <= kLpFew && a.n_top > chunks) {
+        // few and long: whole lists in order, all on their way before the first
+        // is merged in (us, so / as below: 8 x 8000, 64 best 16.4 / 26.9, 8 best
+        // 10.2 / 11.1; 32 x 32000 bf16, 64 best 21.4 / 26.8, 20 best 14.0 / 14.8,
+        // 5 best 11.6 / 11.4)
+        LpKey o[kLpFew];
+#pragma unroll
+        for (int c = 0; c < kLpFew; c++)
+            o[c] = w.tops[(at + min(c, chunks - 1)) * a.n_top + min(lane, a.n_top - 1)];
+        if (lane < a.n_top) best.top = o[0];
+        best.set_edge(a.n_top);
+#pragma unroll
+        for (int c = 1; c < kLpFew; c++)
+            if (c < chunks) best.take<true>(a.n_top, lane < a.n_top ? o[c] : LpKey{0, 0});
+        lp_finish(a, t, p, best.top);
+        return;
+    }
     // a chunk's list a lane, their i-th entries together: as soon as none of those
     // is among the best, none behind them is
-    LpList best;
     for (int c0 = 0; c0 < chunks && a.n_top; c0 += 64) {
         const bool in = c0 + lane < chunks;
         const LpKey *src = w.tops + (at + min(c0 + lane, chunks - 1)) * a.n_top;

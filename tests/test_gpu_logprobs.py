@@ -269,3 +269,20 @@ def test_rows_beyond_32_bit_offsets(hip):
         near(top[at].cpu().numpy(), want_top, b_top)
         np.testing.assert_array_equal(rank[at].cpu().numpy(), r)
         np.testing.assert_array_equal(ids[at].cpu().numpy(), want_ids)
+
+
+@pytest.mark.parametrize("parts", [2, 3, 7, 8, 9])
+def test_lists_of_parts(hip, parts):
+    """Rows cut into a few parts, lists as long as their number, one longer and 64
+    long: the best in one part, in its first or last, masked parts, equal logits
+    across parts."""
+    v = 4096 * parts - 40
+    rng = np.random.default_rng(parts)
+    x, tok = model_logits(rng, 6, v)
+    x[1, v - 100:] += 40.0
+    x[2, :100] += 40.0
+    x[3, 4000:] = -INF
+    x[4, :v - 5] = -INF
+    x[5] = rng.integers(0, 2, v)
+    for n_top in (parts, parts + 1, 64):
+        run(hip, x, tok, n_top)
