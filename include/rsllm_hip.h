@@ -342,7 +342,7 @@ int rsllm_hip_moe_routed(float *out, size_t out_len, const float *x, size_t x_le
  * n_expert, topk_group 0 or above n_group, group_top other than 1 and 2, k 0 or
  * above min(64, topk_group * n_expert / n_group), a scale that is not finite,
  * NULL pointers or logits not aligned to their elements; SHAPE_MISMATCH for
- * n_tok above 4194304 (what a launch holds), logits_stride < n_expert, logits_len < (n_tok - 1) * logits_stride + n_expert,
+ * n_tok above 8388607 (what a launch holds), logits_stride < n_expert, logits_len < (n_tok - 1) * logits_stride + n_expert,
  * bias_len other than 0 and n_expert, ids_len != n_tok * k. Enqueued on
  * `stream`; no workspace. */
 enum {
@@ -516,7 +516,7 @@ int rsllm_hip_matmul_q8_0_batch_dev(float *out, size_t out_len, const uint8_t *w
  * also takes NULL with work_len 0 (its products leave nothing between launches).
  * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for in_dim 0 or
  * above 131071 (where the sum could leave 32 bits), out_dim 0, NULL or
- * misaligned pointers; SHAPE_MISMATCH for n_tok or out_dim above 4194304 (what a
+ * misaligned pointers; SHAPE_MISMATCH for n_tok or out_dim above 8388607 (what a
  * launch holds; work_bytes is then 0), a stride below its row, x_len or out_len below (n_tok - 1) * stride + row, weights_len != out_dim * row bytes,
  * wscale_len != out_dim, bias_len other than 0 and out_dim, xq_len != n_tok *
  * row bytes, scale_len or xscale_len != n_tok, work_len below work_bytes. */
@@ -567,7 +567,7 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
  * not rise with n_tok (many rows need none): ask for each n_tok that is used.
  * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for vocab 0 or above
  * 2^31 - 1, n_top above min(64, vocab), NULL or misaligned pointers;
- * SHAPE_MISMATCH for n_tok above 4194304 (what a launch holds), logits_stride < vocab, logits_len < (n_tok - 1) *
+ * SHAPE_MISMATCH for n_tok above 8388607 (what a launch holds), logits_stride < vocab, logits_len < (n_tok - 1) *
  * logits_stride + vocab, tokens_len other than 0 and n_tok, out_len != n_tok,
  * top_len != n_tok * n_top, work_len below work_bytes. */
 size_t rsllm_hip_token_logprobs_work_bytes(size_t n_tok, size_t vocab, size_t n_top);

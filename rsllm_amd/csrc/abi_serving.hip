@@ -41,8 +41,8 @@ bool product_is(size_t a, size_t b, size_t len) {
 }
 // Rows or channels of one call. A launch holds less than 2^32 threads: these with
 // up to 512 a row, and the int8 product's tiles of as many rows and channels as
-// fit memory (2^30 threads at most, over all such sizes).
-constexpr size_t kMaxRows = (size_t)1 << 22;
+// fit memory (below 2^31 threads, over all such sizes).
+constexpr size_t kMaxRows = ((size_t)1 << 23) - 1;
 bool counts_ok(size_t n) { return n <= kMaxRows; }
 
 constexpr size_t kI8MaxIn = 131071;  // 128 * 128 * 131071 < 2^31
@@ -70,7 +70,7 @@ int check_i8(const void *out, size_t out_len, size_t out_stride, const int8_t *w
         return invalid("matmul_int8: in_dim must be 1..131071 (32-bit sums)");
     if (out_dim == 0) return invalid("matmul_int8: out_dim must be non-zero");
     if (!counts_ok(n_tok) || !counts_ok(out_dim))
-        return mismatch("matmul_int8: n_tok and out_dim must be at most 4194304");
+        return mismatch("matmul_int8: n_tok and out_dim must be at most 8388607");
     if (!product_is(out_dim, i8_row_bytes(in_dim), w_len))
         return mismatch("matmul_int8: weights must be out_dim * int8_row_bytes(in_dim)");
     if (wscale_len != out_dim) return mismatch("matmul_int8: wscale must be out_dim");
@@ -117,7 +117,7 @@ int rsllm_hip_moe_route_dev(int32_t *ids, float *weights, size_t ids_len, const 
     if (k == 0 || k > 64 || k > topk_group * (n_expert / n_group))
         return invalid("moe_route: k must be 1..min(64, experts of topk_group groups)");
     if (!std::isfinite(scale)) return invalid("moe_route: scale must be finite");
-    if (!counts_ok(n_tok)) return mismatch("moe_route: n_tok must be at most 4194304");
+    if (!counts_ok(n_tok)) return mismatch("moe_route: n_tok must be at most 8388607");
     if (logits_stride < n_expert || !span_ok(n_tok, n_expert, logits_stride, logits_len))
         return mismatch("moe_route: logits must hold n_tok rows of n_expert, logits_stride apart");
     if (bias_len != 0 && bias_len != n_expert)
@@ -151,7 +151,7 @@ int rsllm_hip_quantize_int8_dev(const void *x, size_t x_len, size_t x_stride, in
                                 size_t in_dim, uint32_t dtype, rsllm_hip_stream_t stream) {
     if (in_dim == 0 || in_dim > kI8MaxIn)
         return invalid("quantize_int8: in_dim must be 1..131071");
-    if (!counts_ok(n_tok)) return mismatch("quantize_int8: n_tok must be at most 4194304");
+    if (!counts_ok(n_tok)) return mismatch("quantize_int8: n_tok must be at most 8388607");
     if (const int rc = check_x("quantize_int8: x must hold n_tok rows of in_dim, x_stride apart", x,
                                x_len, x_stride, n_tok, in_dim, dtype))
         return rc;
@@ -241,7 +241,7 @@ int rsllm_hip_token_logprobs_dev(float *logprob, float *entropy, int32_t *rank, 
         return set_error(RSLLM_HIP_ERR_UNIMPLEMENTED, "token_logprobs: dtype not implemented");
     if (vocab == 0 || vocab > (size_t)INT_MAX) return invalid("token_logprobs: vocab must be 1..2^31-1");
     if (n_top > 64 || n_top > vocab) return invalid("token_logprobs: n_top must be at most min(64, vocab)");
-    if (!counts_ok(n_tok)) return mismatch("token_logprobs: n_tok must be at most 4194304");
+    if (!counts_ok(n_tok)) return mismatch("token_logprobs: n_tok must be at most 8388607");
     if (logits_stride < vocab || !span_ok(n_tok, vocab, logits_stride, logits_len))
         return mismatch("token_logprobs: logits must hold n_tok rows of vocab, logits_stride apart");
     if (tokens_len != 0 && tokens_len != n_tok)

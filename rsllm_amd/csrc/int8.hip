@@ -455,7 +455,7 @@ template <class G> hipError_t i8_tile_go(const I8Args &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// The same product for many tokens: WM x WN wavefronts, two slices in LDS, and
+// The same product for many tokens: WM x WN wavefronts, ST slices in LDS, and
 // the operands of the next half slice read into registers while the matrix
 // cores work on this one. One barrier a slice, in its middle: behind it the
 // next slice has landed, and every wavefront holds what is left of this one in

@@ -204,20 +204,20 @@ def test_logprobs_refuses_a_short_workspace(hip):
                          work_len=need - 1)
 
 
-LIMIT = 1 << 22  # rows and channels of one call: what every launch's grid can hold
+LIMIT = (1 << 23) - 1  # rows and channels of one call: what every launch's grid can hold
 
 
 def test_more_rows_or_channels_than_a_launch_holds(hip):
     n = LIMIT + 1
-    with pytest.raises(hip.ShapeMismatch, match="4194304"):
+    with pytest.raises(hip.ShapeMismatch, match="8388607"):
         route(hip, n_tok=n, ids_len=2 * n, logits_len=16 * n)
-    with pytest.raises(hip.ShapeMismatch, match="4194304"):
+    with pytest.raises(hip.ShapeMismatch, match="8388607"):
         quantize(hip, n_tok=n, x_len=1 << 40, xq_len=n * 128, scale_len=n)
     for call in (prequant, oneshot):
         for kw in (dict(n_tok=n), dict(out_dim=n, out_stride=n)):
-            with pytest.raises(hip.ShapeMismatch, match="4194304"):
+            with pytest.raises(hip.ShapeMismatch, match="8388607"):
                 call(hip, **kw)
-    with pytest.raises(hip.ShapeMismatch, match="4194304"):
+    with pytest.raises(hip.ShapeMismatch, match="8388607"):
         logprobs(hip, n_tok=n, out_len=n, top_len=0, n_top=0, logits_len=1 << 40, tokens_len=n)
     assert hip.int8_work_bytes(n, 64, 64) == hip.int8_work_bytes(64, 64, n) == 0
     assert hip.int8_work_bytes(LIMIT, 64, LIMIT) > 0
