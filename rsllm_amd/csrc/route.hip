@@ -368,23 +368,31 @@ __device__ __forceinline__ bool route_choose(const RouteArgs &a, const RouteForm
                     b0 = max(b0, c0);
                 }
             }
-            uint32_t sum = a.group_top == 2 && b1 ? route_order(route_value(b0) + route_value(b1) + 0.0f) : b0;
-            if (in_group != 0 || g >= a.n_group) sum = 0;
-            uint32_t last = 0;
+            // What the group counts, and how far that may be off: its two scores (off),
+            // and with K its larger key 2^-24 K for each key's rounding and twice that
+            // for the sum's and for the edge's below. K, not the sum: of keys of opposite
+            // signs little may be left.
+            const bool two = a.group_top == 2 && b1, first = in_group == 0 && g < a.n_group && b0;
+            const float v0 = route_value(b0), v1 = two ? route_value(b1) : 0.0f;
+            const float count = v0 + v1 + 0.0f, far = off + 0x1.9p-22f * fmaxf(fabsf(v0), fabsf(v1));
+            uint32_t sum = first ? route_order(count) : 0;
             bool kept = false;
             for (int r = 0; r < a.topk_group; r++) {
                 const uint32_t best = route_max<W>(sum);
                 const int who = route_first<W>(sum == best && best != 0);
                 kept |= who == head;
-                last = best ? best : last;
                 if (who == sub) sum = 0;
             }
-            // the last kept against the best one left out (half the gap: sums of two)
-            const uint32_t next = route_max<W>(sum);
-            const bool near = next && !route_apart(0.5f * route_value(last), 0.5f * route_value(next), off);
+            // the least that a kept group may count against the most of one left out (a
+            // count beyond f32: anything)
+            const float to = kept ? -far : far;
+            const uint32_t edge = route_order(fabsf(count) < -none ? count + to : kept ? none : -none);
+            const uint32_t low = ~route_max<W>(first && kept ? ~edge : 0), high = route_max<W>(first && !kept ? edge : 0);
+            const bool near = high && low <= high;
             if (__ballot(near)) {
                 // groups of one key each are equal where the logits and biases are
                 bool unsure = near && a.group_top == 2;
+                const uint32_t last = ~route_max<W>(first && kept ? ~route_order(count) : 0);
                 uint32_t l = 0, b = 0;
 #pragma unroll
                 for (int j = 0; j < R; j++)
