@@ -1,0 +1,39 @@
+"""Which kernel the int8 product launches: on the host, with no kernel run."""
+import re
+
+import hip_recorder
+from int8_cases import CASES, TILES
+
+CALL = """
+def go(t, k, n):
+    rb = B.int8_row_bytes(k)
+    B.matmul_int8_prequant_dev(4096, t * n, n, 4096, n * rb, 4096, n, 0, 0, 4096, t * rb, 4096, t, 0, 0, t, k, n)
+    return rec.rec_take().decode()
+"""
+
+
+def tile(name):
+    """Channels x tokens of a kernel, from its (mangled) template arguments."""
+    n = [int(v) for v in re.findall(r"Li(\d+)E", name)]
+    if "I8Tile" in name:
+        wm, wn, _, mf, nf, _ = n
+    else:
+        wm, wn, mf, nf = n[:4]
+    return 16 * mf * wm, 16 * nf * wn
+
+
+def test_every_kernel_is_reached(tmp_path):
+    """The sizes that test_gpu_int8_tiles.py compares go to the kernels they stand
+    for, and no kernel is without some."""
+    out = hip_recorder.run(tmp_path, CALL + f"""
+for i in range(rec.rec_kernels()):
+    name = rec.rec_kernel(i).decode()
+    if any(k in name for k in ("k_i8_tile", "k_i8_big", "k_i8_wide")):
+        print("has", name)
+for t, k, n in {[c[1:] for c in CASES]!r}:
+    print("ran", go(t, k, n))
+""").split("\n")
+    has = {tile(line) for line in out if line.startswith("has")}
+    ran = [tile(line) for line in out if line.startswith("ran")]
+    assert has == set(TILES)
+    assert ran == [c[0] for c in CASES]
