@@ -2,6 +2,7 @@
 #include "buffer_lds.h"
 #include "kernels.h"
 
+#include <atomic>
 #include <type_traits>
 
 namespace rsllm_hip {
@@ -445,10 +446,20 @@ __global__ __launch_bounds__(G::kThreads) void k_i8_tile(I8Args a, int n_ct, int
     }
 }
 
+// More LDS than a kernel gets unasked, asked for until the runtime has granted it once:
+// a refusal is that call's error alone.
+template <class G> hipError_t i8_allow_lds(const void *kernel) {
+    static std::atomic<bool> granted{false};
+    if (granted.load(std::memory_order_acquire)) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+    if (e == hipSuccess) granted.store(true, std::memory_order_release);
+    else (void)hipGetLastError();  // (or the next launch would report it)
+    return e;
+}
+
 template <class G> hipError_t i8_tile_go(const I8Args &a, hipStream_t s) {
-    static const hipError_t attr = hipFuncSetAttribute(
-        reinterpret_cast<const void *>(&k_i8_tile<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-    if (attr != hipSuccess) return attr;
+    const hipError_t e = i8_allow_lds<G>(reinterpret_cast<const void *>(&k_i8_tile<G>));
+    if (e != hipSuccess) return e;
     const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
     const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
     k_i8_tile<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);
@@ -573,9 +584,8 @@ __global__ __launch_bounds__(G::kThreads) void k_i8_big(I8Args a, int n_ct, int 
 }
 
 template <class G> hipError_t i8_big_go(const I8Args &a, hipStream_t s) {
-    static const hipError_t attr = hipFuncSetAttribute(
-        reinterpret_cast<const void *>(&k_i8_big<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-    if (attr != hipSuccess) return attr;
+    const hipError_t e = i8_allow_lds<G>(reinterpret_cast<const void *>(&k_i8_big<G>));
+    if (e != hipSuccess) return e;
     const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
     const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
     k_i8_big<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);
@@ -702,9 +712,8 @@ __global__ __launch_bounds__(G::kThreads) void k_i8_wide(I8Args a, int n_ct, int
 }
 
 template <class G> hipError_t i8_wide_go(const I8Args &a, hipStream_t s) {
-    static const hipError_t attr = hipFuncSetAttribute(
-        reinterpret_cast<const void *>(&k_i8_wide<G>), hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-    if (attr != hipSuccess) return attr;
+    const hipError_t e = i8_allow_lds<G>(reinterpret_cast<const void *>(&k_i8_wide<G>));
+    if (e != hipSuccess) return e;
     const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
     const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
     k_i8_wide<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);

@@ -1,4 +1,5 @@
-"""Which kernel the int8 product launches: on the host, with no kernel run."""
+"""Which kernel the int8 product launches, and what it does when the runtime
+refuses one: on the host, with no kernel run."""
 import re
 
 import hip_recorder
@@ -37,3 +38,24 @@ for t, k, n in {[c[1:] for c in CASES]!r}:
     ran = [tile(line) for line in out if line.startswith("ran")]
     assert has == set(TILES)
     assert ran == [c[0] for c in CASES]
+
+
+def test_a_refused_attribute_is_asked_for_again(tmp_path):
+    """A runtime that cannot set a kernel's LDS size fails that call alone: the next
+    one asks again."""
+    sizes = [sizes[0] for sizes in TILES.values()]
+    out = hip_recorder.run(tmp_path, CALL + f"""
+for t, k, n in {sizes!r}:
+    rec.rec_fail(1)
+    try:
+        go(t, k, n)
+        print("launched")
+    except B.Error as e:
+        print("refused")
+    try:
+        print(go(t, k, n))
+    except B.Error as e:
+        print("refused again")
+""").split("\n")[:-1]
+    assert out[::2] == ["refused"] * len(sizes)
+    assert [tile(o) for o in out[1::2] if o != "refused again"] == list(TILES)
