@@ -446,13 +446,17 @@ __global__ __launch_bounds__(G::kThreads) void k_i8_tile(I8Args a, int n_ct, int
     }
 }
 
-// More LDS than a kernel gets unasked, asked for until the runtime has granted it once:
-// a refusal is that call's error alone.
+// More LDS than a kernel gets unasked, asked for until the runtime has granted it once
+// on the current device: a refusal is that call's error alone.
 template <class G> hipError_t i8_allow_lds(const void *kernel) {
-    static std::atomic<bool> granted{false};
-    if (granted.load(std::memory_order_acquire)) return hipSuccess;
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
-    if (e == hipSuccess) granted.store(true, std::memory_order_release);
+    static std::atomic<uint64_t> granted{0};  // a bit a device; beyond 64 it is asked every time
+    int dev;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (granted.load(std::memory_order_acquire) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::kLds);
+    if (e == hipSuccess) granted.fetch_or(bit, std::memory_order_release);
     else (void)hipGetLastError();  // (or the next launch would report it)
     return e;
 }

@@ -14,7 +14,7 @@ typedef struct { unsigned x, y, z; } dim3_t;
 enum { MAX = 8192 };
 static const void *key[MAX];
 static const char *name[MAX];
-static int n_key, n_call, fail, last; /* last: as hipGetLastError gives it */
+static int n_key, n_call, fail, last, device, set; /* last: as hipGetLastError gives it */
 static const char *call[MAX];
 static dim3_t grid, block;
 static size_t shared;
@@ -43,13 +43,19 @@ int hipLaunchKernel(const void *f, dim3_t g, dim3_t b, void **a, size_t l, void 
 }
 int hipFuncSetAttribute(const void *f, int attr, int value) {
     if (fail > 0) { fail--; return last = 2; } /* hipErrorOutOfMemory */
+    set++;
     return 0;
 }
-int hipGetDevice(int *d) { *d = 0; return 0; }
-int hipSetDevice(int d) { return 0; }
+int hipGetDevice(int *d) { *d = device; return 0; }
+int hipSetDevice(int d) { device = d; return 0; }
+int hipGetDeviceCount(int *n) { *n = 2; return 0; }
+int hipStreamCreateWithFlags(void **s, unsigned f) { *s = &device; return 0; }
+int hipStreamDestroy(void *s) { return 0; }
+int hipGetSymbolAddress(void **p, const void *s) { *p = &device; return 0; }
 int hipGetLastError(void) { int e = last; last = 0; return e; }
 
 void rec_fail(int n) { fail = n; } /* the next n hipFuncSetAttribute */
+int rec_set(void) { int n = set; set = 0; return n; } /* hipFuncSetAttribute granted since */
 int rec_kernels(void) { return n_key; }
 const char *rec_kernel(int i) { return name[i]; }
 const char *rec_take(void) { return n_call ? call[--n_call] : ""; } /* the last one */

@@ -1,5 +1,5 @@
-"""Which kernel the int8 product launches, and what it does when the runtime
-refuses one: on the host, with no kernel run."""
+"""Which kernel the int8 product launches, and what it asks of the runtime first: on
+the host, with no kernel run."""
 import re
 
 import hip_recorder
@@ -59,3 +59,18 @@ for t, k, n in {sizes!r}:
 """).split("\n")[:-1]
     assert out[::2] == ["refused"] * len(sizes)
     assert [tile(o) for o in out[1::2] if o != "refused again"] == list(TILES)
+
+
+def test_each_device_is_asked(tmp_path):
+    """The LDS size is a kernel's on one device: after rsllm_hip_init of another it is
+    asked for there, too, and once on each."""
+    sizes = [sizes[0] for sizes in TILES.values()]
+    out = hip_recorder.run(tmp_path, CALL + f"""
+for device in (0, 1, 0, 1):
+    B.init(device)
+    rec.rec_set()
+    for t, k, n in {sizes!r}:
+        go(t, k, n)
+    print(rec.rec_set())
+""").split()
+    assert out == [str(len(sizes)), str(len(sizes)), "0", "0"]
