@@ -558,7 +558,9 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
  * +inf logits share the row evenly. A NaN anywhere in a row makes its logprob,
  * entropy and listed log-probabilities NaN (a NaN logit is not listed or counted).
  * A token id outside [0, vocab) gives logprob NaN and rank 0, a token whose
- * logit is NaN rank 0.
+ * logit is NaN rank 0. The sums are f32, so log-probabilities and entropies are
+ * off by a few 2^-24 of 1 beside their own rounding: a token whose p is within
+ * 2^-24 of 1 gets logprob 0.
  * tokens (with tokens_len 0) may be NULL: logprob and rank are then not written
  * and may be NULL; rank and entropy may be NULL; n_top 0 takes NULL lists.
  * out_len counts logprob, rank and entropy each. `work`:

@@ -757,9 +757,11 @@ hipError_t launch_i8_quantize(const void *x, size_t stride, int8_t *xq, float *s
 
 bool i8_one_supported(int in_dim) { return in_dim <= 60 * 1024; }  // its codes in LDS
 
-// One token, us, against the quantiser and a tile product: 14336 x 4096 f32 14.4 /
-// 17.1 (59 MB: 4.1 TB/s), 4096 x 14336 18.4 / 18.7 (bf16 15.7 / 17.4), 4096 x 4096
-// bf16 5.7 / 7.5, 1024 x 1024 2.9 / 5.3.
+// One token, us, against the quantiser and a tile product, the weights from memory:
+// 14336 x 4096 f32 14.4 / 17.1 (59 MB: 4.1 TB/s; 13.0 where three matrices take turns,
+// which the cache behind L2 holds in part; a launch that only reads as much 10.2 and
+// 9.2), 4096 x 14336 18.4 / 18.7 (bf16 15.7 / 17.4), 4096 x 4096 bf16 5.7 / 7.5,
+// 1024 x 1024 2.9 / 5.3.
 hipError_t launch_i8_one(const I8Args &a, const void *x, int in_dim, uint32_t dtype, hipStream_t s) {
     if (!i8_one_supported(in_dim) || a.n_tok != 1) return hipErrorNotSupported;
     const int kp = (in_dim + 1023) / 1024 * 1024, vec = i8_vec_ok(x, 0, dtype);

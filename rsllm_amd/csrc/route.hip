@@ -7,9 +7,9 @@
 // bits first, with a bound on their error: only what lies closer together than
 // that is worked out again.
 // Bound by its instructions for many tokens (16384 x 256 bf16, 8 of 4 of 8 groups:
-// 17.7 to 21.6 us by the logits, 1005 vector instructions a wavefront of two
-// tokens; reading 8.4 MB would take 2), by the launch and one chain of loads,
-// reductions and 64-bit scores for few (1 x 256: 5.7 us).
+// 17.4 to 18.3 us, 1012 vector instructions a wavefront of two tokens; reading 8.4 MB
+// would take 1.3; up to 24 us where a token or two is done over in 64 bits), by the
+// launch and one chain of loads, reductions and 64-bit scores for few (1 x 256: 5.7 us).
 #include "kernels.h"
 
 #include <type_traits>
