@@ -540,6 +540,126 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
                               size_t in_dim, size_t out_dim, uint32_t dtype_x, uint32_t dtype_out,
                               rsllm_hip_stream_t stream);
 
+/* ---- microscaled 4-bit floating point ------------------------------------------
+ * No reference counterpart (the formats it reads are GGUF's): rows of 4-bit codes
+ * with an 8-bit scale for every 32 of them, the OCP Microscaling format MXFP4.
+ * A code's low three bits stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6, its high bit for the
+ * sign; a scale byte s stands for 2^(s - 127), 255 for NaN. Code i of a row is the low
+ * (i even) or high half of byte i / 2, scale b that of codes 32 b .. 32 b + 31.
+ * Rows of codes lie rsllm_hip_mxfp4_row_bytes(in_dim) = in_dim / 2 rounded up to 64
+ * bytes apart, rows of scales rsllm_hip_mxfp4_scale_bytes(in_dim) = a byte a block
+ * rounded up to 16; both 16-byte aligned. The quantiser fills the rest of its rows
+ * with zeros; of a weight row, what stands behind in_dim does not matter. Both give 0
+ * for an in_dim outside 1..1048576.
+ * rsllm_hip_quantize_mxfp4_dev: n_rows rows (tokens, or weight channels) of in_dim
+ * values of `dtype` (F32, F16 or BF16), x_stride elements apart. Per block
+ *   s    = 127 + max(-127, floor(log2(max |x|)) - 2)   (0 for a block of zeros)
+ *   code = x / 2^(s - 127) to the nearest, halves to the even code, at most +-6
+ * A block with a non-finite value gets s = 255 and codes of 0: it stands for NaN.
+ * rsllm_hip_dequantize_mxfp4_dev: the values that codes stand for, in f32 (which holds
+ * them exactly up to its largest number) rounded once to `dtype`; what lies between
+ * rows of out is left as it was.
+ * rsllm_hip_matmul_mxfp4_prequant_dev: the product of two such matrices, xcodes
+ * [n_tok x in_dim] and weights [out_dim x in_dim], zeros behind in_dim in xcodes:
+ *   out[t, o] = sum_b 2^(sx[t, b] + sw[o, b] - 254) (sum_i x[t, i] w[o, i]) + bias[o]
+ * summed in f32 (the matrix cores' order), rows of dtype_out (F32, F16 or BF16; rounded
+ * once from f32) out_stride elements apart; bias: out_dim values or NULL. A NaN block
+ * makes its token's, or its channel's, outputs NaN.
+ * rsllm_hip_matmul_mxfp4_dev takes floats x and quantises them on the way: the same
+ * result, bit for bit, as the quantiser and the prequant form.
+ * `work`: rsllm_hip_mxfp4_work_bytes(n_tok, in_dim, out_dim) bytes of the caller's (0
+ * for sizes that are refused), 256-byte aligned, used by this call alone until it has run:
+ * calls that may overlap, and graphs that may replay at once, get one each.
+ * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for in_dim 0 or above
+ * 1048576, out_dim 0, NULL or misaligned pointers; SHAPE_MISMATCH for n_rows, n_tok or
+ * out_dim above 8388607 (what a launch holds), a stride below its row, x_len or out_len
+ * below (rows - 1) * stride + row, code and scale lengths that are not rows * row bytes
+ * and rows * scale bytes, bias_len other than 0 and out_dim, work_len below
+ * work_bytes. */
+size_t rsllm_hip_mxfp4_row_bytes(size_t in_dim);
+size_t rsllm_hip_mxfp4_scale_bytes(size_t in_dim);
+size_t rsllm_hip_mxfp4_work_bytes(size_t n_tok, size_t in_dim, size_t out_dim);
+int rsllm_hip_quantize_mxfp4_dev(const void *x, size_t x_len, size_t x_stride, uint8_t *codes,
+                                 size_t codes_len, uint8_t *scales, size_t scales_len,
+                                 size_t n_rows, size_t in_dim, uint32_t dtype,
+                                 rsllm_hip_stream_t stream);
+int rsllm_hip_dequantize_mxfp4_dev(const uint8_t *codes, size_t codes_len, const uint8_t *scales,
+                                   size_t scales_len, void *out, size_t out_len,
+                                   size_t out_stride, size_t n_rows, size_t in_dim, uint32_t dtype,
+                                   rsllm_hip_stream_t stream);
+int rsllm_hip_matmul_mxfp4_prequant_dev(void *out, size_t out_len, size_t out_stride,
+                                        const uint8_t *weights, size_t weights_len,
+                                        const uint8_t *wscales, size_t wscales_len,
+                                        const float *bias, size_t bias_len, const uint8_t *xcodes,
+                                        size_t xcodes_len, const uint8_t *xscales,
+                                        size_t xscales_len, uint8_t *work, size_t work_len,
+                                        size_t n_tok, size_t in_dim, size_t out_dim,
+                                        uint32_t dtype_out, rsllm_hip_stream_t stream);
+int rsllm_hip_matmul_mxfp4_dev(void *out, size_t out_len, size_t out_stride,
+                               const uint8_t *weights, size_t weights_len, const uint8_t *wscales,
+                               size_t wscales_len, const float *bias, size_t bias_len,
+                               const void *x, size_t x_len, size_t x_stride, uint8_t *work,
+                               size_t work_len, size_t n_tok, size_t in_dim, size_t out_dim,
+                               uint32_t dtype_x, uint32_t dtype_out, rsllm_hip_stream_t stream);
+
+/* ---- a whole mixture-of-experts layer for a few tokens ----------------------------
+ * What the reference does between a layer's norm and its residual (the router's product,
+ * moe_topk_route, accumulate_moe_outputs, apply_shared_expert; models/src/dsv4/moe.rs:
+ * 235-707), for up to 32 tokens and expert weights in MXFP4. Per token:
+ *   l_e   = sum_i router[e, i] x[i]                      (in 64 bits)
+ *   ids, weights of the k chosen experts: as rsllm_hip_moe_route_dev gives them for
+ *           the logits l (in 64 bits), score, bias, groups, renormalise and scale
+ *   h_e   = silu(min(gate_e x, c)) * clamp(up_e x, -c, c)  (no clamp when c <= 1e-6)
+ *   out   = sum_i weights_i down_{ids_i} h_{ids_i} + sum_j down_{n_expert + j} h_{n_expert + j}
+ * the second sum over the n_shared experts that every token takes, which stand behind
+ * the others in the weights. Experts of weight 0 are skipped. x and h are not
+ * quantised: the products take x exactly, and h rounded to 24 bits (f32 outputs) or 16
+ * (f16 and bf16 ones), and sum in f32. A token with a non-finite value in x gets a row
+ * of NaN (its ids and weights by the rules above, whatever its logits became).
+ * The layer: `router` [n_expert x n_embd] of dtype_router (F32, F16 or BF16; router_len
+ * elements), `bias` n_expert values or NULL (bias_len 0); gate, up: (n_expert +
+ * n_shared) * n_ff rows of n_embd codes (gate_up_len bytes each, their scales
+ * gate_up_scales_len); down: (n_expert + n_shared) * n_embd rows of n_ff codes. Rows as
+ * the quantiser lays them out.
+ * out: n_tok rows of n_embd values of dtype_out (F32, F16 or BF16), overwritten,
+ * out_stride elements apart; x: rows of dtype_x likewise; ids, weights [n_tok x k] are
+ * written. out must not overlap x. `work`: rsllm_hip_moe_mxfp4_work_bytes(layer, n_tok)
+ * bytes of the caller's (0 for a layer or n_tok that is refused), 256-byte aligned, used
+ * by this call alone until it has run; what it holds before does not matter. The struct
+ * is read during the call only; what it points to until the work is done.
+ * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for n_tok above 32, n_embd
+ * or n_ff 0 or above 65536, n_expert 0 or above 1024, n_shared above 8, k 0 or above
+ * min(32, experts of topk_group groups), n_group that does not divide n_expert,
+ * topk_group outside 1..n_group, group_top other than 1 or 2, an unknown score, a
+ * scale that is not finite, a NaN clamp, NULL or misaligned pointers; SHAPE_MISMATCH for a stride
+ * below its row, lengths below or other than those above, work_len below work_bytes. */
+typedef struct rsllm_hip_moe_mxfp4 {
+    const void *router;
+    size_t router_len;
+    const float *bias;
+    size_t bias_len;
+    const uint8_t *gate, *up;
+    size_t gate_up_len;
+    const uint8_t *gate_scales, *up_scales;
+    size_t gate_up_scales_len;
+    const uint8_t *down;
+    size_t down_len;
+    const uint8_t *down_scales;
+    size_t down_scales_len;
+    size_t n_embd, n_ff, n_expert, n_shared, k, n_group, topk_group, group_top;
+    uint32_t dtype_router;
+    uint32_t score; /* RSLLM_HIP_SCORE_* */
+    int32_t renormalise;
+    float scale;
+    float clamp;
+} rsllm_hip_moe_mxfp4;
+size_t rsllm_hip_moe_mxfp4_work_bytes(const rsllm_hip_moe_mxfp4 *layer, size_t n_tok);
+int rsllm_hip_moe_mxfp4_dev(const rsllm_hip_moe_mxfp4 *layer, void *out, size_t out_len,
+                            size_t out_stride, int32_t *ids, float *weights, size_t ids_len,
+                            const void *x, size_t x_len, size_t x_stride, uint8_t *work,
+                            size_t work_len, size_t n_tok, uint32_t dtype_x, uint32_t dtype_out,
+                            rsllm_hip_stream_t stream);
+
 /* ---- token log-probabilities --------------------------------------------------
  * No reference counterpart among its compute ops: what a caller reads from the
  * vocabulary projection's product (matmul_weight_f32 or one of the others)

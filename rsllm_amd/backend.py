@@ -129,6 +129,25 @@ class ModelInfo(ctypes.Structure):
                 ("n_tensors", ctypes.c_uint32)]
 
 
+class MoeMxfp4(ctypes.Structure):
+    """rsllm_hip_moe_mxfp4: a mixture-of-experts layer's weights (device pointers) and
+    numbers, for moe_mxfp4_dev."""
+    _fields_ = [("router", ctypes.c_void_p), ("router_len", ctypes.c_size_t),
+                ("bias", ctypes.c_void_p), ("bias_len", ctypes.c_size_t),
+                ("gate", ctypes.c_void_p), ("up", ctypes.c_void_p),
+                ("gate_up_len", ctypes.c_size_t), ("gate_scales", ctypes.c_void_p),
+                ("up_scales", ctypes.c_void_p), ("gate_up_scales_len", ctypes.c_size_t),
+                ("down", ctypes.c_void_p), ("down_len", ctypes.c_size_t),
+                ("down_scales", ctypes.c_void_p), ("down_scales_len", ctypes.c_size_t),
+                ("n_embd", ctypes.c_size_t), ("n_ff", ctypes.c_size_t),
+                ("n_expert", ctypes.c_size_t), ("n_shared", ctypes.c_size_t),
+                ("k", ctypes.c_size_t), ("n_group", ctypes.c_size_t),
+                ("topk_group", ctypes.c_size_t), ("group_top", ctypes.c_size_t),
+                ("dtype_router", ctypes.c_uint32), ("score", ctypes.c_uint32),
+                ("renormalise", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("clamp", ctypes.c_float)]
+
+
 # Every symbol include/rsllm_hip.h declares, with its ctypes signature.
 _P, _S, _U32, _I = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_int
 SIGNATURES = {
@@ -181,6 +200,18 @@ SIGNATURES = {
                                             _S, _S, _S, _S, _U32, _P], _I),
     "rsllm_hip_matmul_int8_dev": ([_P, _S, _S, _P, _S, _P, _S, _P, _S, _P, _S, _S, _P, _S, _S, _S,
                                    _S, _U32, _U32, _P], _I),
+    "rsllm_hip_mxfp4_row_bytes": ([_S], _S),
+    "rsllm_hip_mxfp4_scale_bytes": ([_S], _S),
+    "rsllm_hip_mxfp4_work_bytes": ([_S, _S, _S], _S),
+    "rsllm_hip_quantize_mxfp4_dev": ([_P, _S, _S, _P, _S, _P, _S, _S, _S, _U32, _P], _I),
+    "rsllm_hip_dequantize_mxfp4_dev": ([_P, _S, _P, _S, _P, _S, _S, _S, _S, _U32, _P], _I),
+    "rsllm_hip_matmul_mxfp4_prequant_dev": ([_P, _S, _S, _P, _S, _P, _S, _P, _S, _P, _S, _P, _S, _P,
+                                             _S, _S, _S, _S, _U32, _P], _I),
+    "rsllm_hip_matmul_mxfp4_dev": ([_P, _S, _S, _P, _S, _P, _S, _P, _S, _P, _S, _S, _P, _S, _S, _S,
+                                    _S, _U32, _U32, _P], _I),
+    "rsllm_hip_moe_mxfp4_work_bytes": ([ctypes.POINTER(MoeMxfp4), _S], _S),
+    "rsllm_hip_moe_mxfp4_dev": ([ctypes.POINTER(MoeMxfp4), _P, _S, _S, _P, _P, _S, _P, _S, _S, _P,
+                                 _S, _S, _U32, _U32, _P], _I),
     "rsllm_hip_token_logprobs_work_bytes": ([_S, _S, _S], _S),
     "rsllm_hip_token_logprobs_dev": ([_P, _P, _P, _S, _P, _P, _S, _P, _S, _S, _P, _S, _P, _S, _S,
                                       _S, _S, _U32, _P], _I),
@@ -607,6 +638,84 @@ def matmul_int8_dev(out_ptr: int, out_len: int, out_stride: int, w_ptr: int, w_l
                                          stream or None))
 
 
+def mxfp4_row_bytes(in_dim: int) -> int:
+    """Bytes from one row of 4-bit codes to the next (in_dim / 2 rounded up to 64)."""
+    return LIB.rsllm_hip_mxfp4_row_bytes(in_dim)
+
+
+def mxfp4_scale_bytes(in_dim: int) -> int:
+    """Bytes from one row's scales to the next's (one for 32 codes, rounded up to 16)."""
+    return LIB.rsllm_hip_mxfp4_scale_bytes(in_dim)
+
+
+def mxfp4_work_bytes(n_tok: int, in_dim: int, out_dim: int) -> int:
+    """Workspace of matmul_mxfp4_dev and matmul_mxfp4_prequant_dev."""
+    return LIB.rsllm_hip_mxfp4_work_bytes(n_tok, in_dim, out_dim)
+
+
+def quantize_mxfp4_dev(x_ptr: int, x_len: int, x_stride: int, codes_ptr: int, codes_len: int,
+                       scales_ptr: int, scales_len: int, n_rows: int, in_dim: int,
+                       dtype=GgmlType.F32, stream: int = 0) -> None:
+    """Rows of floats (tokens, or weight channels) -> 4-bit codes and a scale byte
+    for every 32 of them."""
+    _check(LIB.rsllm_hip_quantize_mxfp4_dev(x_ptr or None, x_len, x_stride, codes_ptr or None,
+                                            codes_len, scales_ptr or None, scales_len, n_rows,
+                                            in_dim, int(dtype), stream or None))
+
+
+def dequantize_mxfp4_dev(codes_ptr: int, codes_len: int, scales_ptr: int, scales_len: int,
+                         out_ptr: int, out_len: int, out_stride: int, n_rows: int, in_dim: int,
+                         dtype=GgmlType.F32, stream: int = 0) -> None:
+    """The values that rows of 4-bit codes stand for."""
+    _check(LIB.rsllm_hip_dequantize_mxfp4_dev(codes_ptr or None, codes_len, scales_ptr or None,
+                                              scales_len, out_ptr or None, out_len, out_stride,
+                                              n_rows, in_dim, int(dtype), stream or None))
+
+
+def matmul_mxfp4_prequant_dev(out_ptr: int, out_len: int, out_stride: int, w_ptr: int, w_len: int,
+                              wscales_ptr: int, wscales_len: int, bias_ptr: int, bias_len: int,
+                              xcodes_ptr: int, xcodes_len: int, xscales_ptr: int,
+                              xscales_len: int, work_ptr: int, work_len: int, n_tok: int,
+                              in_dim: int, out_dim: int, dtype_out=GgmlType.F32,
+                              stream: int = 0) -> None:
+    """matmul_mxfp4_dev on the codes quantize_mxfp4_dev made."""
+    _check(LIB.rsllm_hip_matmul_mxfp4_prequant_dev(
+        out_ptr or None, out_len, out_stride, w_ptr or None, w_len, wscales_ptr or None,
+        wscales_len, bias_ptr or None, bias_len, xcodes_ptr or None, xcodes_len,
+        xscales_ptr or None, xscales_len, work_ptr or None, work_len, n_tok, in_dim, out_dim,
+        int(dtype_out), stream or None))
+
+
+def matmul_mxfp4_dev(out_ptr: int, out_len: int, out_stride: int, w_ptr: int, w_len: int,
+                     wscales_ptr: int, wscales_len: int, bias_ptr: int, bias_len: int, x_ptr: int,
+                     x_len: int, x_stride: int, work_ptr: int, work_len: int, n_tok: int,
+                     in_dim: int, out_dim: int, dtype_x=GgmlType.F32, dtype_out=GgmlType.F32,
+                     stream: int = 0) -> None:
+    """x quantised to 4 bits with a scale for every 32 values, times such weights (and
+    a bias): out rows of dtype_out."""
+    _check(LIB.rsllm_hip_matmul_mxfp4_dev(
+        out_ptr or None, out_len, out_stride, w_ptr or None, w_len, wscales_ptr or None,
+        wscales_len, bias_ptr or None, bias_len, x_ptr or None, x_len, x_stride, work_ptr or None,
+        work_len, n_tok, in_dim, out_dim, int(dtype_x), int(dtype_out), stream or None))
+
+
+def moe_mxfp4_work_bytes(layer: MoeMxfp4, n_tok: int) -> int:
+    """Workspace of moe_mxfp4_dev."""
+    return LIB.rsllm_hip_moe_mxfp4_work_bytes(ctypes.byref(layer), n_tok)
+
+
+def moe_mxfp4_dev(layer: MoeMxfp4, out_ptr: int, out_len: int, out_stride: int, ids_ptr: int,
+                  weights_ptr: int, ids_len: int, x_ptr: int, x_len: int, x_stride: int,
+                  work_ptr: int, work_len: int, n_tok: int, dtype_x=GgmlType.F32,
+                  dtype_out=GgmlType.F32, stream: int = 0) -> None:
+    """A mixture-of-experts layer for up to 32 tokens: router, choice of experts, their
+    SwiGLU products and the experts every token takes, weighted and summed."""
+    _check(LIB.rsllm_hip_moe_mxfp4_dev(ctypes.byref(layer), out_ptr or None, out_len, out_stride,
+                                       ids_ptr or None, weights_ptr or None, ids_len, x_ptr or None,
+                                       x_len, x_stride, work_ptr or None, work_len, n_tok,
+                                       int(dtype_x), int(dtype_out), stream or None))
+
+
 def token_logprobs_work_bytes(n_tok: int, vocab: int, n_top: int) -> int:
     """Workspace of token_logprobs_dev."""
     return LIB.rsllm_hip_token_logprobs_work_bytes(n_tok, vocab, n_top)
@@ -695,6 +804,9 @@ __all__ = [
     "matmul_q4k_bf16_dev", "moe_routed", "moe_routed_dev", "quantize_q8_0_batch",
     "matmul_q8_0_batch", "quantize_q8_0_batch_dev", "matmul_q8_0_batch_dev", "HipBackend",
     "RouteScore", "moe_route_dev", "int8_row_bytes", "int8_work_bytes", "quantize_int8_dev",
-    "matmul_int8_dev", "matmul_int8_prequant_dev", "token_logprobs_work_bytes",
+    "matmul_int8_dev", "matmul_int8_prequant_dev", "mxfp4_row_bytes", "mxfp4_scale_bytes",
+    "mxfp4_work_bytes", "quantize_mxfp4_dev", "dequantize_mxfp4_dev", "matmul_mxfp4_dev",
+    "matmul_mxfp4_prequant_dev", "MoeMxfp4", "moe_mxfp4_work_bytes", "moe_mxfp4_dev",
+    "token_logprobs_work_bytes",
     "token_logprobs_dev", "BackendCapability", "LIB", "LIB_PATH", "SIGNATURES",
 ]

@@ -26,7 +26,8 @@ LIB = os.path.join(HERE, "librsllm_hip.so")
 
 SOURCES = ["abi.hip", "dequant.hip", "gemv.hip", "gemv_mfma.hip", "gemm_exact.hip", "moe_gemm.hip",
            "prefill.hip", "moe.hip", "q8_int8.hip", "residency.hip", "probe.hip",
-           "abi_serving.hip", "route.hip", "int8.hip", "logprobs.hip"]
+           "abi_serving.hip", "route.hip", "int8.hip", "logprobs.hip",
+           "abi_mxfp4.hip", "mxfp4.hip", "moe_layer.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -52,6 +53,8 @@ EXTRA_FLAGS = {
     "gemm_exact.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "moe_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "int8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "mxfp4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "moe_layer.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -8,46 +8,15 @@
 #include <cmath>
 
 #include "../../include/rsllm_hip.h"
-#include "abi_internal.h"
+#include "abi_checks.h"
 #include "kernels.h"
 
 using namespace rsllm_hip;
-using abi::set_error;
+using namespace rsllm_hip::abi;
 
 namespace {
 
-#define HIP_TRY(expr, where)                                  \
-    do {                                                      \
-        hipError_t e_ = (expr);                               \
-        if (e_ != hipSuccess) return abi::device_error(e_, where); \
-    } while (0)
-
-int invalid(const char *m) { return set_error(RSLLM_HIP_ERR_INVALID_ARGUMENT, m); }
-int mismatch(const char *m) { return set_error(RSLLM_HIP_ERR_SHAPE_MISMATCH, m); }
-
-bool float_type(uint32_t t) { return t == T_F32 || t == T_F16 || t == T_BF16; }
-bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-size_t elem_bytes(uint32_t t) { return t == T_F32 ? 4 : 2; }
-
-// rows of `row` elements, `stride` apart, inside len elements (0 rows: any)
-bool span_ok(size_t rows, size_t row, size_t stride, size_t len) {
-    size_t n;
-    return rows == 0 || (!__builtin_mul_overflow(rows - 1, stride, &n) &&
-                         !__builtin_add_overflow(n, row, &n) && n <= len);
-}
-bool product_is(size_t a, size_t b, size_t len) {
-    size_t n;
-    return !__builtin_mul_overflow(a, b, &n) && n == len;
-}
-// Rows or channels of one call. A launch holds less than 2^32 threads: these with
-// up to 512 a row, and the int8 product's tiles of as many rows and channels as
-// fit memory (below 2^31 threads, over all such sizes).
-constexpr size_t kMaxRows = ((size_t)1 << 23) - 1;
-bool counts_ok(size_t n) { return n <= kMaxRows; }
-
 constexpr size_t kI8MaxIn = 131071;  // 128 * 128 * 131071 < 2^31
-
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // The caller's work of an int8 product: codes, then scales.
 struct I8Work {

@@ -300,6 +300,47 @@ hipError_t launch_i8_matmul(const I8Args &a, hipStream_t s);
 bool i8_one_supported(int in_dim);
 hipError_t launch_i8_one(const I8Args &a, const void *x, int in_dim, uint32_t dtype, hipStream_t s);
 
+// mxfp4.hip: MXFP4 rows (4-bit codes mx_row_bytes(in_dim) apart, a scale byte for 32
+// codes, mx_scale_bytes(in_dim) apart). Rows of floats (dtype F32, F16 or BF16, `stride`
+// elements apart) to codes and scales, back, and the product of two code matrices.
+constexpr size_t mx_row_bytes(size_t in_dim) { return (in_dim + 127) / 128 * 64; }
+constexpr size_t mx_scale_bytes(size_t in_dim) { return (in_dim + 511) / 512 * 16; }
+hipError_t launch_mx_quantize(const void *x, size_t stride, uint8_t *codes, uint8_t *scales, int n_rows,
+                              int in_dim, uint32_t dtype, hipStream_t s);
+hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, void *out, size_t stride,
+                                int n_rows, int in_dim, uint32_t dtype, hipStream_t s);
+struct MxArgs {
+    const uint8_t *w, *ws;  // out_dim rows of codes, of scales
+    const uint8_t *x, *xs;  // n_tok rows, the codes zero behind in_dim
+    const float *bias;      // or null
+    void *out;              // rows of dtype_out, out_stride elements apart
+    size_t out_stride;
+    int n_tok, out_dim, in_dim;
+    uint32_t dtype_out;
+};
+hipError_t launch_mx_matmul(const MxArgs &a, hipStream_t s);
+
+// moe_layer.hip: a mixture-of-experts layer with MXFP4 experts for up to kMoeMaxTok
+// tokens; `work` holds moe_layer_work_bytes.
+constexpr int kMoeMaxTok = 32;
+struct MoeLayerArgs {
+    const void *router;
+    const float *bias;  // or null
+    const uint8_t *gate, *up, *down, *gate_s, *up_s, *down_s;
+    int n_embd, n_ff, n_expert, n_shared, k, n_group, topk_group, group_top, score, renormalise;
+    float scale, clamp;
+    uint32_t dtype_router, dtype_x, dtype_out;
+    const void *x;
+    size_t x_stride;
+    void *out;
+    size_t out_stride;
+    int *ids;
+    float *weights;
+    int n_tok;
+};
+size_t moe_layer_work_bytes(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_shared);
+hipError_t launch_moe_layer(const MoeLayerArgs &a, uint8_t *work, hipStream_t s);
+
 // logprobs.hip: per row of logits (dtype F32, F16 or BF16, `stride` elements
 // apart) what rsllm_hip_token_logprobs_dev gives. tokens may be null (logprob
 // and rank are then not written); rank, entropy may be null. `work` holds
