@@ -27,7 +27,7 @@ LIB = os.path.join(HERE, "librsllm_hip.so")
 SOURCES = ["abi.hip", "dequant.hip", "gemv.hip", "gemv_mfma.hip", "gemm_exact.hip", "moe_gemm.hip",
            "prefill.hip", "moe.hip", "q8_int8.hip", "residency.hip", "probe.hip",
            "abi_serving.hip", "route.hip", "int8.hip", "logprobs.hip",
-           "abi_mxfp4.hip", "mxfp4.hip", "moe_layer.hip"]
+           "abi_mxfp4.hip", "mxfp4.hip", "mxfp4_wide.hip", "moe_layer.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1,7 +1,11 @@
 // MXFP4 rows: quantising, decoding, and the product of two code matrices.
-#include "fp4_common.h"
+#include "buffer_lds.h"
+#include "mxfp4_product.h"
 
 #include <algorithm>
+#include <climits>
+#include <atomic>
+#include <type_traits>
 
 namespace rsllm_hip {
 
@@ -77,36 +81,281 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict
 }
 
 // ---- the product -------------------------------------------------------------------
+
+namespace {
+
+// ---- few tokens: the weights streamed into registers ----------------------------------
 //
-// v_mfma_scale_f32_16x16x128: lane l holds 32 codes (16 bytes) and a scale byte of row
-// l % 16 of either operand, block l / 16 of the step's four; its four sums are rows
-// 4 (l / 16) + i of the first operand (channels) at row l % 16 of the second (tokens).
-// A wavefront per 16 x 16 outputs.
-__global__ __launch_bounds__(64) void k_mx_simple(MxArgs a) {
-    const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
-    const int o0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+// A workgroup's tile: 16 MF channels x 16 NF tokens; its WK wavefronts take every WK-th
+// piece of 512 codes, and their sums are added through LDS. A lane reads 16 codes' bytes
+// of a row for each step of 128 and the 16 scale bytes of its row for the piece's four
+// steps; the operands of the next piece are on their way while this one is multiplied.
+template <int MF_, int NF_, int WK_> struct MxFew {
+    static constexpr int MF = MF_, NF = NF_, WK = WK_, BM = 16 * MF, BN = 16 * NF;
+};
+struct MxPiece {
+    mx_v4u c[4], s;
+};
+
+template <class G> __global__ __launch_bounds__(64 * G::WK) void k_mx_few(MxArgs a, int n_ct) {
+    constexpr int MF = G::MF, NF = G::NF, WK = G::WK;
+    __shared__ float red[WK * MF * NF * 256];
+    const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int o0 = (blockIdx.x % n_ct) * G::BM, t0 = (blockIdx.x / n_ct) * G::BN;
     const size_t rb = mx_row_bytes(a.in_dim), sb = mx_scale_bytes(a.in_dim);
-    const int blocks = (a.in_dim + 31) / 32;
-    const size_t wr = (size_t)min(o0 + r, a.out_dim - 1), xr = (size_t)min(t0 + r, a.n_tok - 1);
-    mx_v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int st = 0; st < (int)(rb / 64); st++) {
-        const int b = 4 * st + q;
-        const uint4 cw = *reinterpret_cast<const uint4 *>(a.w + wr * rb + 16 * (size_t)b);
-        const uint4 cx = *reinterpret_cast<const uint4 *>(a.x + xr * rb + 16 * (size_t)b);
-        // (a weight row's scales behind its last block may be anything)
-        const int sw = b < blocks ? a.ws[wr * sb + b] : 127, sx = b < blocks ? a.xs[xr * sb + b] : 127;
-        const mx_v8i fw = {(int)cw.x, (int)cw.y, (int)cw.z, (int)cw.w, 0, 0, 0, 0};
-        const mx_v8i fx = {(int)cx.x, (int)cx.y, (int)cx.z, (int)cx.w, 0, 0, 0, 0};
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx, acc, 4, 4, 0, sw, 0, sx);
-    }
-    if (t0 + r >= a.n_tok) return;
+    const int blocks = (a.in_dim + 31) / 32, pieces = (int)(sb / 16), steps = (int)(rb / 64);
+    const uint8_t *w[MF], *ws[MF], *x[NF], *xs[NF];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int o = o0 + 4 * q + i;
-        if (o < a.out_dim)
-            mx_store(a.out, (size_t)(t0 + r) * a.out_stride + o, a.bias ? acc[i] + a.bias[o] : acc[i], a.dtype_out);
+    for (int m = 0; m < MF; m++) {
+        const size_t row = (size_t)min(o0 + 16 * m + r, a.out_dim - 1);
+        w[m] = a.w + row * rb + 16 * q;
+        ws[m] = a.ws + row * sb;
+    }
+#pragma unroll
+    for (int n = 0; n < NF; n++) {
+        const size_t row = (size_t)min(t0 + 16 * n + r, a.n_tok - 1);
+        x[n] = a.x + row * rb + 16 * q;
+        xs[n] = a.xs + row * sb;
+    }
+    auto load = [&](MxPiece &p, const uint8_t *c, const uint8_t *s, int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            p.c[j] = mx_v4u{0, 0, 0, 0};
+            if (4 * i + j < steps) p.c[j] = *reinterpret_cast<const mx_v4u *>(c + 256 * (size_t)i + 64 * j);
+        }
+        p.s = *reinterpret_cast<const mx_v4u *>(s + 16 * (size_t)i);
+    };
+    mx_v4f acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[m][n] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    MxPiece pw[MF], px[NF];
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+        if (i < pieces) {
+#pragma unroll
+            for (int m = 0; m < MF; m++) load(pw[m], w[m], ws[m], i);
+#pragma unroll
+            for (int n = 0; n < NF; n++) load(px[n], x[n], xs[n], i);
+        }
+    };
+    fetch(wv);
+    for (int i = wv; i < pieces; i += WK) {
+        MxPiece cw[MF], cx[NF];
+#pragma unroll
+        for (int m = 0; m < MF; m++) cw[m] = pw[m];
+#pragma unroll
+        for (int n = 0; n < NF; n++) cx[n] = px[n];
+        fetch(i + WK);
+        // (scales behind a row's last block may be anything: there 1)
+        const bool tail = 16 * i + 16 > blocks;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (4 * i + j < steps) {
+                const bool in = !tail || 16 * i + 4 * j + q < blocks;
+                int sw[MF], sx[NF];
+#pragma unroll
+                for (int m = 0; m < MF; m++) sw[m] = in ? (int)(cw[m].s[j] >> (8 * q)) : 127;
+#pragma unroll
+                for (int n = 0; n < NF; n++) sx[n] = in ? (int)(cx[n].s[j] >> (8 * q)) : 127;
+#pragma unroll
+                for (int m = 0; m < MF; m++)
+#pragma unroll
+                    for (int n = 0; n < NF; n++) acc[m][n] = mx_mfma(cw[m].c[j], cx[n].c[j], acc[m][n], sw[m], sx[n]);
+            }
+        }
+    }
+    mx_v4f *const part = reinterpret_cast<mx_v4f *>(red);
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) part[(wv * MF * NF + m * NF + n) * 64 + lane] = acc[m][n];
+    __syncthreads();
+    const bool vec = mx_vec(a);
+    for (int f = wv; f < MF * NF; f += WK) {
+        mx_v4f s = part[f * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < WK; k++) s += part[(k * MF * NF + f) * 64 + lane];
+        const int o = o0 + 16 * (f / NF) + 4 * q;
+        mx_finish(a, s, mx_bias(a, o), o, t0 + 16 * (f % NF) + r, vec);
     }
 }
+
+template <class G> hipError_t mx_few_go(const MxArgs &a, hipStream_t s) {
+    const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
+    k_mx_few<G><<<(unsigned)n_ct * (unsigned)n_tt, 64 * G::WK, 0, s>>>(a, n_ct);
+    return hipGetLastError();
+}
+
+// ---- many tokens: both operands through LDS -------------------------------------------
+//
+// A workgroup's tile: BM = 16 MF WM channels x BN = 16 NF WN tokens, a wavefront 16 MF x
+// 16 NF of it. Slices of 128 bytes (256 codes) of both operands are copied to LDS ST deep;
+// the scales, 16 bytes a row for two slices, into a ring of their own. The operands of a
+// slice's next half are read into registers while the matrix cores work on this one. One
+// barrier a slice, in its middle: behind it the next slice has landed, and every
+// wavefront holds what is left of this one in registers, so the slice ST further on can be
+// copied over it.
+template <int WM_, int WN_, int MF_, int NF_, int ST_> struct MxBig {
+    static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, ST = ST_, NW = WM * WN;
+    static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * NW;
+    static constexpr int kSlice = (BM + BN) * 128, kCopies = (BM + BN) / 8;
+    static constexpr int D = (kCopies + NW - 1) / NW;
+    // scales: a copy brings 64 rows of 16 bytes; the channels' with the even slices, the
+    // tokens' of the next two slices with the odd ones
+    static constexpr int kRows = BM > BN ? BM : BN, kScaleCopies = (kRows + 63) / 64;
+    static constexpr int DS = (kScaleCopies + NW - 1) / NW, kPairs = ST / 2 + 2;
+    static constexpr int kScaleSlot = kScaleCopies * 1024;  // of one operand, two slices
+    static constexpr int kRing = ST * kSlice, kLds = kRing + kPairs * 2 * kScaleSlot;
+    // P fragments' rows interleaved, so that a lane ends up with 4 P consecutive channels
+    static constexpr int P = MF % 4 == 0 ? 4 : MF % 2 == 0 ? 2 : 1;
+    static_assert(kLds <= 160 * 1024 && (D + DS) * (ST - 1) <= 63, "tile");
+};
+// Where byte 16 c of a row's slice lies: at place c ^ key, so that the 16 rows which an
+// operand read takes at one c are spread over all banks.
+template <int P> __device__ __forceinline__ constexpr int mx_key(int row) {
+    return ((row >> 1) & 1) | ((row / (4 * P)) & 3) << 1;
+}
+
+template <class G> __global__ __launch_bounds__(G::kThreads) void k_mx_big(MxArgs a, int n_ct, int n_tt) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int MF = G::MF, NF = G::NF, D = G::D, DS = G::DS, NW = G::NW, ST = G::ST, P = G::P;
+    // Workgroups go round the 8 XCDs: each takes a run of tiles, token tiles fastest, so
+    // the tiles that share a weight row are behind one L2.
+    const int total = n_ct * n_tt, per = (total + 7) / 8;
+    const int L = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || L >= total) return;  // the whole workgroup
+    const int tt = L % n_tt, ct = L / n_tt;
+    const int lane = threadIdx.x & 63;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wn = wv % G::WN, wm = wv / G::WN;
+    const int o0 = ct * G::BM, t0 = tt * G::BN;
+    const uint32_t rb = (uint32_t)mx_row_bytes(a.in_dim), sb = (uint32_t)mx_scale_bytes(a.in_dim);
+    const int blocks = (a.in_dim + 31) / 32, n_sl = (int)((rb + 127) / 128);
+
+    const int w_rows = min(G::BM, a.out_dim - o0), x_rows = min(G::BN, a.n_tok - t0);
+    const bl_rsrc rw = bl_make_rsrc(a.w + (size_t)o0 * rb, (uint32_t)w_rows * rb);
+    const bl_rsrc rx = bl_make_rsrc(a.x + (size_t)t0 * rb, (uint32_t)x_rows * rb);
+    const bl_rsrc rws = bl_make_rsrc(a.ws + (size_t)o0 * sb, (uint32_t)w_rows * sb);
+    const bl_rsrc rxs = bl_make_rsrc(a.xs + (size_t)t0 * sb, (uint32_t)x_rows * sb);
+    const uint32_t lds0 = bl_lds(smem);
+    // copy c: 8 rows of channels (c < BM / 8) or tokens; rows behind the last repeat it
+    // (their products are not stored)
+    uint32_t off[D];
+    bool half[D];  // this lane's 16 bytes lie in the slice's second half
+#pragma unroll
+    for (int p = 0; p < D; p++) {
+        const int c = min(wv + NW * p, G::kCopies - 1);
+        const bool is_w = c < G::BM / 8;
+        const int row = (is_w ? 8 * c : 8 * c - G::BM) + (lane >> 3);
+        const int at = (lane & 7) ^ (is_w ? mx_key<P>(row) : mx_key<1>(row));
+        off[p] = (uint32_t)min(row, (is_w ? w_rows : x_rows) - 1) * rb + 16u * (uint32_t)at;
+        half[p] = at >= 4;
+    }
+    auto copy1 = [&](int i, int buf, int p) __attribute__((always_inline)) {
+        const int c = min(wv + NW * p, G::kCopies - 1);
+        const bool is_w = c < G::BM / 8;
+        uint32_t o = off[p] + 128u * (uint32_t)i;
+        if (128u * (uint32_t)i + 128u > rb && half[p]) o = 0xFFFFFFF0u;  // zeros behind the row
+        const bl_rsrc r = is_w ? rw : rx;
+        bl_dma16(bl_rsrc{r[0], r[1], i < n_sl ? r[2] : 0u, r[3]}, o, 0, lds0 + (uint32_t)(buf * G::kSlice + c * 1024));
+    };
+    // the scales of pair j (slices 2 j and 2 j + 1) of the channels or the tokens
+    auto copy_scales = [&](bool is_w, int j, int p) __attribute__((always_inline)) {
+        const int c = min(wv + NW * p, G::kScaleCopies - 1), row = 64 * c + lane;
+        const uint32_t o = (uint32_t)min(row, (is_w ? w_rows : x_rows) - 1) * sb + 16u * (uint32_t)j;
+        const bl_rsrc r = is_w ? rws : rxs;
+        bl_dma16(bl_rsrc{r[0], r[1], 2 * j < n_sl ? r[2] : 0u, r[3]}, o, 0,
+                 lds0 + (uint32_t)(G::kRing + (j % G::kPairs * 2 + (is_w ? 0 : 1)) * G::kScaleSlot + c * 1024));
+    };
+    mx_v4f acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[m][n] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    const int r16 = lane & 15, q = lane >> 4;
+    // rows of this lane: of fragment m of the channels, n of the tokens
+    const int wrow0 = wm * 16 * MF + mx_frag_row<P>(0, r16), xrow0 = wn * 16 * NF + r16;
+    const uint8_t *const lw = smem + wrow0 * 128, *const lx = smem + (G::BM + xrow0) * 128;
+    const uint8_t *const sw0 = smem + G::kRing + wrow0 * 16 + q, *const sx0 = smem + G::kRing + G::kScaleSlot + xrow0 * 16 + q;
+    // (the key of every fragment's row r16 is that of fragment 0's)
+    const int pw0 = 16 * (q ^ mx_key<P>(wrow0)), px0 = 16 * (q ^ mx_key<1>(xrow0));
+    mx_v4u f[2][MF + NF];  // operands of a half slice: NF of tokens, MF of channels
+    int sc[2][MF + NF];
+    auto read1 = [&](int h, int buf, int i, int j) __attribute__((always_inline)) {
+        const int slot = i / 2 % G::kPairs * 2 * G::kScaleSlot + 8 * (i & 1) + 4 * h;
+        if (j < NF) {
+            f[h][j] = *reinterpret_cast<const mx_v4u *>(lx + j * 2048 + (px0 ^ (64 * h)) + buf * G::kSlice);
+            sc[h][j] = sx0[slot + j * 256];
+        } else {
+            const int row = mx_frag_row<P>(j - NF, 0);
+            f[h][j] = *reinterpret_cast<const mx_v4u *>(lw + row * 128 + (pw0 ^ (64 * h)) + buf * G::kSlice);
+            sc[h][j] = sw0[slot + row * 16];
+        }
+    };
+    // the MFMAs of half h of slice i; between them the reads of the other half's next
+    // operands (slice ri in buffer rbuf) and, with `cp`, the copies of slice i + ST
+    auto phase = [&](auto h_c, int i, int rbuf, int ri, int cbuf, bool cp) __attribute__((always_inline)) {
+        constexpr int h = decltype(h_c)::value;
+        // (scales behind a row's last block may be anything: there 1)
+        if (8 * i + 8 > blocks) {
+#pragma unroll
+            for (int j = 0; j < MF + NF; j++) sc[h][j] = 8 * i + 4 * h + q < blocks ? sc[h][j] : 127;
+        }
+#pragma unroll
+        for (int m = 0; m < MF; m++) {
+#pragma unroll
+            for (int j = m * (MF + NF) / MF; j < (m + 1) * (MF + NF) / MF; j++) read1(h ^ 1, rbuf, ri, j);
+            if (cp) {
+#pragma unroll
+                for (int p = m * D / MF; p < (m + 1) * D / MF; p++) copy1(i + ST, cbuf, p);
+                if (m == MF - 1) {
+                    const int s = i + ST;
+#pragma unroll
+                    for (int p = 0; p < DS; p++) copy_scales((s & 1) == 0, (s + 1) / 2, p);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NF; n++)
+                acc[m][n] = mx_mfma(f[h][NF + m], f[h][n], acc[m][n], sc[h][NF + m], sc[h][n]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < DS; p++) copy_scales(false, 0, p);
+#pragma unroll
+    for (int i = 0; i < ST; i++) {
+#pragma unroll
+        for (int p = 0; p < D; p++) copy1(i, i, p);
+#pragma unroll
+        for (int p = 0; p < DS; p++) copy_scales((i & 1) == 0, (i + 1) / 2, p);
+    }
+    bl_barrier<(D + DS) * (ST - 1)>();
+#pragma unroll
+    for (int j = 0; j < MF + NF; j++) read1(0, 0, 0, j);
+    int buf = 0;
+    for (int i = 0; i < n_sl; i++) {
+        const int next = buf + 1 == ST ? 0 : buf + 1;
+        phase(std::integral_constant<int, 0>{}, i, buf, i, 0, false);
+        bl_barrier<(D + DS) * (ST - 2)>();
+        phase(std::integral_constant<int, 1>{}, i, next, i + 1, buf, true);
+        buf = next;
+    }
+    bl_wait<0>();  // (the copies past the last slice, zeros, land in the ring too)
+    mx_write_tile<MF, NF, G::WM, G::WN, P, G::kLds>(a, acc, smem, o0, t0, wm, wn);
+}
+
+template <class G> hipError_t mx_big_go(const MxArgs &a, hipStream_t s) {
+    const hipError_t e = mx_allow_lds<G>(reinterpret_cast<const void *>(&k_mx_big<G>));
+    if (e != hipSuccess) return e;
+    const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
+    const long long wgs = ((long long)n_ct * n_tt + 7) / 8 * 8;
+    k_mx_big<G><<<(unsigned)wgs, G::kThreads, G::kLds, s>>>(a, n_ct, n_tt);
+    return hipGetLastError();
+}
+
+}  // namespace
 
 namespace {
 
@@ -137,18 +386,68 @@ hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, voi
     return hipGetLastError();
 }
 
+namespace {
+
+// A kernel of the product and what it takes, by an estimate in us:
+//   us = c0 + r c1 + (L c2 + r c3) slices
+// with L workgroups a CU, r of them one after the other (`occ` run at once) and `slices`
+// pieces of `unit` codes a wavefront, fitted to 150 sizes (1 to 2048 tokens, weights from
+// memory). Slower than the fastest of sixteen kernels: 3% on average and 29% at most at
+// those sizes. From 129 tokens on the tiles without LDS, which read the tokens' codes for
+// every 16 or 32 channels, are up to three times slower and not looked at.
+struct MxKernel {
+    hipError_t (*go)(const MxArgs &, hipStream_t);
+    int bm, bn, wk, unit, occ, max_tok, threads;
+    float c0, c1, c2, c3;
+    bool fits(const MxArgs &a) const {  // a launch holds less than 2^32 threads
+        const long long tiles = (long long)((a.out_dim + bm - 1) / bm) * ((a.n_tok + bn - 1) / bn);
+        return a.n_tok <= max_tok && (tiles + 8) * threads < (1ll << 32);
+    }
+    float us(const MxArgs &a) const {
+        const long long tiles = (long long)((a.out_dim + bm - 1) / bm) * ((a.n_tok + bn - 1) / bn);
+        const long long L = (tiles + 255) / 256, r = (L + occ - 1) / occ;
+        const int slices = ((a.in_dim + unit - 1) / unit + wk - 1) / wk;
+        return c0 + (float)r * c1 + ((float)L * c2 + (float)r * c3) * (float)slices;
+    }
+};
+template <int MF, int NF, int WK> constexpr MxKernel mx_few(int occ, float c0, float c1, float c2, float c3) {
+    using G = MxFew<MF, NF, WK>;
+    return {&mx_few_go<G>, G::BM, G::BN, WK, 512, occ, 128, 64 * WK, c0, c1, c2, c3};
+}
+template <int WM, int WN, int MF, int NF, int ST> constexpr MxKernel mx_big(int occ, float c0, float c1, float c2) {
+    using G = MxBig<WM, WN, MF, NF, ST>;
+    return {&mx_big_go<G>, G::BM, G::BN, 1, 256, occ, INT_MAX, G::kThreads, c0, c1, c2, 0.0f};
+}
+const MxKernel kMxKernels[] = {
+    mx_few<1, 1, 8>(2, 4.57f, 0.0f, 0.434f, 0.328f),  // 16 channels x 16 tokens
+    mx_few<2, 1, 8>(1, 4.26f, 0.0f, 1.196f, 0.0f),    // 32 x 16
+    mx_few<2, 1, 4>(3, 4.33f, 0.0f, 0.547f, 0.308f),
+    mx_few<2, 2, 8>(1, 3.66f, 0.0f, 1.834f, 0.0f),    // 32 x 32
+    mx_few<2, 2, 4>(2, 4.03f, 0.0f, 1.105f, 0.066f),
+    mx_few<2, 4, 4>(1, 3.34f, 0.23f, 1.938f, 0.0f),   // 32 x 64
+    mx_big<4, 2, 1, 2, 4>(2, 1.43f, 3.01f, 0.409f),   // 64 x 64
+    mx_big<2, 4, 2, 2, 4>(1, 0.39f, 4.36f, 0.499f),   // 64 x 128
+    mx_big<2, 4, 4, 2, 3>(1, 0.0f, 5.10f, 0.768f),    // 128 x 128
+    mx_big<4, 2, 3, 4, 2>(1, 0.54f, 4.50f, 1.153f),   // 192 x 128
+    mx_big<2, 4, 8, 2, 2>(1, 2.66f, 4.56f, 1.351f),   // 256 x 128
+    {&mx_wide_224, 224, 256, 1, 256, 1, INT_MAX, 256, 0.0f, 10.26f, 1.216f, 0.0f},
+};
+
+}  // namespace
+
 hipError_t launch_mx_matmul(const MxArgs &a, hipStream_t s) {
     if (a.n_tok <= 0) return hipSuccess;
-    // (the second grid dimension holds 65535: more tokens go in turns)
-    for (int t = 0; t < a.n_tok; t += 65535 * 16) {
-        MxArgs part = a;
-        part.n_tok = std::min(a.n_tok - t, 65535 * 16);
-        part.x += (size_t)t * mx_row_bytes(a.in_dim);
-        part.xs += (size_t)t * mx_scale_bytes(a.in_dim);
-        part.out = static_cast<uint8_t *>(a.out) + (size_t)t * a.out_stride * (a.dtype_out == T_F32 ? 4 : 2);
-        k_mx_simple<<<dim3((a.out_dim + 15) / 16, (part.n_tok + 15) / 16), 64, 0, s>>>(part);
+    const MxKernel *best = nullptr;
+    float us = 0.0f;
+    for (const MxKernel &k : kMxKernels) {
+        if (!k.fits(a)) continue;
+        const float t = k.us(a);
+        if (!best || t < us) {
+            best = &k;
+            us = t;
+        }
     }
-    return hipGetLastError();
+    return best ? best->go(a, s) : hipErrorInvalidValue;
 }
 
 }  // namespace rsllm_hip

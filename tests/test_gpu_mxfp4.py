@@ -127,7 +127,7 @@ def test_dequantize(hip, kind, n, k, gap):
 
 class Product:
     def __init__(self, hip, t, k, n, kx="f32", ky="f32", bias=False, x_gap=0, y_gap=0, low=118, high=124, seed=0):
-        rng = np.random.default_rng(seed + t * 7 + k * 13 + n)
+        self.rng = rng = np.random.default_rng(seed + t * 7 + k * 13 + n)
         self.hip, self.t, self.k, self.n, self.kx, self.ky = hip, t, k, n, kx, ky
         self.w, self.ws = M.random_rows(rng, n, k, low, high)
         self.bias = rng.normal(0, 1, n).astype(np.float32) if bias else None
@@ -164,8 +164,8 @@ class Product:
         """Steps of 128 products are exact sums rounded to f32 with what was there, off by
         at most 2^-23 of the terms' magnitudes; joins of up to 16 parts and the bias as
         much each; then the output's rounding."""
-        want, size = M.product(M.values(codes, scales, self.k), M.values(self.w, self.ws, self.k),
-                               None if self.bias is None else self.bias.astype(np.float64))
+        bias = None if self.bias is None else self.bias.astype(np.float64)
+        want, size = M.product(M.values(codes, scales, self.k), M.values(self.w, self.ws, self.k), bias)
         tol = ((self.k + 127) // 128 + 17) * 2.0 ** -23 * size + M.rounding(want, self.ky)
         got = out[:, :self.n].cpu().double().numpy()
         assert np.array_equal(np.isnan(got), np.isnan(want))
