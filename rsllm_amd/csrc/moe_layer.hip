@@ -9,37 +9,39 @@
 #include "route_scores.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace rsllm_hip {
 
 namespace {
 
+constexpr int kInWaves = 16, kWaves = 8;
 constexpr int kMoeMaxExpert = 1024, kMoeMaxShared = 8, kMoeMaxSlots = 40;
 constexpr int kMoeMaxPairs = kMoeMaxTok * kMoeMaxSlots, kMoeMaxAll = kMoeMaxExpert + kMoeMaxShared;
 
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 __host__ __device__ constexpr int pad128(int n) { return (n + 127) / 128 * 128; }
 
-// What the tokens chose: every token's slots (the k chosen experts, then the shared ones;
-// -1: none, or of weight 0), and the jobs: an expert, in rising order, and the tokens that
-// take it, a bit each, as many jobs as it takes with at most `cap` tokens.
+// What the tokens chose, in LDS: every token's slots (the k chosen experts, then the shared
+// ones; -1: none, or of weight 0), and the jobs: an expert, in rising order, and the tokens
+// that take it, a bit each, as many jobs as it takes with at most `cap` tokens.
 struct MoePlan {
     int n_jobs;
     uint32_t tokens[kMoeMaxPairs];
     float weight[kMoeMaxPairs];
     int16_t expert[kMoeMaxPairs];
     uint16_t job[kMoeMaxPairs];
+    uint32_t takes[kMoeMaxAll];
 };
 
-// The caller's work: logits and scores (f64), x and h as bf16 terms, a flag a token, the plan.
+// The caller's work: logits and scores (f64), x and h as bf16 terms, a flag a token.
 struct MoeWork {
     double *logits;  // [n_tok, n_expert]
     double *scores;  // [n_tok, n_expert], not of softmax
     __bf16 *x;       // [n_tok][3][pad128(n_embd)]
     __bf16 *h;       // [n_tok * (k + n_shared)][3][pad128(n_ff)], weighted
     int *bad;        // [n_tok]: x is not finite
-    MoePlan *plan;
 };
 size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_shared, uint8_t *base, MoeWork *w) {
     size_t at = 0;
@@ -53,9 +55,8 @@ size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_sha
     uint8_t *const x = take((size_t)n_tok * 3 * pad128(n_embd) * 2);
     uint8_t *const h = take((size_t)n_tok * (k + n_shared) * 3 * pad128(n_ff) * 2);
     uint8_t *const bad = take((size_t)n_tok * 4);
-    uint8_t *const plan = take(n_tok ? sizeof(MoePlan) : 0);
     if (w) *w = {reinterpret_cast<double *>(logits), reinterpret_cast<double *>(scores), reinterpret_cast<__bf16 *>(x),
-                 reinterpret_cast<__bf16 *>(h), reinterpret_cast<int *>(bad), reinterpret_cast<MoePlan *>(plan)};
+                 reinterpret_cast<__bf16 *>(h), reinterpret_cast<int *>(bad)};
     return at;
 }
 
@@ -72,78 +73,78 @@ __device__ __forceinline__ double route_score(double l, int score, double m, dou
 
 // ---- the router's product -------------------------------------------------------------
 
-// TB tokens' sums over the wavefronts' lanes: lane `i` of the first TB ends up with token i's.
-template <int TB> __device__ __forceinline__ double moe_wave_sums(double (&s)[TB]) {
-    const int lane = threadIdx.x & 63;
-    // the upper half of the lanes takes over the upper half of the sums, and so on
+// N sums over the lanes of a wavefront: the upper half of the lanes (bit OFF) takes over the
+// upper half of the sums, and so on, so lanes whose upper bits are i end up with sum i.
+template <int N, int OFF, int TB> __device__ __forceinline__ void moe_halve(double (&s)[TB]) {
+    if constexpr (N > 1) {
+        const bool up = (threadIdx.x & OFF) != 0;
 #pragma unroll
-    for (int n = TB, off = 32; n > 1; n >>= 1, off >>= 1) {
-        const bool up = (lane & off) != 0;
-#pragma unroll
-        for (int i = 0; i < n / 2; i++) {
-            const double mine = up ? s[n / 2 + i] : s[i], other = up ? s[i] : s[n / 2 + i];
-            s[i] = mine + __shfl_xor(other, off, 64);
+        for (int i = 0; i < N / 2; i++) {
+            const double mine = up ? s[N / 2 + i] : s[i], other = up ? s[i] : s[N / 2 + i];
+            s[i] = mine + __shfl_xor(other, OFF, 64);
         }
+        moe_halve<N / 2, OFF / 2>(s);
+    } else if constexpr (OFF > 0) {
+        s[0] += __shfl_xor(s[0], OFF, 64);
+        moe_halve<1, OFF / 2>(s);
     }
-#pragma unroll
-    for (int off = 32 / TB; off >= 1; off >>= 1) s[0] += __shfl_xor(s[0], off, 64);
-    return s[0];  // of token i at the lanes whose upper bits are i
 }
 
-// Logits of expert e for tokens t0 .. t0 + TB - 1 (those behind the last repeat it).
+// Part `part` of `parts` of expert e's logits for tokens t0 .. t0 + TB - 1 (those behind the
+// last repeat it), a wavefront's work, to red[token][part].
 template <uint32_t DX, uint32_t DR, int TB>
-__device__ __forceinline__ void moe_logits(const MoeLayerArgs &a, const MoeWork &w, int e, int t0, bool vx, bool vr,
-                                           double (*red)[TB]) {
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+__device__ __forceinline__ void moe_logits(const MoeLayerArgs &a, int e, int t0, int part, int parts, bool vx, bool vr,
+                                           double (*red)[kInWaves]) {
+    const int lane = threadIdx.x & 63;
     double s[TB];
 #pragma unroll
     for (int t = 0; t < TB; t++) s[t] = 0.0;
-    for (int i = 8 * tid; i < a.n_embd; i += 8 * 256) {
+    for (int i = 512 * part + 8 * lane; i < a.n_embd; i += 512 * parts) {
         float r[8], x[TB][8];
         mx_load8<DR>(a.router, (size_t)e * a.n_embd, i, a.n_embd, vr, r);
 #pragma unroll
         for (int t = 0; t < TB; t++)
             mx_load8<DX>(a.x, (size_t)min(t0 + t, a.n_tok - 1) * a.x_stride, i, a.n_embd, vx, x[t]);
 #pragma unroll
-        for (int t = 0; t < TB; t++)
+        for (int k = 0; k < 8; k++) {
+            const double rk = (double)r[k];  // (behind the row's end both are 0)
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (vr || i + k < a.n_embd) s[t] = fma((double)x[t][k], (double)r[k], s[t]);
+            for (int t = 0; t < TB; t++) s[t] = fma((double)x[t][k], rk, s[t]);
+        }
     }
-    const double sum = moe_wave_sums<TB>(s);
-    __syncthreads();
-    if (lane % (64 / TB) == 0) red[wv][lane / (64 / TB)] = sum;
-    __syncthreads();
-    if (tid < TB && t0 + tid < a.n_tok) {
-        const size_t at = (size_t)(t0 + tid) * a.n_expert + e;
-        const double l = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
-        w.logits[at] = l;
-        if (a.score != ROUTE_SOFTMAX) w.scores[at] = route_score(l, a.score, 0.0, 1.0);
-    }
+    moe_halve<TB, 32>(s);
+    if (lane % (64 / TB) == 0) red[t0 + lane / (64 / TB)][part] = s[0];
 }
 
 }  // namespace
 
-// Workgroup e < n_expert: the 64-bit logits (and scores) of expert e for every token; the others: a
-// token's x as bf16 terms, zeros behind it, and whether it is finite.
+// Workgroup e < n_expert: the 64-bit logits (and scores) of expert e for every token, groups
+// of up to 8 tokens and parts of K over the wavefronts; the others: a token's x as bf16
+// terms, zeros behind it, and whether it is finite.
 template <uint32_t DX, uint32_t DR>
-__global__ __launch_bounds__(256) void k_moe_in(MoeLayerArgs a, MoeWork w, int vx, int vr) {
+__global__ __launch_bounds__(64 * kInWaves) void k_moe_in(MoeLayerArgs a, MoeWork w, int vx, int vr) {
     constexpr int kTerms = DX == T_F32 ? 3 : DX == T_F16 ? 2 : 1;
-    __shared__ double red1[4][1], red4[4][4];
-    const int tid = threadIdx.x;
+    __shared__ double red[kMoeMaxTok][kInWaves];
+    const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     if ((int)blockIdx.x < a.n_expert) {
-        const int e = blockIdx.x;
-        if (a.n_tok == 1) {
-            moe_logits<DX, DR, 1>(a, w, e, 0, vx, vr, red1);
-        } else {
-            for (int t0 = 0; t0 < a.n_tok; t0 += 4) moe_logits<DX, DR, 4>(a, w, e, t0, vx, vr, red4);
+        const int e = blockIdx.x, groups = a.n_tok <= 8 ? 1 : a.n_tok <= 16 ? 2 : 4, parts = kInWaves / groups;
+        if (a.n_tok == 1) moe_logits<DX, DR, 1>(a, e, 0, wv, parts, vx, vr, red);
+        else if (a.n_tok <= 4) moe_logits<DX, DR, 4>(a, e, 0, wv, parts, vx, vr, red);
+        else moe_logits<DX, DR, 8>(a, e, wv / parts * 8, wv % parts, parts, vx, vr, red);
+        __syncthreads();
+        if (tid < a.n_tok) {
+            double l = 0.0;
+            for (int i = 0; i < parts; i++) l += red[tid][i];
+            const size_t at = (size_t)tid * a.n_expert + e;
+            w.logits[at] = l;
+            if (a.score != ROUTE_SOFTMAX) w.scores[at] = route_score(l, a.score, 0.0, 1.0);
         }
         return;
     }
     const int t = blockIdx.x - a.n_expert, row = pad128(a.n_embd);
     __bf16 *const dst = w.x + (size_t)t * 3 * row;
     bool ok = true;
-    for (int i = 8 * tid; i < row; i += 8 * 256) {
+    for (int i = 8 * tid; i < row; i += 8 * 64 * kInWaves) {
         float v[8];
         mx_load8<DX>(a.x, (size_t)t * a.x_stride, i, a.n_embd, vx, v);
 #pragma unroll
@@ -184,31 +185,59 @@ __device__ __forceinline__ int moe_best(uint64_t key, int id) {
     return __ffsll((unsigned long long)__ballot(in && ~(uint32_t)id == mi)) - 1;
 }
 
-// A wavefront's choice for token t: ids and weights of its k slots, -1 and 0 where there is
-// none, at lane r the r-th. key: n_expert doubles of LDS, gsum: n_group.
-__device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *l, const double *scores, double *key, double *gsum, int &id,
-                                           float &weight) {
+// A wavefront's choice for a token of logits l: id and weight of slot r at lane r, -1 and 0
+// where there is none. With R > 0 lane `sub` holds the keys of experts sub, sub + 64, .. in
+// registers (n_expert <= 64 R), else in `key`. gsum: n_group doubles of LDS, key: n_expert.
+template <int R>
+__device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *l, const double *scores, double *key,
+                                           double *gsum, int &id, float &weight) {
     const int lane = threadIdx.x & 63, per = a.n_expert / a.n_group;
     double m = kNever, sum = 0.0;
-    auto score = [&](int e) { return a.score == ROUTE_SOFTMAX ? route_exp(l[e], m) / sum : scores[e]; };
+    auto score = [&](int e, double le) { return a.score == ROUTE_SOFTMAX ? route_exp(le, m) / sum : scores[e]; };
+    auto place = [&](int e, double le) {
+        double p = kNever;
+        if (le > kNever) {  // (a NaN is not)
+            p = a.bias || a.n_group > 1 ? score(e, le) + (a.bias ? (double)a.bias[e] : 0.0) : le;
+            if (!(p > kNever)) p = kNever;
+        }
+        return p;
+    };
+    double own[R > 0 ? R : 1], lg[R > 0 ? R : 1];
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int j = 0; j < R; j++) lg[j] = lane + 64 * j < a.n_expert ? l[lane + 64 * j] : kNever;
+    }
     if (a.score == ROUTE_SOFTMAX) {
-        for (int e = lane; e < a.n_expert; e += 64)
-            if (l[e] > m) m = l[e];  // (a NaN is not)
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; j++) m = lg[j] > m ? lg[j] : m;
+        } else {
+            for (int e = lane; e < a.n_expert; e += 64) m = l[e] > m ? l[e] : m;
+        }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) m = fmax(m, __shfl_xor(m, off, 64));
-        for (int e = lane; e < a.n_expert; e += 64)
-            if (l[e] > kNever) sum += route_exp(l[e], m);
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; j++) sum += lg[j] > kNever ? route_exp(lg[j], m) : 0.0;
+        } else {
+            for (int e = lane; e < a.n_expert; e += 64)
+                if (l[e] > kNever) sum += route_exp(l[e], m);
+        }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
     }
-    for (int e = lane; e < a.n_expert; e += 64) {
-        const double le = l[e];
-        double p = kNever;
-        if (le > kNever) {
-            p = a.bias || a.n_group > 1 ? score(e) + (a.bias ? (double)a.bias[e] : 0.0) : le;
-            if (!(p > kNever)) p = kNever;
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int j = 0; j < R; j++) own[j] = lane + 64 * j < a.n_expert ? place(lane + 64 * j, lg[j]) : kNever;
+    }
+    if constexpr (R > 0) {
+        if (a.n_group > 1) {
+#pragma unroll
+            for (int j = 0; j < R; j++)
+                if (lane + 64 * j < a.n_expert) key[lane + 64 * j] = own[j];
         }
-        key[e] = p;
+    } else {
+        for (int e = lane; e < a.n_expert; e += 64) key[e] = place(e, l[e]);
     }
     __builtin_amdgcn_wave_barrier();
     if (a.n_group > 1) {
@@ -232,74 +261,113 @@ __device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *
             if (lane == who) gsum[i] = __builtin_nan("");
             __builtin_amdgcn_wave_barrier();
         }
-        for (int e = lane; e < a.n_expert; e += 64) {
+        auto kept = [&](int e, double k, double le) {
             const double g = gsum[e / per];
-            if (g == g) key[e] = kNever;
-            else if (!a.bias && key[e] > kNever) key[e] = l[e];
+            return g == g ? kNever : !a.bias && k > kNever ? le : k;
+        };
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; j++)
+                if (lane + 64 * j < a.n_expert) own[j] = kept(lane + 64 * j, own[j], lg[j]);
+        } else {
+            for (int e = lane; e < a.n_expert; e += 64) key[e] = kept(e, key[e], l[e]);
+            __builtin_amdgcn_wave_barrier();
         }
-        __builtin_amdgcn_wave_barrier();
     }
     // every lane's best of its keys; the one that gives it looks for its next
     double v = kNever;
     int i = a.n_expert;
-    for (int e = lane; e < a.n_expert; e += 64) route_best(v, i, key[e], e);
+    auto best = [&]() __attribute__((always_inline)) {
+        v = kNever;
+        i = a.n_expert;
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; j++) route_best(v, i, own[j], lane + 64 * j);
+        } else {
+            for (int e = lane; e < a.n_expert; e += 64) route_best(v, i, key[e], e);
+        }
+    };
+    best();
     id = -1;
     for (int r = 0; r < a.k; r++) {
         const int who = moe_best(order64(v), i);
         if (who < 0) break;
-        const int best = __shfl(i, who, 64);
-        if (lane == r) id = best;
+        const int chosen = __builtin_amdgcn_readlane(i, who);
+        if (lane == r) id = chosen;
         if (lane == who) {
-            key[i] = kNever;
-            v = kNever;
-            i = a.n_expert;
-            for (int e = lane; e < a.n_expert; e += 64) route_best(v, i, key[e], e);
+            if constexpr (R > 0) {
+#pragma unroll
+                for (int j = 0; j < R; j++) own[j] = lane + 64 * j == chosen ? kNever : own[j];
+            } else {
+                key[chosen] = kNever;
+            }
+            best();
         }
     }
-    const double s = id >= 0 ? score(id) : 0.0;
+    const double s = id >= 0 ? score(id, a.score == ROUTE_SOFTMAX ? l[id] : 0.0) : 0.0;
     double total = s;
+    if (a.renormalise) {
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+        for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+    }
     double out = s * (double)a.scale;
     if (a.renormalise) out = total == 0.0 ? 0.0 : out / total;
     weight = id >= 0 ? (float)out : 0.0f;
 }
+// A slot of the plan.
+__device__ __forceinline__ void moe_slot(const MoeLayerArgs &a, MoePlan &plan, int t, int i, int id, float weight) {
+    const bool on = id >= 0 && weight != 0.0f;
+    plan.expert[t * (a.k + a.n_shared) + i] = (int16_t)(on ? id : -1);
+    plan.weight[t * (a.k + a.n_shared) + i] = weight;
+    if (on) atomicOr(&plan.takes[id], 1u << t);
+}
+// Token t's choice by this wavefront; ids and weights written if `write`, the plan filled if
+// there is one. keys: n_expert + n_group doubles of LDS.
+__device__ __forceinline__ void moe_choose_token(const MoeLayerArgs &a, const MoeWork &w, int t, double *keys, bool write, MoePlan *plan) {
+    const double *const l = w.logits + (size_t)t * a.n_expert, *const s = w.scores + (size_t)t * a.n_expert;
+    const int lane = threadIdx.x & 63;
+    int id;
+    float weight;
+    if (a.n_expert <= 256) moe_choose<4>(a, l, s, keys, keys + a.n_expert, id, weight);
+    else moe_choose<0>(a, l, s, keys, keys + a.n_expert, id, weight);
+    if (lane >= a.k) return;
+    if (write) {
+        a.ids[t * a.k + lane] = id;
+        a.weights[t * a.k + lane] = weight;
+    }
+    if (plan) moe_slot(a, *plan, t, lane, id, weight);
+}
 
-// The whole workgroup's choice for every token, to `plan` in LDS; workgroup 0 writes ids
-// and weights, and the plan for the launch that follows. keys: (n_expert + n_group)
-// doubles for each of the first `choosers` wavefronts, who choose. takes: a word an expert.
+// The workgroup's plan, jobs of at most cap tokens. `choose`: the first `choose` wavefronts
+// make the tokens' choice themselves (workgroup 0 writes it), keys: n_expert + n_group doubles
+// for each; 0: it is read.
 template <int W> __device__ __forceinline__ void moe_plan(const MoeLayerArgs &a, const MoeWork &w, MoePlan &plan, int cap,
-                                                          double *keys, uint32_t *takes, int choosers) {
+                                                          double *keys, int choose) {
     __shared__ int part[W];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, slots = a.k + a.n_shared;
     const int all = a.n_expert + a.n_shared;
     for (int e = tid; e < all; e += 64 * W)
-        takes[e] = e < a.n_expert ? 0u : a.n_tok == 32 ? 0xFFFFFFFFu : (1u << a.n_tok) - 1u;
+        plan.takes[e] = e < a.n_expert ? 0u : a.n_tok == 32 ? 0xFFFFFFFFu : (1u << a.n_tok) - 1u;
+    for (int i = tid; i < a.n_tok * a.n_shared; i += 64 * W) {
+        const int t = i / a.n_shared, j = i - t * a.n_shared;
+        plan.expert[t * slots + a.k + j] = (int16_t)(a.n_expert + j);
+        plan.weight[t * slots + a.k + j] = 1.0f;
+    }
     __syncthreads();
-    double *const key = keys + wv * (a.n_expert + a.n_group);
-    for (int t = wv < choosers ? wv : a.n_tok; t < a.n_tok; t += choosers) {
-        int id;
-        float weight;
-        moe_choose(a, w.logits + (size_t)t * a.n_expert, w.scores + (size_t)t * a.n_expert, key, key + a.n_expert, id, weight);
-        if (lane < a.k) {
-            if (blockIdx.x == 0) {
-                a.ids[t * a.k + lane] = id;
-                a.weights[t * a.k + lane] = weight;
-            }
-            const bool on = id >= 0 && weight != 0.0f;
-            plan.expert[t * slots + lane] = (int16_t)(on ? id : -1);
-            plan.weight[t * slots + lane] = weight;
-            if (on) atomicOr(&takes[id], 1u << t);
-        } else if (lane < slots) {
-            plan.expert[t * slots + lane] = (int16_t)(a.n_expert + lane - a.k);
-            plan.weight[t * slots + lane] = 1.0f;
+    if (choose) {
+        for (int t = wv < choose ? wv : a.n_tok; t < a.n_tok; t += choose)
+            moe_choose_token(a, w, t, keys + wv * (a.n_expert + a.n_group), blockIdx.x == 0, &plan);
+    } else {
+        for (int i = tid; i < a.n_tok * a.k; i += 64 * W) {
+            const int t = i / a.k;
+            moe_slot(a, plan, t, i - t * a.k, a.ids[i], a.weights[i]);
         }
     }
     __syncthreads();
     // the jobs of a run of experts a thread, behind those of the threads before it
     const int run = (all + 64 * W - 1) / (64 * W), e0 = min(all, tid * run), e1 = min(all, e0 + run);
     int n = 0;
-    for (int e = e0; e < e1; e++) n += (__popc(takes[e]) + cap - 1) / cap;
+    for (int e = e0; e < e1; e++) n += (__popc(plan.takes[e]) + cap - 1) / cap;
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -311,7 +379,7 @@ template <int W> __device__ __forceinline__ void moe_plan(const MoeLayerArgs &a,
     int at = inc - n;
     for (int i = 0; i < wv; i++) at += part[i];
     for (int e = e0; e < e1; e++) {
-        for (uint32_t left = takes[e]; left; at++) {
+        for (uint32_t left = plan.takes[e]; left; at++) {
             uint32_t mine = 0;
             for (int i = 0; i < cap && left; i++) {
                 mine |= left & -left;
@@ -324,24 +392,12 @@ template <int W> __device__ __forceinline__ void moe_plan(const MoeLayerArgs &a,
     if (tid == 64 * W - 1) plan.n_jobs = at;
     __syncthreads();
 }
-// As much of a plan as there is, from LDS to memory or back, by a workgroup of N threads.
-template <int N> __device__ __forceinline__ void moe_copy_plan(MoePlan &to, const MoePlan &from, int pairs, int n_jobs) {
-    for (int i = threadIdx.x; i < pairs; i += N) {
-        to.weight[i] = from.weight[i];
-        to.expert[i] = from.expert[i];
-    }
-    for (int i = threadIdx.x; i < n_jobs; i += N) {
-        to.job[i] = from.job[i];
-        to.tokens[i] = from.tokens[i];
-    }
-    if (threadIdx.x == 0) to.n_jobs = n_jobs;
-}
 
 // ---- the products -----------------------------------------------------------------------
 //
-// v_mfma_f32_16x16x32_bf16: rows of weights by columns of terms: column c of a job's tile of
-// 16 is term c % terms of its (c / terms)-th token (16 / terms of them a tile), columns
-// behind its last token bring zeros.
+// v_mfma_f32_16x16x32_bf16: rows of weights by columns of terms: column c of a job is term
+// c % terms of its (c / terms)-th token (16 / terms of them a job), columns behind its last
+// token bring zeros.
 
 // 512 codes of FR times 16 rows, a lane's 16 codes' bytes of each step of 128 and its row's
 // 16 scale bytes.
@@ -371,27 +427,26 @@ __device__ __forceinline__ mx_bf8 moe_widen(uint32_t d, float unit) {
     f[4] = c[0]; f[5] = c[1]; f[6] = e[0]; f[7] = e[1];
     return f;
 }
-// acc += the piece's rows times the terms at `at` (bytes; this lane's column and block of
-// step 0, beyond the buffer where the column brings zeros) of the first `tiles` tiles.
-template <int FR, int NT>
-__device__ __forceinline__ void moe_multiply(const MoePiece<FR> &p, __amdgpu_buffer_rsrc_t terms, const uint32_t (&at)[NT],
-                                             int tiles, int i, int steps, int blocks, mx_v4f (&acc)[FR][NT]) {
+// A job's terms for a piece: this lane's column, its block of each step (`at`: bytes of that
+// of step 0, beyond the buffer where the column brings zeros; behind a row's end the next
+// row's or zeros come, which are not used).
+struct MoeTerms {
+    mx_bf8 v[4][4];
+};
+__device__ __forceinline__ void moe_terms(MoeTerms &x, __amdgpu_buffer_rsrc_t terms, uint32_t at, int i) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+            x.v[j][m] = __builtin_bit_cast(mx_bf8, bload16(terms, at + 1024u * (uint32_t)i + 256u * (uint32_t)j + 16u * (uint32_t)m, 0));
+}
+// acc[f] += the piece's rows times the terms; term(j, m): 8 of them of step j
+template <int FR, class F>
+__device__ __forceinline__ void moe_multiply(const MoePiece<FR> &p, F &&term, int i, int steps, int blocks, mx_v4f (&acc)[FR]) {
     const int q = (threadIdx.x & 63) >> 4;
-    mx_bf8 x[NT][4], next[NT][4];
-    auto get = [&](mx_bf8 (&d)[NT][4], int j) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-            if (n < tiles) {
-#pragma unroll
-                for (int m = 0; m < 4; m++)
-                    d[n][m] = __builtin_bit_cast(mx_bf8, bload16(terms, at[n] + 1024u * (uint32_t)i + 256u * (uint32_t)j + 16u * (uint32_t)m, 0));
-            }
-    };
-    get(x, 0);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if (4 * i + j >= steps) break;
-        if (j < 3) get(next, j + 1);  // (behind the row's end: the next row's, or zeros; not used)
         // (scales behind a row's last block may be anything: there 1)
         const bool in = 16 * i + 4 * j + q < blocks;
         float unit[FR];
@@ -402,19 +457,14 @@ __device__ __forceinline__ void moe_multiply(const MoePiece<FR> &p, __amdgpu_buf
         }
 #pragma unroll
         for (int m = 0; m < 4; m++) {
+            const mx_bf8 x = term(j, m);
 #pragma unroll
             for (int f = 0; f < FR; f++) {
                 const uint4 &c = p.c[f][j];
-                const mx_bf8 w = moe_widen(m == 0 ? c.x : m == 1 ? c.y : m == 2 ? c.z : c.w, unit[f]);
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-                    if (n < tiles) acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[n][m], acc[f][n], 0, 0, 0);
+                acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(moe_widen(m == 0 ? c.x : m == 1 ? c.y : m == 2 ? c.z : c.w, unit[f]), x,
+                                                                 acc[f], 0, 0, 0);
             }
         }
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int m = 0; m < 4; m++) x[n][m] = next[n][m];
     }
 }
 constexpr uint32_t kMoeNone = 0x80000000u;  // an offset beyond any buffer of terms
@@ -431,164 +481,246 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
     return mask ? __ffs((int)mask) - 1 : -1;
 }
 
-constexpr int kUpWaves = 4, kDownWaves = 8, kUpRows = 4;
-
 }  // namespace
 
-// Gate and up products of RU = 8 FR rows of a job a turn, K in pieces of 512 over the
-// wavefronts, and the weighted SwiGLU of their sums as bf16 terms. Jobs of at most `cap`
-// tokens, NT tiles.
-template <int NT> __global__ __launch_bounds__(64 * kUpWaves, 2)
-void k_moe_up(MoeLayerArgs a, MoeWork w, int terms, int hterms, int cap, int choosers) {
-    constexpr int W = kUpWaves, FR = kUpRows, RU = 8 * FR, H = FR / 2;  // fragments 0 .. H - 1: gate
-    extern __shared__ __align__(16) uint8_t smem[];  // keys of the choice, then the wavefronts' sums
+// A token's choice a wavefront, for more tokens than the up kernel's workgroups make it for
+// themselves.
+__global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs a, MoeWork w) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    moe_choose_token(a, w, blockIdx.x, reinterpret_cast<double *>(smem), true, nullptr);
+}
+
+// Gate and up products, and the weighted SwiGLU of their sums as bf16 terms. The pieces of K
+// go over `kw` of the wavefronts, XP each, whose terms a wavefront keeps while it goes through
+// a run of (job, 16 rows): its loads are the weights' alone, NB turns ahead. (Loads return in
+// order: terms fetched for every turn would wait for weights asked for before them.) With
+// XP = 0 there are more pieces than that, and their terms come with every turn. The
+// wavefronts' sums meet in LDS, where one of them finishes the turn.
+template <int XP, int TERMS> __global__ __launch_bounds__(64 * kWaves)
+void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
+    constexpr int W = kWaves, NB = XP == 1 ? 3 : 2, TPT = 16 / TERMS, NX = XP > 0 ? XP : 1;
+    extern __shared__ __align__(16) uint8_t smem[];  // keys of the choice, then sums [2][W][2][64][4]
     __shared__ MoePlan plan;
-    __shared__ uint32_t takes[kMoeMaxAll];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slots = a.k + a.n_shared, ff = a.n_ff, frow = pad128(ff), erow = pad128(a.n_embd);
-    moe_plan<W>(a, w, plan, cap, reinterpret_cast<double *>(smem), takes, choosers);
-    if (blockIdx.x == 0) moe_copy_plan<64 * W>(*w.plan, plan, a.n_tok * slots, plan.n_jobs);
+    moe_plan<W>(a, w, plan, TPT, reinterpret_cast<double *>(smem), choose);
     const size_t rb = mx_row_bytes(a.n_embd), sb = mx_scale_bytes(a.n_embd);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_embd + 31) / 32;
-    const int per = (ff + RU - 1) / RU, units = plan.n_jobs * per, tpt = 16 / terms;
+    const int per = (ff + 15) / 16, turns = plan.n_jobs * per;
     const __amdgpu_buffer_rsrc_t xt = make_rsrc(w.x, (uint32_t)a.n_tok * 3u * (uint32_t)erow * 2u);
-    float *const red = reinterpret_cast<float *>(smem);  // [W][FR][NT][64][4]
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
-        const int job = u / per, e = plan.job[job], r0 = u % per * RU;
+    float *const red = reinterpret_cast<float *>(smem);
+    // this wavefront's pieces (from `k` on, kw apart) and its group's run of turns
+    const int k = wv % kw, group = wv / kw, groups = W / kw, streams = (int)gridDim.x * groups;
+    const int stream = (int)blockIdx.x * groups + group;
+    const int from = (int)((long long)turns * stream / streams), to = (int)((long long)turns * (stream + 1) / streams);
+    const int rounds = (turns + streams - 1) / streams;  // of every wavefront, for the barriers
+    const int np = XP > 0 ? XP : (pieces + kw - 1) / kw;
+    MoeTerms x[NX];
+    MoePiece<2> p[NB];
+    auto fetch = [&](MoePiece<2> &d, int m) __attribute__((always_inline)) {  // piece m % np of turn m / np
+        const int turn = from + m / np, i = k + kw * (m % np);
+        if (turn < to && i < pieces) {
+            const size_t row = (size_t)plan.job[turn / per] * ff + min(turn % per * 16 + r, ff - 1);
+            const MoeRows rows[2] = {{a.gate + row * rb + 16 * q, a.gate_s + row * sb}, {a.up + row * rb + 16 * q, a.up_s + row * sb}};
+            moe_fetch<2>(d, rows, i, steps);
+        }
+    };
+    auto column = [&](int job) {  // this lane's
+        const int t = r < TPT * TERMS ? moe_token(plan.tokens[job], r / TERMS) : -1;
+        return t >= 0 ? (uint32_t)((t * 3 + r % TERMS) * erow + 32 * q) * 2u : kMoeNone;
+    };
+    int mine = -1;  // the job whose terms are held
+    uint32_t at = kMoeNone;
+    auto keep = [&](int job) __attribute__((always_inline)) {
+        if (job != mine) {
+            mine = job;
+            at = column(job);
+            if constexpr (XP > 0) {
+#pragma unroll
+                for (int n = 0; n < XP; n++) moe_terms(x[n], xt, at, k + kw * n);
+            }
+        }
+    };
+    if (from < to) keep(from / per);
+#pragma unroll
+    for (int b = 0; b < NB; b++) fetch(p[b], b);
+    mx_v4f acc[2];
+    // one of the NB buffers' turn (or, of more pieces, part of one)
+    auto part = [&](auto b_c, int m) __attribute__((always_inline)) {
+        constexpr int b = decltype(b_c)::value;
+        const int round = m / np, n = m % np, turn = from + round, i = k + kw * n;
+        const bool on = turn < to;
+        if (n == 0) {
+            acc[0] = acc[1] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            if (on) keep(turn / per);
+        }
+        if (on && i < pieces) {
+            if constexpr (XP > 0) {
+                auto mul = [&](const MoeTerms &t) __attribute__((always_inline)) {
+                    moe_multiply<2>(p[b], [&](int j, int h) { return t.v[j][h]; }, i, steps, blocks, acc);
+                };
+                mul(x[XP == 2 ? b : 0]);  // (buffer b: piece b of a turn)
+            } else {
+                moe_terms(x[0], xt, at, i);
+                moe_multiply<2>(p[b], [&](int j, int h) { return x[0].v[j][h]; }, i, steps, blocks, acc);
+            }
+        }
+        fetch(p[b], m + NB);
+        if (n != np - 1) return;
+        mx_v4f *const sums = reinterpret_cast<mx_v4f *>(red) + (round & 1) * W * 128;
+        sums[(wv * 2) * 64 + lane] = acc[0];
+        sums[(wv * 2 + 1) * 64 + lane] = acc[1];
+        // (LDS alone: the weights on their way are not waited for)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // One wavefront of the group finishes the turn. Its sums are not overwritten before
+        // the barrier of the next turn, which it reaches behind this.
+        if (!on || k != round % kw) return;
+        const int job = turn / per, e = plan.job[job], r0 = turn % per * 16;
         const uint32_t mask = plan.tokens[job];
-        const int count = __popc(mask), tiles = (count + tpt - 1) / tpt;
-        uint32_t at[NT];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int t = r < tpt * terms ? moe_token(mask, n * tpt + r / terms) : -1;
-            at[n] = t >= 0 ? (uint32_t)((t * 3 + r % terms) * erow + 32 * q) * 2u : kMoeNone;
-        }
-        MoeRows rows[FR];
-#pragma unroll
-        for (int f = 0; f < FR; f++) {
-            const size_t row = (size_t)e * ff + min(r0 + 16 * (f % H) + r, ff - 1);
-            rows[f].c = (f < H ? a.gate : a.up) + row * rb + 16 * q;
-            rows[f].s = (f < H ? a.gate_s : a.up_s) + row * sb;
-        }
-        mx_v4f acc[FR][NT];
-#pragma unroll
-        for (int f = 0; f < FR; f++)
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[f][n] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        MoePiece<FR> p;
-        if (wv < pieces) moe_fetch<FR>(p, rows, wv, steps);
-        for (int i = wv; i < pieces; i += W) {
-            const MoePiece<FR> now = p;
-            if (i + W < pieces) moe_fetch<FR>(p, rows, i + W, steps);
-            moe_multiply<FR, NT>(now, xt, at, tiles, i, steps, blocks, acc);
-        }
-        __syncthreads();  // (the last turn's sums are read)
-        mx_v4f *const part = reinterpret_cast<mx_v4f *>(red);
-#pragma unroll
-        for (int f = 0; f < FR; f++)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-                if (n < tiles) part[((wv * FR + f) * NT + n) * 64 + lane] = acc[f][n];
-        __syncthreads();
-        // a thread's row, a token a turn
-        const int row = tid % RU, lanes = 16 * ((row & 15) >> 2), k = row & 3;
-        for (int n = tid / RU; n < count; n += 64 * W / RU) {
-            const int t = moe_token(mask, n), i = moe_slot_of(a, plan, t, e);
+        const int count = __popc(mask), row = r;
+        for (int c0 = q; c0 < count; c0 += 4) {
+            const int t = moe_token(mask, c0), slot = moe_slot_of(a, plan, t, e);
+            const float *const src = reinterpret_cast<const float *>(sums) + (group * kw * 2 * 64 + c0 * TERMS + 16 * (row >> 2)) * 4 + (row & 3);
             float g = 0.0f, v = 0.0f;
-            for (int j = 0; j < terms; j++) {
-                const int c = n % tpt * terms + j;
-                const float *const src = red + ((row >> 4) * NT + n / tpt) * 256 + (c + lanes) * 4 + k;
+            for (int y = 0; y < kw; y++) {
 #pragma unroll
-                for (int x = 0; x < W; x++) {
-                    g += src[x * FR * NT * 256];
-                    v += src[(x * FR + H) * NT * 256];
+                for (int j = 0; j < TERMS; j++) {
+                    g += src[(y * 2 * 64 + j) * 4];
+                    v += src[((y * 2 + 1) * 64 + j) * 4];
                 }
             }
             if (a.clamp > 1e-6f) {
                 g = g > a.clamp ? a.clamp : g;
                 v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
             }
-            float h = r0 + row < ff ? g / (1.0f + expf(-g)) * v * plan.weight[t * slots + i] : 0.0f;
-            __bf16 *const dst = w.h + (size_t)(t * slots + i) * 3 * frow + r0 + row;
+            float h = r0 + row < ff ? g / (1.0f + expf(-g)) * v * plan.weight[t * slots + slot] : 0.0f;
+            __bf16 *const dst = w.h + (size_t)(t * slots + slot) * 3 * frow + r0 + row;
             for (int j = 0; j < hterms; j++) {
-                const __bf16 b = (__bf16)h;
-                if (r0 + row < frow) dst[j * frow] = b;
-                h = finite(h) ? h - (float)b : 0.0f;
-                if (r0 + RU >= ff)  // zeros up to whole steps
-                    for (int z = RU; r0 + row + z < frow; z += RU) dst[j * frow + z] = (__bf16)0.0f;
+                const __bf16 b16 = (__bf16)h;
+                dst[j * frow] = b16;
+                h = finite(h) ? h - (float)b16 : 0.0f;
+                if (r0 + 16 >= ff)  // zeros up to whole steps
+                    for (int z = 16; r0 + row + z < frow; z += 16) dst[j * frow + z] = (__bf16)0.0f;
             }
+        }
+    };
+    const int total = rounds * np;
+    for (int m = 0; m < total; m += NB) {
+        part(std::integral_constant<int, 0>{}, m);
+        if (m + 1 < total) part(std::integral_constant<int, 1>{}, m + 1);
+        if constexpr (NB == 3) {
+            if (m + 2 < total) part(std::integral_constant<int, 2>{}, m + 2);
         }
     }
 }
 
-// The down products of 16 rows a turn over all jobs, their pieces over the wavefronts, every
-// one of which adds its jobs' columns to sums of its own for each token.
-template <int NT> __global__ __launch_bounds__(64 * kDownWaves) void k_moe_down(MoeLayerArgs a, MoeWork w, int hterms) {
-    constexpr int W = kDownWaves;
+// The down products of 16 rows a turn over all jobs, (job, piece of K) over the wavefronts,
+// every one of which adds its jobs' columns to sums of its own for each token. LDS: h is read
+// from there, where it fits (few tokens): weights are then all that is waited for in order.
+template <bool LDS, int TERMS> __global__ __launch_bounds__(64 * kWaves)
+void k_moe_down(MoeLayerArgs a, MoeWork w) {
+    constexpr int W = kWaves, NB = 4, TPT = 16 / TERMS;
     __shared__ MoePlan plan;
-    extern __shared__ __align__(16) uint8_t smem[];  // sums [W][n_tok][16]
+    extern __shared__ __align__(16) uint8_t smem[];  // sums [W][n_tok][16], h [pairs][TERMS][frow]
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int slots = a.k + a.n_shared, frow = pad128(a.n_ff), n_jobs = w.plan->n_jobs;
-    moe_copy_plan<64 * W>(plan, *w.plan, a.n_tok * slots, n_jobs);
-    float *const sums = reinterpret_cast<float *>(smem), *const mine = sums + wv * a.n_tok * 16;
+    const int slots = a.k + a.n_shared, frow = pad128(a.n_ff), pairs = a.n_tok * slots;
+    float *const sums = reinterpret_cast<float *>(smem), *const own = sums + wv * a.n_tok * 16;
+    uint8_t *const hs = smem + (size_t)W * a.n_tok * 64;
+    if constexpr (LDS) {
+        const int row16 = frow / 8;  // 16-byte pieces of a row
+        for (int i = tid; i < pairs * TERMS * row16; i += 64 * W) {
+            const int pr = i / row16;
+            reinterpret_cast<uint4 *>(hs)[i] =
+                reinterpret_cast<const uint4 *>(w.h)[(size_t)(pr / TERMS * 3 + pr % TERMS) * row16 + i - pr * row16];
+        }
+    }
+    moe_plan<W>(a, w, plan, TPT, nullptr, 0);
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
-    const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32, tpt = 16 / hterms;
-    const __amdgpu_buffer_rsrc_t ht = make_rsrc(w.h, (uint32_t)(a.n_tok * slots) * 3u * (uint32_t)frow * 2u);
-    const int total = n_jobs * pieces;
+    const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
+    const __amdgpu_buffer_rsrc_t ht = make_rsrc(w.h, (uint32_t)pairs * 3u * (uint32_t)frow * 2u);
+    const int total = plan.n_jobs * pieces;
     const int from = (int)((long long)total * wv / W), to = (int)((long long)total * (wv + 1) / W);
     for (int r0 = blockIdx.x * 16; r0 < a.n_embd; r0 += gridDim.x * 16) {
-        __syncthreads();  // (the plan is there, the last turn's sums are read)
-        for (int i = lane; i < a.n_tok * 16; i += 64) mine[i] = 0.0f;
+        __syncthreads();  // (the last turn's sums are read)
+        for (int i = lane; i < a.n_tok * 16; i += 64) own[i] = 0.0f;
         const size_t row = (size_t)min(r0 + r, a.n_embd - 1);
-        MoePiece<1> next;
-        auto fetch = [&](int c) __attribute__((always_inline)) {
+        MoePiece<1> p[NB];
+        MoeTerms x[2];
+        auto fetch = [&](MoePiece<1> &d, int c) __attribute__((always_inline)) {
             if (c < to) {
                 const size_t e = plan.job[c / pieces];
                 const MoeRows rows[1] = {{a.down + (e * a.n_embd + row) * rb + 16 * q, a.down_s + (e * a.n_embd + row) * sb}};
-                moe_fetch<1>(next, rows, c % pieces, steps);
+                moe_fetch<1>(d, rows, c % pieces, steps);
             }
         };
-        fetch(from);
-        for (int c = from; c < to;) {
-            const int job = c / pieces, e = plan.job[job], end = min(to, (job + 1) * pieces);
-            const uint32_t mask = plan.tokens[job];
-            const int tiles = (__popc(mask) + tpt - 1) / tpt;
-            int tok[NT];
-            uint32_t at[NT];
-            mx_v4f acc[1][NT];
+        // this lane's column of a job: its token, and where its terms lie
+        int tok = -1, tok_next = -1, job = -1, job_next = -1;
+        uint32_t at = kMoeNone, at_next = kMoeNone;
+        auto column = [&](int j) __attribute__((always_inline)) {
+            if (j == job_next) return;
+            job_next = j;
+            tok_next = r < TPT * TERMS ? moe_token(plan.tokens[j], r / TERMS) : -1;
+            const int pair = tok_next >= 0 ? tok_next * slots + moe_slot_of(a, plan, tok_next, plan.job[j]) : 0;
+            at_next = tok_next >= 0 ? (uint32_t)((pair * (LDS ? TERMS : 3) + r % TERMS) * frow + 32 * q) * 2u : kMoeNone;
+        };
+        mx_v4f acc[1] = {mx_v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+        // a token's terms stand in neighbouring lanes: to the first of them, and to its sums
+        auto flush = [&]() __attribute__((always_inline)) {
+            mx_v4f y = acc[0];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                tok[n] = r < tpt * hterms ? moe_token(mask, n * tpt + r / hterms) : -1;
-                at[n] = tok[n] >= 0 ? (uint32_t)(((tok[n] * slots + moe_slot_of(a, plan, tok[n], e)) * 3 + r % hterms) * frow + 32 * q) * 2u
-                                    : kMoeNone;
-                acc[0][n] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 4; i++) {
+                const float v1 = __shfl_down(acc[0][i], 1, 64), v2 = __shfl_down(acc[0][i], 2, 64);
+                y[i] += TERMS == 3 ? v1 + v2 : v1;
             }
-            for (; c < end; c++) {
-                const MoePiece<1> now = next;
-                fetch(c + 1);
-                moe_multiply<1, NT>(now, ht, at, tiles, c % pieces, steps, blocks, acc);
-            }
-            // a token's terms stand in neighbouring lanes: to the first of them, and to its sums
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                if (n >= tiles) continue;
-                mx_v4f y = acc[0][n];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float v1 = __shfl_down(acc[0][n][k], 1, 64), v2 = __shfl_down(acc[0][n][k], 2, 64);
-                    y[k] += hterms == 3 ? v1 + v2 : v1;
-                }
-                if (tok[n] >= 0 && r % hterms == 0) *reinterpret_cast<mx_v4f *>(mine + tok[n] * 16 + 4 * q) += y;
-            }
+            if (tok >= 0 && r % TERMS == 0) *reinterpret_cast<mx_v4f *>(own + tok * 16 + 4 * q) += y;
+            acc[0] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        };
+        if (from < to) {
+            column(from / pieces);
+            if constexpr (!LDS) moe_terms(x[0], ht, at_next, from % pieces);
         }
+#pragma unroll
+        for (int b = 0; b < NB; b++) fetch(p[b], from + b);
+        auto part = [&](auto b_c, int c) __attribute__((always_inline)) {
+            constexpr int b = decltype(b_c)::value;
+            if (c / pieces != job) {
+                if (job >= 0) flush();
+                column(c / pieces);
+                job = job_next;
+                tok = tok_next;
+                at = at_next;
+            }
+            const int i = c % pieces;
+            if constexpr (LDS) {
+                const uint8_t *const src = hs + (at == kMoeNone ? 0u : at) + 1024 * i;
+                moe_multiply<1>(p[b], [&](int j, int m) {
+                    const mx_bf8 v = *reinterpret_cast<const mx_bf8 *>(src + 256 * j + 16 * m);
+                    return at == kMoeNone ? mx_bf8{} : v;
+                }, i, steps, blocks, acc);
+            } else {
+                if (c + 1 < to) {
+                    column((c + 1) / pieces);
+                    moe_terms(x[(b + 1) & 1], ht, at_next, (c + 1) % pieces);
+                }
+                moe_multiply<1>(p[b], [&](int j, int m) { return x[b & 1].v[j][m]; }, i, steps, blocks, acc);
+            }
+            fetch(p[b], c + NB);
+        };
+        for (int c = from; c < to; c += NB) {
+            part(std::integral_constant<int, 0>{}, c);
+            if (c + 1 < to) part(std::integral_constant<int, 1>{}, c + 1);
+            if (c + 2 < to) part(std::integral_constant<int, 2>{}, c + 2);
+            if (c + 3 < to) part(std::integral_constant<int, 3>{}, c + 3);
+        }
+        if (job >= 0) flush();
         __syncthreads();
         for (int i = tid; i < a.n_tok * 16; i += 64 * W) {
             const int t = i >> 4, o = r0 + (i & 15);
             float y = 0.0f;
 #pragma unroll
-            for (int x = 0; x < W; x++) y += sums[x * a.n_tok * 16 + i];
+            for (int v = 0; v < W; v++) y += sums[v * a.n_tok * 16 + i];
             if (o < a.n_embd) mx_store(a.out, (size_t)t * a.out_stride + o, w.bad[t] ? __builtin_nanf("") : y, a.dtype_out);
         }
     }
@@ -604,26 +736,72 @@ template <uint32_t DX> void moe_in_go(const MoeLayerArgs &a, const MoeWork &w, h
     const int size = DX == T_F32 ? 4 : 2, rsize = a.dtype_router == T_F32 ? 4 : 2;
     const int vx = (uintptr_t)a.x % 16 == 0 && a.x_stride * size % 16 == 0;
     const int vr = (uintptr_t)a.router % 16 == 0 && (size_t)a.n_embd * rsize % 16 == 0;
-    const dim3 g((unsigned)(a.n_expert + a.n_tok));
-    if (a.dtype_router == T_F32) k_moe_in<DX, T_F32><<<g, 256, 0, s>>>(a, w, vx, vr);
-    else if (a.dtype_router == T_F16) k_moe_in<DX, T_F16><<<g, 256, 0, s>>>(a, w, vx, vr);
-    else k_moe_in<DX, T_BF16><<<g, 256, 0, s>>>(a, w, vx, vr);
+    const dim3 g((unsigned)(a.n_expert + a.n_tok)), n(64 * kInWaves);
+    if (a.dtype_router == T_F32) k_moe_in<DX, T_F32><<<g, n, 0, s>>>(a, w, vx, vr);
+    else if (a.dtype_router == T_F16) k_moe_in<DX, T_F16><<<g, n, 0, s>>>(a, w, vx, vr);
+    else k_moe_in<DX, T_BF16><<<g, n, 0, s>>>(a, w, vx, vr);
 }
 
-template <int NT> hipError_t moe_go(const MoeLayerArgs &a, const MoeWork &w, int terms, int hterms, hipStream_t s) {
-    const int cap = NT * (16 / std::max(terms, hterms));
-    // 48 KB at most for the choice's keys and the sums
-    const size_t keys = (size_t)(a.n_expert + a.n_group) * 8, sums = (size_t)kUpWaves * kUpRows * NT * 1024;
-    static_assert(kUpWaves * kUpRows * NT <= 48, "LDS");
-    const int choosers = (int)std::min((size_t)kUpWaves, (size_t)48 * 1024 / keys);
-    const int pairs = a.n_tok * (a.k + a.n_shared);  // at most as many jobs
-    const long long units = (long long)pairs * ((a.n_ff + 8 * kUpRows - 1) / (8 * kUpRows));
-    k_moe_up<NT><<<(unsigned)std::min(units, (long long)512), 64 * kUpWaves, std::max(choosers * keys, sums), s>>>(
-        a, w, terms, hterms, cap, choosers);
-    hipError_t e = hipGetLastError();
+// More LDS than a kernel gets unasked, asked for until the runtime has granted it once on
+// the current device: a refusal is that call's error alone.
+template <int KERNEL> hipError_t moe_allow_lds(const void *kernel, size_t bytes) {
+    static std::atomic<uint64_t> granted{0};  // a bit a device; beyond 64 it is asked every time
+    int dev;
+    hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return e;
-    k_moe_down<NT><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kDownWaves, (size_t)kDownWaves * a.n_tok * 64, s>>>(a, w, hterms);
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (granted.load(std::memory_order_acquire) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess) granted.fetch_or(bit, std::memory_order_release);
+    else (void)hipGetLastError();  // (or the next launch would report it)
+    return e;
+}
+
+// Tokens up to which the up kernel's workgroups make the choice for themselves: one a
+// wavefront.
+constexpr int kChooseTok = kWaves;
+
+template <int XP, int TERMS>
+hipError_t moe_up_go(const MoeLayerArgs &a, const MoeWork &w, int hterms, int kw, hipStream_t s) {
+    // 32 KB of sums, and no more than 48 for the choice's keys
+    const size_t keys = (size_t)(a.n_expert + a.n_group) * 8;
+    int choose = 0;
+    if (a.n_tok <= kChooseTok) {
+        choose = (int)std::min((size_t)kWaves, 48 * 1024 / keys);
+    } else {
+        k_moe_choose<<<(unsigned)a.n_tok, 64, keys, s>>>(a, w);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    // a workgroup a CU, no more than there can be turns
+    const long long turns = (long long)a.n_tok * (a.k + a.n_shared) * ((a.n_ff + 15) / 16);
+    const long long wgs = (turns * kw + kWaves - 1) / kWaves;
+    k_moe_up<XP, TERMS><<<(unsigned)std::min(wgs, (long long)256), 64 * kWaves, std::max(choose * keys, (size_t)kWaves * 4096), s>>>(
+        a, w, hterms, kw, choose);
     return hipGetLastError();
+}
+template <int TERMS> hipError_t moe_up(const MoeLayerArgs &a, const MoeWork &w, int hterms, hipStream_t s) {
+    const int pieces = (int)mx_scale_bytes(a.n_embd) / 16;
+    if (pieces > 2 * kWaves) return moe_up_go<0, TERMS>(a, w, hterms, kWaves, s);
+    if (pieces > kWaves) return moe_up_go<2, TERMS>(a, w, hterms, kWaves, s);
+    const int kw = pieces > 4 ? 8 : pieces > 2 ? 4 : pieces;
+    return moe_up_go<1, TERMS>(a, w, hterms, kw, s);
+}
+
+// LDS of the down kernel's sums and h, up to which h is held there.
+constexpr size_t kDownLds = 128 * 1024;
+
+template <bool LDS, int TERMS> hipError_t moe_down_go(const MoeLayerArgs &a, const MoeWork &w, size_t lds, hipStream_t s) {
+    if (LDS) {
+        const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<LDS, TERMS>), kDownLds);
+        if (e != hipSuccess) return e;
+    }
+    k_moe_down<LDS, TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, lds, s>>>(a, w);
+    return hipGetLastError();
+}
+template <int TERMS> hipError_t moe_down(const MoeLayerArgs &a, const MoeWork &w, hipStream_t s) {
+    const size_t sums = (size_t)kWaves * a.n_tok * 64, h = (size_t)a.n_tok * (a.k + a.n_shared) * TERMS * pad128(a.n_ff) * 2;
+    return sums + h <= kDownLds ? moe_down_go<true, TERMS>(a, w, sums + h, s) : moe_down_go<false, TERMS>(a, w, sums, s);
 }
 
 }  // namespace
@@ -632,14 +810,15 @@ hipError_t launch_moe_layer(const MoeLayerArgs &a, uint8_t *work, hipStream_t s)
     if (a.n_tok <= 0) return hipSuccess;
     MoeWork w;
     moe_parts(a.n_tok, a.n_embd, a.n_ff, a.n_expert, a.k, a.n_shared, work, &w);
-    const int terms = a.dtype_x == T_F32 ? 3 : a.dtype_x == T_F16 ? 2 : 1, hterms = a.dtype_out == T_F32 ? 3 : 2;
+    const int hterms = a.dtype_out == T_F32 ? 3 : 2;
     if (a.dtype_x == T_F32) moe_in_go<T_F32>(a, w, s);
     else if (a.dtype_x == T_F16) moe_in_go<T_F16>(a, w, s);
     else moe_in_go<T_BF16>(a, w, s);
-    const hipError_t e = hipGetLastError();
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // one tile where it holds every token
-    return a.n_tok <= 16 / std::max(terms, hterms) ? moe_go<1>(a, w, terms, hterms, s) : moe_go<2>(a, w, terms, hterms, s);
+    e = a.dtype_x == T_F32 ? moe_up<3>(a, w, hterms, s) : a.dtype_x == T_F16 ? moe_up<2>(a, w, hterms, s) : moe_up<1>(a, w, hterms, s);
+    if (e != hipSuccess) return e;
+    return hterms == 3 ? moe_down<3>(a, w, s) : moe_down<2>(a, w, s);
 }
 
 }  // namespace rsllm_hip
