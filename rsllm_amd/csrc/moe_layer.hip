@@ -17,6 +17,8 @@ namespace rsllm_hip {
 namespace {
 
 constexpr int kInWaves = 16, kWaves = 8;
+constexpr int kBatch = 4;
+constexpr size_t kDownLds = 112 * 1024;  // of h in LDS, beside the sums
 constexpr int kMoeMaxExpert = 1024, kMoeMaxShared = 8, kMoeMaxSlots = 40;
 constexpr int kMoeMaxPairs = kMoeMaxTok * kMoeMaxSlots, kMoeMaxAll = kMoeMaxExpert + kMoeMaxShared;
 
@@ -178,11 +180,20 @@ __device__ __forceinline__ uint64_t order64(double v) {
 __device__ __forceinline__ int moe_best(uint64_t key, int id) {
     const uint32_t hi = (uint32_t)(key >> 32), lo = (uint32_t)key;
     const uint32_t mh = wave_max_u32(hi);
-    const uint32_t ml = wave_max_u32(hi == mh ? lo : 0u);
-    const bool in = hi == mh && lo == ml;
-    if (((uint64_t)mh << 32 | ml) <= order64(kNever)) return -1;
-    const uint32_t mi = wave_max_u32(in ? ~(uint32_t)id : 0u);
-    return __ffsll((unsigned long long)__ballot(in && ~(uint32_t)id == mi)) - 1;
+    bool in = hi == mh;
+    unsigned long long who = __ballot(in);
+    if (who & (who - 1)) {  // rarely: the lower halves, then the ids
+        const uint32_t ml = wave_max_u32(in ? lo : 0u);
+        in = in && lo == ml;
+        who = __ballot(in);
+        if (who & (who - 1)) {
+            const uint32_t mi = wave_max_u32(in ? ~(uint32_t)id : 0u);
+            who = __ballot(in && ~(uint32_t)id == mi);
+        }
+    }
+    const int lane = __ffsll(who) - 1;
+    const uint64_t best = (uint64_t)mh << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, lane);
+    return best <= order64(kNever) ? -1 : lane;
 }
 
 // A wavefront's choice for a token of logits l: id and weight of slot r at lane r, -1 and 0
@@ -191,26 +202,26 @@ __device__ __forceinline__ int moe_best(uint64_t key, int id) {
 template <int R>
 __device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *l, const double *scores, double *key,
                                            double *gsum, int &id, float &weight) {
+    constexpr int N = R > 0 ? R : 1;
     const int lane = threadIdx.x & 63, per = a.n_expert / a.n_group;
-    double m = kNever, sum = 0.0;
-    auto score = [&](int e, double le) { return a.score == ROUTE_SOFTMAX ? route_exp(le, m) / sum : scores[e]; };
-    auto place = [&](int e, double le) {
-        double p = kNever;
-        if (le > kNever) {  // (a NaN is not)
-            p = a.bias || a.n_group > 1 ? score(e, le) + (a.bias ? (double)a.bias[e] : 0.0) : le;
-            if (!(p > kNever)) p = kNever;
-        }
-        return p;
-    };
-    double own[R > 0 ? R : 1], lg[R > 0 ? R : 1];
-    if constexpr (R > 0) {
+    const bool soft = a.score == ROUTE_SOFTMAX, scored = a.bias || a.n_group > 1;
+    double m = kNever, sum = 0.0, own[N], lg[N], sc[N];
+    float bias[N];
+    if constexpr (R > 0) {  // (all of them asked for at once)
 #pragma unroll
-        for (int j = 0; j < R; j++) lg[j] = lane + 64 * j < a.n_expert ? l[lane + 64 * j] : kNever;
+        for (int j = 0; j < R; j++) {
+            const int e = min(lane + 64 * j, a.n_expert - 1);
+            lg[j] = l[e];
+            sc[j] = soft ? 0.0 : scores[e];
+            bias[j] = a.bias ? a.bias[e] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < R; j++) lg[j] = lane + 64 * j < a.n_expert ? lg[j] : kNever;
     }
-    if (a.score == ROUTE_SOFTMAX) {
+    if (soft) {
         if constexpr (R > 0) {
 #pragma unroll
-            for (int j = 0; j < R; j++) m = lg[j] > m ? lg[j] : m;
+            for (int j = 0; j < R; j++) m = lg[j] > m ? lg[j] : m;  // (a NaN is not)
         } else {
             for (int e = lane; e < a.n_expert; e += 64) m = l[e] > m ? l[e] : m;
         }
@@ -218,26 +229,37 @@ __device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *
         for (int off = 32; off >= 1; off >>= 1) m = fmax(m, __shfl_xor(m, off, 64));
         if constexpr (R > 0) {
 #pragma unroll
-            for (int j = 0; j < R; j++) sum += lg[j] > kNever ? route_exp(lg[j], m) : 0.0;
+            for (int j = 0; j < R; j++) {
+                sc[j] = lg[j] > kNever ? route_exp(lg[j], m) : 0.0;
+                sum += sc[j];
+            }
         } else {
             for (int e = lane; e < a.n_expert; e += 64)
                 if (l[e] > kNever) sum += route_exp(l[e], m);
         }
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int j = 0; j < R; j++) sc[j] /= sum;
+        }
     }
+    auto score = [&](int e) { return soft ? route_exp(l[e], m) / sum : scores[e]; };
+    auto place = [&](double le, double s, float b) {
+        const double p = scored ? s + (double)b : le;
+        return le > kNever && p > kNever ? p : kNever;
+    };
     if constexpr (R > 0) {
 #pragma unroll
-        for (int j = 0; j < R; j++) own[j] = lane + 64 * j < a.n_expert ? place(lane + 64 * j, lg[j]) : kNever;
-    }
-    if constexpr (R > 0) {
+        for (int j = 0; j < R; j++) own[j] = place(lg[j], sc[j], bias[j]);
         if (a.n_group > 1) {
 #pragma unroll
             for (int j = 0; j < R; j++)
                 if (lane + 64 * j < a.n_expert) key[lane + 64 * j] = own[j];
         }
     } else {
-        for (int e = lane; e < a.n_expert; e += 64) key[e] = place(e, l[e]);
+        for (int e = lane; e < a.n_expert; e += 64)
+            key[e] = place(l[e], scored ? score(e) : 0.0, a.bias ? a.bias[e] : 0.0f);
     }
     __builtin_amdgcn_wave_barrier();
     if (a.n_group > 1) {
@@ -274,15 +296,21 @@ __device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *
             __builtin_amdgcn_wave_barrier();
         }
     }
-    // every lane's best of its keys; the one that gives it looks for its next
-    double v = kNever;
-    int i = a.n_expert;
+    // every lane's best of its keys (and its score); the one that gives it looks for its next
+    double v, vs = 0.0, s = 0.0;
+    int i;
     auto best = [&]() __attribute__((always_inline)) {
         v = kNever;
         i = a.n_expert;
         if constexpr (R > 0) {
 #pragma unroll
-            for (int j = 0; j < R; j++) route_best(v, i, own[j], lane + 64 * j);
+            for (int j = 0; j < R; j++) {
+                if (route_before(own[j], lane + 64 * j, v, i)) {
+                    v = own[j];
+                    vs = sc[j];
+                    i = lane + 64 * j;
+                }
+            }
         } else {
             for (int e = lane; e < a.n_expert; e += 64) route_best(v, i, key[e], e);
         }
@@ -293,7 +321,13 @@ __device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *
         const int who = moe_best(order64(v), i);
         if (who < 0) break;
         const int chosen = __builtin_amdgcn_readlane(i, who);
-        if (lane == r) id = chosen;
+        const uint64_t bits = __builtin_bit_cast(uint64_t, vs);
+        const uint32_t s0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, who);
+        const uint32_t s1 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), who);
+        if (lane == r) {
+            id = chosen;
+            s = __builtin_bit_cast(double, (uint64_t)s1 << 32 | s0);
+        }
         if (lane == who) {
             if constexpr (R > 0) {
 #pragma unroll
@@ -304,14 +338,14 @@ __device__ __forceinline__ void moe_choose(const MoeLayerArgs &a, const double *
             best();
         }
     }
-    const double s = id >= 0 ? score(id, a.score == ROUTE_SOFTMAX ? l[id] : 0.0) : 0.0;
-    double total = s;
+    if constexpr (R == 0) s = id >= 0 ? score(id) : 0.0;
+    double out = s * (double)a.scale;
     if (a.renormalise) {
+        double total = s;
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
+        out = total == 0.0 ? 0.0 : out / total;
     }
-    double out = s * (double)a.scale;
-    if (a.renormalise) out = total == 0.0 ? 0.0 : out / total;
     weight = id >= 0 ? (float)out : 0.0f;
 }
 // A slot of the plan.
@@ -495,11 +529,11 @@ __global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs a, MoeWork w) {
 // a run of (job, 16 rows): its loads are the weights' alone, NB turns ahead. (Loads return in
 // order: terms fetched for every turn would wait for weights asked for before them.) With
 // XP = 0 there are more pieces than that, and their terms come with every turn. The
-// wavefronts' sums meet in LDS, where one of them finishes the turn.
+// wavefronts' sums meet in LDS, where kBatch turns are finished at once.
 template <int XP, int TERMS> __global__ __launch_bounds__(64 * kWaves)
 void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     constexpr int W = kWaves, NB = XP == 1 ? 3 : 2, TPT = 16 / TERMS, NX = XP > 0 ? XP : 1;
-    extern __shared__ __align__(16) uint8_t smem[];  // keys of the choice, then sums [2][W][2][64][4]
+    extern __shared__ __align__(16) uint8_t smem[];  // keys of the choice, then sums [kBatch][W][2][64][4]
     __shared__ MoePlan plan;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -545,6 +579,47 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     if (from < to) keep(from / per);
 #pragma unroll
     for (int b = 0; b < NB; b++) fetch(p[b], b);
+    // The turns from round b0 on, all wavefronts' sums of which are in LDS: a token of one of
+    // them for every 16 lanes (rows). (LDS alone is waited for, not the weights on their way.)
+    auto finish = [&](int b0) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int task = wv * 4 + q; task < kBatch * groups * TPT; task += W * 4) {
+            const int c0 = task % TPT, g0 = task / TPT % groups, b = task / TPT / groups;
+            const int s0 = (int)blockIdx.x * groups + g0;
+            const int turn = (int)((long long)turns * s0 / streams) + b0 + b;
+            if (b0 + b >= rounds || turn >= (int)((long long)turns * (s0 + 1) / streams)) continue;
+            const int job = turn / per, e = plan.job[job], r0 = turn % per * 16;
+            const int t = moe_token(plan.tokens[job], c0);
+            if (t < 0) continue;
+            const int slot = moe_slot_of(a, plan, t, e);
+            const float *const src = red + ((b * W + g0 * kw) * 2 * 64 + c0 * TERMS + 16 * (r >> 2)) * 4 + (r & 3);
+            float g = 0.0f, v = 0.0f;
+#pragma unroll
+            for (int y = 0; y < W; y++) {
+                if (y < kw) {
+#pragma unroll
+                    for (int j = 0; j < TERMS; j++) {
+                        g += src[(y * 2 * 64 + j) * 4];
+                        v += src[((y * 2 + 1) * 64 + j) * 4];
+                    }
+                }
+            }
+            if (a.clamp > 1e-6f) {
+                g = g > a.clamp ? a.clamp : g;
+                v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
+            }
+            float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[t * slots + slot] : 0.0f;
+            __bf16 *const dst = w.h + (size_t)(t * slots + slot) * 3 * frow + r0 + r;
+            for (int j = 0; j < hterms; j++) {
+                const __bf16 b16 = (__bf16)h;
+                dst[j * frow] = b16;
+                h = finite(h) ? h - (float)b16 : 0.0f;
+                if (r0 + 16 >= ff)  // zeros up to whole steps
+                    for (int z = 16; r0 + r + z < frow; z += 16) dst[j * frow + z] = (__bf16)0.0f;
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
     mx_v4f acc[2];
     // one of the NB buffers' turn (or, of more pieces, part of one)
     auto part = [&](auto b_c, int m) __attribute__((always_inline)) {
@@ -567,42 +642,11 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
             }
         }
         fetch(p[b], m + NB);
-        if (n != np - 1) return;
-        mx_v4f *const sums = reinterpret_cast<mx_v4f *>(red) + (round & 1) * W * 128;
-        sums[(wv * 2) * 64 + lane] = acc[0];
-        sums[(wv * 2 + 1) * 64 + lane] = acc[1];
-        // (LDS alone: the weights on their way are not waited for)
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        // One wavefront of the group finishes the turn. Its sums are not overwritten before
-        // the barrier of the next turn, which it reaches behind this.
-        if (!on || k != round % kw) return;
-        const int job = turn / per, e = plan.job[job], r0 = turn % per * 16;
-        const uint32_t mask = plan.tokens[job];
-        const int count = __popc(mask), row = r;
-        for (int c0 = q; c0 < count; c0 += 4) {
-            const int t = moe_token(mask, c0), slot = moe_slot_of(a, plan, t, e);
-            const float *const src = reinterpret_cast<const float *>(sums) + (group * kw * 2 * 64 + c0 * TERMS + 16 * (row >> 2)) * 4 + (row & 3);
-            float g = 0.0f, v = 0.0f;
-            for (int y = 0; y < kw; y++) {
-#pragma unroll
-                for (int j = 0; j < TERMS; j++) {
-                    g += src[(y * 2 * 64 + j) * 4];
-                    v += src[((y * 2 + 1) * 64 + j) * 4];
-                }
-            }
-            if (a.clamp > 1e-6f) {
-                g = g > a.clamp ? a.clamp : g;
-                v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
-            }
-            float h = r0 + row < ff ? g / (1.0f + expf(-g)) * v * plan.weight[t * slots + slot] : 0.0f;
-            __bf16 *const dst = w.h + (size_t)(t * slots + slot) * 3 * frow + r0 + row;
-            for (int j = 0; j < hterms; j++) {
-                const __bf16 b16 = (__bf16)h;
-                dst[j * frow] = b16;
-                h = finite(h) ? h - (float)b16 : 0.0f;
-                if (r0 + 16 >= ff)  // zeros up to whole steps
-                    for (int z = 16; r0 + row + z < frow; z += 16) dst[j * frow + z] = (__bf16)0.0f;
-            }
+        if (n == np - 1) {
+            mx_v4f *const sums = reinterpret_cast<mx_v4f *>(red) + round % kBatch * W * 128;
+            sums[(wv * 2) * 64 + lane] = acc[0];
+            sums[(wv * 2 + 1) * 64 + lane] = acc[1];
+            if (round % kBatch == kBatch - 1 || round == rounds - 1) finish(round / kBatch * kBatch);
         }
     };
     const int total = rounds * np;
@@ -628,15 +672,27 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
     const int slots = a.k + a.n_shared, frow = pad128(a.n_ff), pairs = a.n_tok * slots;
     float *const sums = reinterpret_cast<float *>(smem), *const own = sums + wv * a.n_tok * 16;
     uint8_t *const hs = smem + (size_t)W * a.n_tok * 64;
+    // h, in chunks of 512 of a row, on its way while the plan is made
+    constexpr int kChunks = LDS ? (int)(kDownLds / 1024) / W : 1;
+    const int cpr = (frow + 511) / 512, chunks = pairs * TERMS * cpr;
+    uint4 held[kChunks];
     if constexpr (LDS) {
-        const int row16 = frow / 8;  // 16-byte pieces of a row
-        for (int i = tid; i < pairs * TERMS * row16; i += 64 * W) {
-            const int pr = i / row16;
-            reinterpret_cast<uint4 *>(hs)[i] =
-                reinterpret_cast<const uint4 *>(w.h)[(size_t)(pr / TERMS * 3 + pr % TERMS) * row16 + i - pr * row16];
+#pragma unroll
+        for (int i = 0; i < kChunks; i++) {
+            const int c = wv + W * i, hr = c / cpr, col = 512 * (c - hr * cpr) + 8 * lane;
+            held[i] = make_uint4(0, 0, 0, 0);
+            if (c < chunks && col < frow)
+                held[i] = *reinterpret_cast<const uint4 *>(w.h + (size_t)(hr / TERMS * 3 + hr % TERMS) * frow + col);
         }
     }
     moe_plan<W>(a, w, plan, TPT, nullptr, 0);
+    if constexpr (LDS) {
+#pragma unroll
+        for (int i = 0; i < kChunks; i++) {
+            const int c = wv + W * i, hr = c / cpr, col = 512 * (c - hr * cpr) + 8 * lane;
+            if (c < chunks && col < frow) *reinterpret_cast<uint4 *>(hs + ((size_t)hr * frow + col) * 2) = held[i];
+        }
+    }
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
     const __amdgpu_buffer_rsrc_t ht = make_rsrc(w.h, (uint32_t)pairs * 3u * (uint32_t)frow * 2u);
@@ -763,7 +819,7 @@ constexpr int kChooseTok = kWaves;
 
 template <int XP, int TERMS>
 hipError_t moe_up_go(const MoeLayerArgs &a, const MoeWork &w, int hterms, int kw, hipStream_t s) {
-    // 32 KB of sums, and no more than 48 for the choice's keys
+    // sums, and no more than 48 KB for the choice's keys
     const size_t keys = (size_t)(a.n_expert + a.n_group) * 8;
     int choose = 0;
     if (a.n_tok <= kChooseTok) {
@@ -776,7 +832,10 @@ hipError_t moe_up_go(const MoeLayerArgs &a, const MoeWork &w, int hterms, int kw
     // a workgroup a CU, no more than there can be turns
     const long long turns = (long long)a.n_tok * (a.k + a.n_shared) * ((a.n_ff + 15) / 16);
     const long long wgs = (turns * kw + kWaves - 1) / kWaves;
-    k_moe_up<XP, TERMS><<<(unsigned)std::min(wgs, (long long)256), 64 * kWaves, std::max(choose * keys, (size_t)kWaves * 4096), s>>>(
+    constexpr size_t sums = (size_t)kBatch * kWaves * 2048;
+    const hipError_t e = moe_allow_lds<16 * XP + TERMS + 8>(reinterpret_cast<const void *>(&k_moe_up<XP, TERMS>), sums);
+    if (e != hipSuccess) return e;
+    k_moe_up<XP, TERMS><<<(unsigned)std::min(wgs, (long long)256), 64 * kWaves, std::max(choose * keys, sums), s>>>(
         a, w, hterms, kw, choose);
     return hipGetLastError();
 }
@@ -788,20 +847,19 @@ template <int TERMS> hipError_t moe_up(const MoeLayerArgs &a, const MoeWork &w, 
     return moe_up_go<1, TERMS>(a, w, hterms, kw, s);
 }
 
-// LDS of the down kernel's sums and h, up to which h is held there.
-constexpr size_t kDownLds = 128 * 1024;
-
 template <bool LDS, int TERMS> hipError_t moe_down_go(const MoeLayerArgs &a, const MoeWork &w, size_t lds, hipStream_t s) {
     if (LDS) {
-        const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<LDS, TERMS>), kDownLds);
+        const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<LDS, TERMS>), kDownLds + kWaves * kMoeMaxTok * 64);
         if (e != hipSuccess) return e;
     }
     k_moe_down<LDS, TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, lds, s>>>(a, w);
     return hipGetLastError();
 }
 template <int TERMS> hipError_t moe_down(const MoeLayerArgs &a, const MoeWork &w, hipStream_t s) {
-    const size_t sums = (size_t)kWaves * a.n_tok * 64, h = (size_t)a.n_tok * (a.k + a.n_shared) * TERMS * pad128(a.n_ff) * 2;
-    return sums + h <= kDownLds ? moe_down_go<true, TERMS>(a, w, sums + h, s) : moe_down_go<false, TERMS>(a, w, sums, s);
+    // (a row of h is copied in chunks of 1 KB)
+    const size_t sums = (size_t)kWaves * a.n_tok * 64, rows = (size_t)a.n_tok * (a.k + a.n_shared) * TERMS;
+    const size_t h = rows * pad128(a.n_ff) * 2, chunks = rows * ((pad128(a.n_ff) + 511) / 512) * 1024;
+    return chunks <= kDownLds ? moe_down_go<true, TERMS>(a, w, sums + h, s) : moe_down_go<false, TERMS>(a, w, sums, s);
 }
 
 }  // namespace
