@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kInWaves = 16, kWaves = 8;
 constexpr int kBatch = 4;
-constexpr size_t kDownLds = 112 * 1024;  // of h in LDS, beside the sums
+constexpr int kDownColumns = 6;  // of a job: two tokens of three terms, three of two
 constexpr int kMoeMaxExpert = 1024, kMoeMaxShared = 8, kMoeMaxSlots = 40;
 constexpr int kMoeMaxPairs = kMoeMaxTok * kMoeMaxSlots, kMoeMaxAll = kMoeMaxExpert + kMoeMaxShared;
 
@@ -660,67 +660,62 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
 }
 
 // The down products of 16 rows a turn over all jobs, (job, piece of K) over the wavefronts,
-// every one of which adds its jobs' columns to sums of its own for each token. LDS: h is read
-// from there, where it fits (few tokens): weights are then all that is waited for in order.
-template <bool LDS, int TERMS> __global__ __launch_bounds__(64 * kWaves)
+// every one of which adds its jobs' columns to sums of its own for each token. An item's
+// weights and its terms of h, a row of h (a column) a load, are asked for NB items ahead and
+// in the order they are used in; the terms then go through LDS, the wavefront's own, to the
+// lanes that hold them for the products. Few columns a job: an expert of more tokens is read
+// again, mostly from the caches.
+template <int TERMS> __global__ __launch_bounds__(64 * kWaves, 2)
 void k_moe_down(MoeLayerArgs a, MoeWork w) {
-    constexpr int W = kWaves, NB = 4, TPT = 16 / TERMS;
+    constexpr int W = kWaves, NB = 4, C = kDownColumns, CAP = C / TERMS, PITCH = 1024 + 16;  // (16: no bank conflicts)
     __shared__ MoePlan plan;
-    extern __shared__ __align__(16) uint8_t smem[];  // sums [W][n_tok][16], h [pairs][TERMS][frow]
+    __shared__ uint16_t pairs[kMoeMaxPairs * CAP];
+    extern __shared__ __align__(16) uint8_t smem[];  // [W][C + 1][PITCH], sums [W][n_tok][16]
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int slots = a.k + a.n_shared, frow = pad128(a.n_ff), pairs = a.n_tok * slots;
-    float *const sums = reinterpret_cast<float *>(smem), *const own = sums + wv * a.n_tok * 16;
-    uint8_t *const hs = smem + (size_t)W * a.n_tok * 64;
-    // h, in chunks of 512 of a row, on its way while the plan is made
-    constexpr int kChunks = LDS ? (int)(kDownLds / 1024) / W : 1;
-    const int cpr = (frow + 511) / 512, chunks = pairs * TERMS * cpr;
-    uint4 held[kChunks];
-    if constexpr (LDS) {
-#pragma unroll
-        for (int i = 0; i < kChunks; i++) {
-            const int c = wv + W * i, hr = c / cpr, col = 512 * (c - hr * cpr) + 8 * lane;
-            held[i] = make_uint4(0, 0, 0, 0);
-            if (c < chunks && col < frow)
-                held[i] = *reinterpret_cast<const uint4 *>(w.h + (size_t)(hr / TERMS * 3 + hr % TERMS) * frow + col);
-        }
-    }
-    moe_plan<W>(a, w, plan, TPT, nullptr, 0);
-    if constexpr (LDS) {
-#pragma unroll
-        for (int i = 0; i < kChunks; i++) {
-            const int c = wv + W * i, hr = c / cpr, col = 512 * (c - hr * cpr) + 8 * lane;
-            if (c < chunks && col < frow) *reinterpret_cast<uint4 *>(hs + ((size_t)hr * frow + col) * 2) = held[i];
-        }
+    const int slots = a.k + a.n_shared, frow = pad128(a.n_ff);
+    uint8_t *const mine = smem + wv * (C + 1) * PITCH;
+    float *const sums = reinterpret_cast<float *>(smem + W * (C + 1) * PITCH), *const own = sums + wv * a.n_tok * 16;
+    *reinterpret_cast<uint4 *>(mine + C * PITCH + 16 * lane) = make_uint4(0, 0, 0, 0);  // a column of zeros
+    moe_plan<W>(a, w, plan, CAP, nullptr, 0);
+    for (int i = tid; i < plan.n_jobs * CAP; i += 64 * W) {
+        const int job = i / CAP, t = moe_token(plan.tokens[job], i - job * CAP);
+        pairs[i] = t >= 0 ? (uint16_t)(t * slots + moe_slot_of(a, plan, t, plan.job[job])) : 0xFFFFu;
     }
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
-    const __amdgpu_buffer_rsrc_t ht = make_rsrc(w.h, (uint32_t)pairs * 3u * (uint32_t)frow * 2u);
     const int total = plan.n_jobs * pieces;
     const int from = (int)((long long)total * wv / W), to = (int)((long long)total * (wv + 1) / W);
+    struct Item {
+        MoePiece<1> p;
+        uint4 h[C];
+    };
     for (int r0 = blockIdx.x * 16; r0 < a.n_embd; r0 += gridDim.x * 16) {
-        __syncthreads();  // (the last turn's sums are read)
+        __syncthreads();  // (pairs are there, the last turn's sums are read)
         for (int i = lane; i < a.n_tok * 16; i += 64) own[i] = 0.0f;
         const size_t row = (size_t)min(r0 + r, a.n_embd - 1);
-        MoePiece<1> p[NB];
-        MoeTerms x[2];
-        auto fetch = [&](MoePiece<1> &d, int c) __attribute__((always_inline)) {
-            if (c < to) {
-                const size_t e = plan.job[c / pieces];
-                const MoeRows rows[1] = {{a.down + (e * a.n_embd + row) * rb + 16 * q, a.down_s + (e * a.n_embd + row) * sb}};
-                moe_fetch<1>(d, rows, c % pieces, steps);
+        Item item[NB];
+        auto fetch = [&](Item &d, int c) __attribute__((always_inline)) {
+            if (c >= to) return;
+            const int job = c / pieces, i = c - job * pieces;
+            const size_t e = plan.job[job];
+            const MoeRows rows[1] = {{a.down + (e * a.n_embd + row) * rb + 16 * q, a.down_s + (e * a.n_embd + row) * sb}};
+            moe_fetch<1>(d.p, rows, i, steps);
+            const int col = 512 * i + 8 * lane;
+#pragma unroll
+            for (int n = 0; n < CAP; n++) {
+                const int pair = __builtin_amdgcn_readfirstlane((int)pairs[job * CAP + n]);
+                if (pair == 0xFFFF) break;
+#pragma unroll
+                for (int j = 0; j < TERMS; j++) {
+                    d.h[n * TERMS + j] = make_uint4(0, 0, 0, 0);
+                    if (col < frow)
+                        d.h[n * TERMS + j] = *reinterpret_cast<const uint4 *>(w.h + ((size_t)pair * 3 + j) * frow + col);
+                }
             }
         };
-        // this lane's column of a job: its token, and where its terms lie
-        int tok = -1, tok_next = -1, job = -1, job_next = -1;
-        uint32_t at = kMoeNone, at_next = kMoeNone;
-        auto column = [&](int j) __attribute__((always_inline)) {
-            if (j == job_next) return;
-            job_next = j;
-            tok_next = r < TPT * TERMS ? moe_token(plan.tokens[j], r / TERMS) : -1;
-            const int pair = tok_next >= 0 ? tok_next * slots + moe_slot_of(a, plan, tok_next, plan.job[j]) : 0;
-            at_next = tok_next >= 0 ? (uint32_t)((pair * (LDS ? TERMS : 3) + r % TERMS) * frow + 32 * q) * 2u : kMoeNone;
-        };
+        int job = -1, tok = -1, columns = 0;
+        const uint8_t *src = mine;
         mx_v4f acc[1] = {mx_v4f{0.0f, 0.0f, 0.0f, 0.0f}};
         // a token's terms stand in neighbouring lanes: to the first of them, and to its sums
         auto flush = [&]() __attribute__((always_inline)) {
@@ -733,36 +728,24 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
             if (tok >= 0 && r % TERMS == 0) *reinterpret_cast<mx_v4f *>(own + tok * 16 + 4 * q) += y;
             acc[0] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
         };
-        if (from < to) {
-            column(from / pieces);
-            if constexpr (!LDS) moe_terms(x[0], ht, at_next, from % pieces);
-        }
 #pragma unroll
-        for (int b = 0; b < NB; b++) fetch(p[b], from + b);
+        for (int b = 0; b < NB; b++) fetch(item[b], from + b);
         auto part = [&](auto b_c, int c) __attribute__((always_inline)) {
-            constexpr int b = decltype(b_c)::value;
+            Item &d = item[decltype(b_c)::value];
             if (c / pieces != job) {
                 if (job >= 0) flush();
-                column(c / pieces);
-                job = job_next;
-                tok = tok_next;
-                at = at_next;
+                job = c / pieces;
+                const int pair = r < C ? pairs[job * CAP + min(r / TERMS, CAP - 1)] : 0xFFFF;
+                tok = pair == 0xFFFF ? -1 : pair / slots;
+                columns = __popc(plan.tokens[job]) * TERMS;
+                src = mine + (tok >= 0 ? r : C) * PITCH + 64 * q;
             }
-            const int i = c % pieces;
-            if constexpr (LDS) {
-                const uint8_t *const src = hs + (at == kMoeNone ? 0u : at) + 1024 * i;
-                moe_multiply<1>(p[b], [&](int j, int m) {
-                    const mx_bf8 v = *reinterpret_cast<const mx_bf8 *>(src + 256 * j + 16 * m);
-                    return at == kMoeNone ? mx_bf8{} : v;
-                }, i, steps, blocks, acc);
-            } else {
-                if (c + 1 < to) {
-                    column((c + 1) / pieces);
-                    moe_terms(x[(b + 1) & 1], ht, at_next, (c + 1) % pieces);
-                }
-                moe_multiply<1>(p[b], [&](int j, int m) { return x[b & 1].v[j][m]; }, i, steps, blocks, acc);
-            }
-            fetch(p[b], c + NB);
+#pragma unroll
+            for (int n = 0; n < C; n++)
+                if (n < columns) *reinterpret_cast<uint4 *>(mine + n * PITCH + 16 * lane) = d.h[n];
+            moe_multiply<1>(d.p, [&](int j, int m) { return *reinterpret_cast<const mx_bf8 *>(src + 256 * j + 16 * m); },
+                            c - job * pieces, steps, blocks, acc);
+            fetch(d, c + NB);
         };
         for (int c = from; c < to; c += NB) {
             part(std::integral_constant<int, 0>{}, c);
@@ -847,19 +830,12 @@ template <int TERMS> hipError_t moe_up(const MoeLayerArgs &a, const MoeWork &w, 
     return moe_up_go<1, TERMS>(a, w, hterms, kw, s);
 }
 
-template <bool LDS, int TERMS> hipError_t moe_down_go(const MoeLayerArgs &a, const MoeWork &w, size_t lds, hipStream_t s) {
-    if (LDS) {
-        const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<LDS, TERMS>), kDownLds + kWaves * kMoeMaxTok * 64);
-        if (e != hipSuccess) return e;
-    }
-    k_moe_down<LDS, TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, lds, s>>>(a, w);
-    return hipGetLastError();
-}
 template <int TERMS> hipError_t moe_down(const MoeLayerArgs &a, const MoeWork &w, hipStream_t s) {
-    // (a row of h is copied in chunks of 1 KB)
-    const size_t sums = (size_t)kWaves * a.n_tok * 64, rows = (size_t)a.n_tok * (a.k + a.n_shared) * TERMS;
-    const size_t h = rows * pad128(a.n_ff) * 2, chunks = rows * ((pad128(a.n_ff) + 511) / 512) * 1024;
-    return chunks <= kDownLds ? moe_down_go<true, TERMS>(a, w, sums + h, s) : moe_down_go<false, TERMS>(a, w, sums, s);
+    constexpr size_t columns = (size_t)kWaves * (kDownColumns + 1) * 1040, sums = (size_t)kWaves * 64;
+    const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<TERMS>), columns + sums * kMoeMaxTok);
+    if (e != hipSuccess) return e;
+    k_moe_down<TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w);
+    return hipGetLastError();
 }
 
 }  // namespace
