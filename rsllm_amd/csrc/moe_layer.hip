@@ -18,6 +18,9 @@ namespace {
 
 constexpr int kInWaves = 16, kWaves = 8;
 constexpr int kBatch = 4;
+// Tokens (one a wavefront) and experts (keys in registers) up to which the up kernel's
+// workgroups make the choice for themselves.
+constexpr int kChooseTok = kWaves, kChooseExperts = 256;
 constexpr int kDownColumns = 6;  // of a job: two tokens of three terms, three of two
 constexpr int kMoeMaxExpert = 1024, kMoeMaxShared = 8, kMoeMaxSlots = 40;
 constexpr int kMoeMaxPairs = kMoeMaxTok * kMoeMaxSlots, kMoeMaxAll = kMoeMaxExpert + kMoeMaxShared;
@@ -357,13 +360,13 @@ __device__ __forceinline__ void moe_slot(const MoeLayerArgs &a, MoePlan &plan, i
 }
 // Token t's choice by this wavefront; ids and weights written if `write`, the plan filled if
 // there is one. keys: n_expert + n_group doubles of LDS.
+template <int R>
 __device__ __forceinline__ void moe_choose_token(const MoeLayerArgs &a, const MoeWork &w, int t, double *keys, bool write, MoePlan *plan) {
     const double *const l = w.logits + (size_t)t * a.n_expert, *const s = w.scores + (size_t)t * a.n_expert;
     const int lane = threadIdx.x & 63;
     int id;
     float weight;
-    if (a.n_expert <= 256) moe_choose<4>(a, l, s, keys, keys + a.n_expert, id, weight);
-    else moe_choose<0>(a, l, s, keys, keys + a.n_expert, id, weight);
+    moe_choose<R>(a, l, s, keys, keys + a.n_expert, id, weight);
     if (lane >= a.k) return;
     if (write) {
         a.ids[t * a.k + lane] = id;
@@ -390,7 +393,7 @@ template <int W> __device__ __forceinline__ void moe_plan(const MoeLayerArgs &a,
     __syncthreads();
     if (choose) {
         for (int t = wv < choose ? wv : a.n_tok; t < a.n_tok; t += choose)
-            moe_choose_token(a, w, t, keys + wv * (a.n_expert + a.n_group), blockIdx.x == 0, &plan);
+            moe_choose_token<kChooseExperts / 64>(a, w, t, keys + wv * (a.n_expert + a.n_group), blockIdx.x == 0, &plan);
     } else {
         for (int i = tid; i < a.n_tok * a.k; i += 64 * W) {
             const int t = i / a.k;
@@ -517,11 +520,11 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
 
 }  // namespace
 
-// A token's choice a wavefront, for more tokens than the up kernel's workgroups make it for
-// themselves.
-__global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs a, MoeWork w) {
+// A token's choice a wavefront, for more tokens or experts than the up kernel's workgroups make
+// it of for themselves.
+template <int R> __global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs a, MoeWork w) {
     extern __shared__ __align__(16) uint8_t smem[];
-    moe_choose_token(a, w, blockIdx.x, reinterpret_cast<double *>(smem), true, nullptr);
+    moe_choose_token<R>(a, w, blockIdx.x, reinterpret_cast<double *>(smem), true, nullptr);
 }
 
 // Gate and up products, and the weighted SwiGLU of their sums as bf16 terms. The pieces of K
@@ -579,29 +582,28 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     if (from < to) keep(from / per);
 #pragma unroll
     for (int b = 0; b < NB; b++) fetch(p[b], b);
-    // The turns from round b0 on, all wavefronts' sums of which are in LDS: a token of one of
-    // them for every 16 lanes (rows). (LDS alone is waited for, not the weights on their way.)
+    int held = 0;  // rounds whose sums are in LDS
+    // The last `held` rounds up to b0 + held: a token of one of them for every 16 lanes (rows).
+    // (LDS alone is waited for, not the weights on their way.)
     auto finish = [&](int b0) __attribute__((always_inline)) {
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        for (int task = wv * 4 + q; task < kBatch * groups * TPT; task += W * 4) {
+        for (int task = wv * 4 + q; task < held * groups * TPT; task += W * 4) {
             const int c0 = task % TPT, g0 = task / TPT % groups, b = task / TPT / groups;
             const int s0 = (int)blockIdx.x * groups + g0;
             const int turn = (int)((long long)turns * s0 / streams) + b0 + b;
-            if (b0 + b >= rounds || turn >= (int)((long long)turns * (s0 + 1) / streams)) continue;
+            if (turn >= (int)((long long)turns * (s0 + 1) / streams)) continue;
             const int job = turn / per, e = plan.job[job], r0 = turn % per * 16;
             const int t = moe_token(plan.tokens[job], c0);
             if (t < 0) continue;
             const int slot = moe_slot_of(a, plan, t, e);
             const float *const src = red + ((b * W + g0 * kw) * 2 * 64 + c0 * TERMS + 16 * (r >> 2)) * 4 + (r & 3);
             float g = 0.0f, v = 0.0f;
+#pragma unroll 2
+            for (int y = 0; y < kw; y++) {
 #pragma unroll
-            for (int y = 0; y < W; y++) {
-                if (y < kw) {
-#pragma unroll
-                    for (int j = 0; j < TERMS; j++) {
-                        g += src[(y * 2 * 64 + j) * 4];
-                        v += src[((y * 2 + 1) * 64 + j) * 4];
-                    }
+                for (int j = 0; j < TERMS; j++) {
+                    g += src[(y * 2 * 64 + j) * 4];
+                    v += src[((y * 2 + 1) * 64 + j) * 4];
                 }
             }
             if (a.clamp > 1e-6f) {
@@ -619,6 +621,7 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        held = 0;
     };
     mx_v4f acc[2];
     // one of the NB buffers' turn (or, of more pieces, part of one)
@@ -643,10 +646,10 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
         }
         fetch(p[b], m + NB);
         if (n == np - 1) {
-            mx_v4f *const sums = reinterpret_cast<mx_v4f *>(red) + round % kBatch * W * 128;
+            mx_v4f *const sums = reinterpret_cast<mx_v4f *>(red) + held * W * 128;
             sums[(wv * 2) * 64 + lane] = acc[0];
             sums[(wv * 2 + 1) * 64 + lane] = acc[1];
-            if (round % kBatch == kBatch - 1 || round == rounds - 1) finish(round / kBatch * kBatch);
+            held++;
         }
     };
     const int total = rounds * np;
@@ -656,6 +659,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
         if constexpr (NB == 3) {
             if (m + 2 < total) part(std::integral_constant<int, 2>{}, m + 2);
         }
+        const int end = min(total, m + NB);
+        if (held + (XP == 1 ? NB : 1) > kBatch || end == total) finish(end / np - held);
     }
 }
 
@@ -796,19 +801,16 @@ template <int KERNEL> hipError_t moe_allow_lds(const void *kernel, size_t bytes)
     return e;
 }
 
-// Tokens up to which the up kernel's workgroups make the choice for themselves: one a
-// wavefront.
-constexpr int kChooseTok = kWaves;
-
 template <int XP, int TERMS>
 hipError_t moe_up_go(const MoeLayerArgs &a, const MoeWork &w, int hterms, int kw, hipStream_t s) {
-    // sums, and no more than 48 KB for the choice's keys
+    // sums, or the choice's keys (32 KB at most)
     const size_t keys = (size_t)(a.n_expert + a.n_group) * 8;
     int choose = 0;
-    if (a.n_tok <= kChooseTok) {
-        choose = (int)std::min((size_t)kWaves, 48 * 1024 / keys);
+    if (a.n_tok <= kChooseTok && a.n_expert <= kChooseExperts) {
+        choose = kWaves;
     } else {
-        k_moe_choose<<<(unsigned)a.n_tok, 64, keys, s>>>(a, w);
+        if (a.n_expert <= kChooseExperts) k_moe_choose<kChooseExperts / 64><<<(unsigned)a.n_tok, 64, keys, s>>>(a, w);
+        else k_moe_choose<0><<<(unsigned)a.n_tok, 64, keys, s>>>(a, w);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
