@@ -664,14 +664,20 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     }
 }
 
-// The down products of 16 rows a turn over all jobs, (job, piece of K) over the wavefronts,
-// every one of which adds its jobs' columns to sums of its own for each token. An item's
+// The value of the N-th lane after this one, of the same 16.
+template <int N> __device__ __forceinline__ float moe_lane_after(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x100 + N, 0xf, 0xf, true));
+}
+
+// The down products of 16 rows a turn over all jobs: the pieces of K over kw of the
+// wavefronts, runs of jobs over the groups of so many, so that neighbours read a job's rows
+// in full at about one time. Every one adds its jobs' columns to sums of its own for each token. An item's
 // weights and its terms of h, a row of h (a column) a load, are asked for NB items ahead and
 // in the order they are used in; the terms then go through LDS, the wavefront's own, to the
 // lanes that hold them for the products. Few columns a job: an expert of more tokens is read
 // again, mostly from the caches.
 template <int TERMS> __global__ __launch_bounds__(64 * kWaves, 2)
-void k_moe_down(MoeLayerArgs a, MoeWork w) {
+void k_moe_down(MoeLayerArgs a, MoeWork w, int kw) {
     constexpr int W = kWaves, NB = 4, C = kDownColumns, CAP = C / TERMS, PITCH = 1024 + 16;  // (16: no bank conflicts)
     __shared__ MoePlan plan;
     __shared__ uint16_t pairs[kMoeMaxPairs * CAP];
@@ -689,8 +695,19 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
     }
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
-    const int total = plan.n_jobs * pieces;
-    const int from = (int)((long long)total * wv / W), to = (int)((long long)total * (wv + 1) / W);
+    const int k = wv % kw, group = wv / kw, groups = W / kw;  // this wavefront's pieces and jobs
+    const int from = plan.n_jobs * group / groups, to = k < pieces ? plan.n_jobs * (group + 1) / groups : from;
+    const int total = (to - from) * ((pieces - k + kw - 1) / kw);
+    struct At {
+        int job, i;
+    };
+    auto next = [&](At &at) __attribute__((always_inline)) {
+        at.i += kw;
+        if (at.i >= pieces) {
+            at.i = k;
+            at.job++;
+        }
+    };
     struct Item {
         MoePiece<1> p;
         uint4 h[C];
@@ -700,10 +717,12 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
         for (int i = lane; i < a.n_tok * 16; i += 64) own[i] = 0.0f;
         const size_t row = (size_t)min(r0 + r, a.n_embd - 1);
         Item item[NB];
-        auto fetch = [&](Item &d, int c) __attribute__((always_inline)) {
-            if (c >= to) return;
-            const int job = c / pieces, i = c - job * pieces;
-            const size_t e = plan.job[job];
+        At ahead = {from, k}, here = ahead;
+        auto fetch = [&](Item &d) __attribute__((always_inline)) {
+            const int job = ahead.job, i = ahead.i;
+            if (job >= to) return;
+            next(ahead);
+            const size_t e = (size_t)__builtin_amdgcn_readfirstlane((int)plan.job[job]);
             const MoeRows rows[1] = {{a.down + (e * a.n_embd + row) * rb + 16 * q, a.down_s + (e * a.n_embd + row) * sb}};
             moe_fetch<1>(d.p, rows, i, steps);
             const int col = 512 * i + 8 * lane;
@@ -719,7 +738,7 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
                 }
             }
         };
-        int job = -1, tok = -1, columns = 0;
+        int tok = -1, columns = 0;
         const uint8_t *src = mine;
         mx_v4f acc[1] = {mx_v4f{0.0f, 0.0f, 0.0f, 0.0f}};
         // a token's terms stand in neighbouring lanes: to the first of them, and to its sums
@@ -727,38 +746,38 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
             mx_v4f y = acc[0];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float v1 = __shfl_down(acc[0][i], 1, 64), v2 = __shfl_down(acc[0][i], 2, 64);
-                y[i] += TERMS == 3 ? v1 + v2 : v1;
+                y[i] += moe_lane_after<1>(acc[0][i]);
+                if (TERMS == 3) y[i] += moe_lane_after<2>(acc[0][i]);
             }
             if (tok >= 0 && r % TERMS == 0) *reinterpret_cast<mx_v4f *>(own + tok * 16 + 4 * q) += y;
             acc[0] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
         };
 #pragma unroll
-        for (int b = 0; b < NB; b++) fetch(item[b], from + b);
-        auto part = [&](auto b_c, int c) __attribute__((always_inline)) {
+        for (int b = 0; b < NB; b++) fetch(item[b]);
+        auto part = [&](auto b_c) __attribute__((always_inline)) {
             Item &d = item[decltype(b_c)::value];
-            if (c / pieces != job) {
-                if (job >= 0) flush();
-                job = c / pieces;
-                const int pair = r < C ? pairs[job * CAP + min(r / TERMS, CAP - 1)] : 0xFFFF;
+            const int i = here.i;
+            if (i == k) {
+                const int pair = r < C ? pairs[here.job * CAP + min(r / TERMS, CAP - 1)] : 0xFFFF;
                 tok = pair == 0xFFFF ? -1 : pair / slots;
-                columns = __popc(plan.tokens[job]) * TERMS;
+                columns = __builtin_amdgcn_readfirstlane(__popc(plan.tokens[here.job])) * TERMS;
                 src = mine + (tok >= 0 ? r : C) * PITCH + 64 * q;
             }
 #pragma unroll
             for (int n = 0; n < C; n++)
                 if (n < columns) *reinterpret_cast<uint4 *>(mine + n * PITCH + 16 * lane) = d.h[n];
             moe_multiply<1>(d.p, [&](int j, int m) { return *reinterpret_cast<const mx_bf8 *>(src + 256 * j + 16 * m); },
-                            c - job * pieces, steps, blocks, acc);
-            fetch(d, c + NB);
+                            i, steps, blocks, acc);
+            fetch(d);
+            next(here);
+            if (here.i == k) flush();
         };
-        for (int c = from; c < to; c += NB) {
-            part(std::integral_constant<int, 0>{}, c);
-            if (c + 1 < to) part(std::integral_constant<int, 1>{}, c + 1);
-            if (c + 2 < to) part(std::integral_constant<int, 2>{}, c + 2);
-            if (c + 3 < to) part(std::integral_constant<int, 3>{}, c + 3);
+        for (int c = 0; c < total; c += NB) {
+            part(std::integral_constant<int, 0>{});
+            if (c + 1 < total) part(std::integral_constant<int, 1>{});
+            if (c + 2 < total) part(std::integral_constant<int, 2>{});
+            if (c + 3 < total) part(std::integral_constant<int, 3>{});
         }
-        if (job >= 0) flush();
         __syncthreads();
         for (int i = tid; i < a.n_tok * 16; i += 64 * W) {
             const int t = i >> 4, o = r0 + (i & 15);
@@ -836,7 +855,10 @@ template <int TERMS> hipError_t moe_down(const MoeLayerArgs &a, const MoeWork &w
     constexpr size_t columns = (size_t)kWaves * (kDownColumns + 1) * 1040, sums = (size_t)kWaves * 64;
     const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<TERMS>), columns + sums * kMoeMaxTok);
     if (e != hipSuccess) return e;
-    k_moe_down<TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w);
+    const int pieces = (int)mx_scale_bytes(a.n_ff) / 16;
+    int kw = kWaves;  // (at most a fifth of the wavefronts without a piece)
+    while (5 * pieces < 4 * kw * ((pieces + kw - 1) / kw)) kw /= 2;
+    k_moe_down<TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w, kw);
     return hipGetLastError();
 }
 
