@@ -566,7 +566,8 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
  * once from f32) out_stride elements apart; bias: out_dim values or NULL. A NaN block
  * makes its token's, or its channel's, outputs NaN.
  * rsllm_hip_matmul_mxfp4_dev takes floats x and quantises them on the way: the same
- * result, bit for bit, as the quantiser and the prequant form.
+ * result, bit for bit, as the quantiser and the prequant form. An output must not
+ * overlap what its call reads.
  * `work`: rsllm_hip_mxfp4_work_bytes(n_tok, in_dim, out_dim) bytes of the caller's (0
  * for sizes that are refused), 256-byte aligned, used by this call alone until it has run:
  * calls that may overlap, and graphs that may replay at once, get one each.

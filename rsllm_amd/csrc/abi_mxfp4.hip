@@ -207,12 +207,10 @@ int rsllm_hip_matmul_mxfp4_dev(void *out, size_t out_len, size_t out_stride,
     if (parts.total && !work) return invalid("NULL pointer with a nonzero length");
     if (n_tok == 0) return ok_status();
     if (const int rc = make_device_current()) return rc;
-    uint8_t *const xc = work, *const xs = work + parts.codes;
-    HIP_TRY(launch_mx_quantize(x, x_stride, xc, xs, (int)n_tok, (int)in_dim, dtype_x, (hipStream_t)stream),
-            "quantize_mxfp4");
-    const MxArgs a{weights, wscales, xc, xs, bias_len ? bias : nullptr, out, out_stride,
+    const MxArgs a{weights, wscales, nullptr, nullptr, bias_len ? bias : nullptr, out, out_stride,
                    (int)n_tok, (int)out_dim, (int)in_dim, dtype_out};
-    HIP_TRY(launch_mx_matmul(a, (hipStream_t)stream), "matmul_mxfp4");
+    HIP_TRY(launch_mx_matmul_float(a, x, x_stride, dtype_x, work, work + parts.codes, (hipStream_t)stream),
+            "matmul_mxfp4");
     return ok_status();
 }
 

@@ -317,8 +317,14 @@ struct MxArgs {
     size_t out_stride;
     int n_tok, out_dim, in_dim;
     uint32_t dtype_out;
+    const void *xf;  // float tokens in place of the codes, for kernels that quantise them
+    size_t x_stride;
+    int x_vec;  // their rows are 16-byte aligned
 };
 hipError_t launch_mx_matmul(const MxArgs &a, hipStream_t s);
+// Of float tokens, dtype_x; codes and scales: room for theirs.
+hipError_t launch_mx_matmul_float(MxArgs a, const void *x, size_t x_stride, uint32_t dtype_x, uint8_t *codes,
+                                  uint8_t *scales, hipStream_t s);
 
 // moe_layer.hip: a mixture-of-experts layer with MXFP4 experts for up to kMoeMaxTok
 // tokens; `work` holds moe_layer_work_bytes.

@@ -766,8 +766,10 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int kw) {
 #pragma unroll
             for (int n = 0; n < C; n++)
                 if (n < columns) *reinterpret_cast<uint4 *>(mine + n * PITCH + 16 * lane) = d.h[n];
+            __builtin_amdgcn_wave_barrier();
             moe_multiply<1>(d.p, [&](int j, int m) { return *reinterpret_cast<const mx_bf8 *>(src + 256 * j + 16 * m); },
                             i, steps, blocks, acc);
+            __builtin_amdgcn_wave_barrier();
             fetch(d);
             next(here);
             if (here.i == k) flush();

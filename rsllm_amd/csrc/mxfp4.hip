@@ -32,6 +32,23 @@ __device__ __forceinline__ size_t mx_row_of(size_t n, int groups) {
     return n >> 32 ? n / (size_t)groups : (size_t)((uint32_t)n / (uint32_t)groups);
 }
 
+// Eight elements (four neighbouring lanes hold a block) as codes; s: the block's scale.
+__device__ __forceinline__ uint32_t mx_quantize8(const float (&v)[8], uint32_t &s) {
+    uint32_t big = 0;
+#pragma unroll
+    for (int k = 0; k < 8; k++) big = max(big, mx_abs_bits(v[k]));
+    s = mx_scale_of(mx_max4(big));
+    uint32_t c = 0;
+    if (s != 255u) {
+        const float unit = mx_unit(s);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], unit, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], unit, 1);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], unit, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], unit, 3);
+    }
+    return c;
+}
+
 }  // namespace
 
 // A lane's eight elements at a time, four lanes a block: `groups` of eight a row (its
@@ -50,18 +67,8 @@ __global__ __launch_bounds__(256) void k_mx_quantize(const void *__restrict__ x,
         const int g = (int)(n - row * (size_t)groups), i = 8 * g;
         float v[8];
         mx_load8<DT>(x, row * stride, i, in_dim, vec, v);
-        uint32_t big = 0;
-#pragma unroll
-        for (int k = 0; k < 8; k++) big = max(big, mx_abs_bits(v[k]));
-        const uint32_t s = mx_scale_of(mx_max4(big));
-        uint32_t c = 0;
-        if (s != 255u) {
-            const float unit = mx_unit(s);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], unit, 0);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], unit, 1);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], unit, 2);
-            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], unit, 3);
-        }
+        uint32_t s;
+        const uint32_t c = mx_quantize8(v, s);
         *reinterpret_cast<uint32_t *>(codes + row * rb + 4 * g) = c;
         uint8_t *const sr = scales + row * sb;
         if ((g & 3) == 0) sr[g >> 2] = (uint8_t)s;
@@ -137,9 +144,22 @@ struct MxPiece {
     mx_v4u c[4], s;
 };
 
-template <class G> __global__ __launch_bounds__(64 * G::WK) void k_mx_few(MxArgs a, int n_ct) {
+// DX: kMxCodes, or the type of float tokens (up to kMxFloatTok, a.xf), of which every
+// wavefront quantises its pieces for itself, through LDS, before it multiplies them: the same
+// codes, and one launch less. With one and two tokens that takes 4.5 and 4.8 us at 4096 x
+// 4096 f32 in place of 6.6 and 6.7, 10.0 and 10.8 in place of 12.6 and 12.9 at 14336 x 4096.
+// Every workgroup repeats it, though, and a wavefront waits for each piece's codes: with four
+// tokens (in a build of up to eight) 5.7 in place of 6.9 and 12.9 in place of 13.4, but 14.3
+// in place of 12.0 where rows are 14336 long, with eight 7.5 and 7.1, 16.5 and 13.8.
+constexpr uint32_t kMxCodes = ~0u;
+constexpr int kMxFloatTok = 2, kMxFloatPitch = 256 + 16;  // (16: the row's scales)
+
+template <class G, uint32_t DX> __global__ __launch_bounds__(64 * G::WK) void k_mx_few(MxArgs a, int n_ct) {
     constexpr int MF = G::MF, NF = G::NF, WK = G::WK;
-    __shared__ float red[WK * MF * NF * 256];
+    constexpr bool kFloat = DX != kMxCodes;
+    static_assert(!kFloat || NF == 1, "few tokens");
+    constexpr int kRed = WK * MF * NF * 1024, kTok = kFloat ? WK * kMxFloatTok * kMxFloatPitch : 0;
+    __shared__ __align__(16) uint8_t red[kRed > kTok ? kRed : kTok];
     const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int o0 = (blockIdx.x % n_ct) * G::BM, t0 = (blockIdx.x / n_ct) * G::BN;
@@ -172,21 +192,49 @@ template <class G> __global__ __launch_bounds__(64 * G::WK) void k_mx_few(MxArgs
 #pragma unroll
         for (int n = 0; n < NF; n++) acc[m][n] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};
     MxPiece pw[MF], px[NF];
+    float xf[kFloat ? kMxFloatTok : 1][8];
     auto fetch = [&](int i) __attribute__((always_inline)) {
         if (i < pieces) {
+            if constexpr (kFloat) {  // (first: loads return in order, and these come from near)
+#pragma unroll
+                for (int t = 0; t < kMxFloatTok; t++)
+                    if (t < a.n_tok) mx_load8<DX>(a.xf, (size_t)t * a.x_stride, 512 * i + 8 * lane, a.in_dim, a.x_vec, xf[t]);
+            }
 #pragma unroll
             for (int m = 0; m < MF; m++) load(pw[m], w[m], ws[m], i);
+            if constexpr (!kFloat) {
 #pragma unroll
-            for (int n = 0; n < NF; n++) load(px[n], x[n], xs[n], i);
+                for (int n = 0; n < NF; n++) load(px[n], x[n], xs[n], i);
+            }
         }
     };
+    uint8_t *const mine = red + wv * kMxFloatTok * kMxFloatPitch;  // this wavefront's tokens
     fetch(wv);
     for (int i = wv; i < pieces; i += WK) {
         MxPiece cw[MF], cx[NF];
 #pragma unroll
         for (int m = 0; m < MF; m++) cw[m] = pw[m];
+        if constexpr (kFloat) {
 #pragma unroll
-        for (int n = 0; n < NF; n++) cx[n] = px[n];
+            for (int t = 0; t < kMxFloatTok; t++) {
+                if (t < a.n_tok) {
+                    uint32_t s;
+                    const uint32_t c = mx_quantize8(xf[t], s);
+                    *reinterpret_cast<uint32_t *>(mine + t * kMxFloatPitch + 4 * lane) = c;
+                    if (lane % 4 == 0) mine[t * kMxFloatPitch + 256 + lane / 4] = (uint8_t)s;
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            // (columns behind the last token repeat one)
+            const uint8_t *const src = mine + (r < a.n_tok ? r : 0) * kMxFloatPitch;
+#pragma unroll
+            for (int j = 0; j < 4; j++) cx[0].c[j] = *reinterpret_cast<const mx_v4u *>(src + 64 * j + 16 * q);
+            cx[0].s = *reinterpret_cast<const mx_v4u *>(src + 256);
+            __builtin_amdgcn_wave_barrier();
+        } else {
+#pragma unroll
+            for (int n = 0; n < NF; n++) cx[n] = px[n];
+        }
         fetch(i + WK);
         // (scales behind a row's last block may be anything: there 1)
         const bool tail = 16 * i + 16 > blocks;
@@ -206,6 +254,7 @@ template <class G> __global__ __launch_bounds__(64 * G::WK) void k_mx_few(MxArgs
             }
         }
     }
+    if constexpr (kFloat) __syncthreads();
     mx_v4f *const part = reinterpret_cast<mx_v4f *>(red);
 #pragma unroll
     for (int m = 0; m < MF; m++)
@@ -224,7 +273,15 @@ template <class G> __global__ __launch_bounds__(64 * G::WK) void k_mx_few(MxArgs
 
 template <class G> hipError_t mx_few_go(const MxArgs &a, hipStream_t s) {
     const int n_ct = (a.out_dim + G::BM - 1) / G::BM, n_tt = (a.n_tok + G::BN - 1) / G::BN;
-    k_mx_few<G><<<(unsigned)n_ct * (unsigned)n_tt, 64 * G::WK, 0, s>>>(a, n_ct);
+    k_mx_few<G, kMxCodes><<<(unsigned)n_ct * (unsigned)n_tt, 64 * G::WK, 0, s>>>(a, n_ct);
+    return hipGetLastError();
+}
+// Of a.xf, dtype_x.
+template <class G> hipError_t mx_few_float_go(const MxArgs &a, uint32_t dtype_x, hipStream_t s) {
+    const unsigned n_ct = (unsigned)((a.out_dim + G::BM - 1) / G::BM), n = 64 * G::WK;
+    if (dtype_x == T_F32) k_mx_few<G, T_F32><<<n_ct, n, 0, s>>>(a, (int)n_ct);
+    else if (dtype_x == T_F16) k_mx_few<G, T_F16><<<n_ct, n, 0, s>>>(a, (int)n_ct);
+    else k_mx_few<G, T_BF16><<<n_ct, n, 0, s>>>(a, (int)n_ct);
     return hipGetLastError();
 }
 
@@ -399,6 +456,9 @@ template <class G> hipError_t mx_big_go(const MxArgs &a, hipStream_t s) {
 
 namespace {
 
+bool mx_rows_vec(const void *p, size_t stride, uint32_t dtype) {
+    return (uintptr_t)p % 16 == 0 && stride * (dtype == T_F32 ? 4 : 2) % 16 == 0;
+}
 // Workgroups of 256 for `total` threads' work, in turns behind 2^20 of them.
 unsigned mx_grid(size_t total) { return (unsigned)std::min<size_t>((total + 255) / 256, (size_t)1 << 20); }
 
@@ -409,7 +469,7 @@ hipError_t launch_mx_quantize(const void *x, size_t stride, uint8_t *codes, uint
     if (n_rows <= 0) return hipSuccess;
     const int groups = (int)mx_row_bytes(in_dim) / 4;
     const size_t total = (size_t)n_rows * groups;
-    const int vec = (uintptr_t)x % 16 == 0 && stride * (dtype == T_F32 ? 4 : 2) % 16 == 0;
+    const int vec = mx_rows_vec(x, stride, dtype);
     const unsigned g = mx_grid(total);
     if (dtype == T_F32) k_mx_quantize<T_F32><<<g, 256, 0, s>>>(x, stride, codes, scales, total, groups, in_dim, vec);
     else if (dtype == T_F16) k_mx_quantize<T_F16><<<g, 256, 0, s>>>(x, stride, codes, scales, total, groups, in_dim, vec);
@@ -422,7 +482,7 @@ hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, voi
     if (n_rows <= 0) return hipSuccess;
     const int groups = (in_dim + 7) / 8;
     const size_t total = (size_t)n_rows * groups;
-    const int vec = (uintptr_t)out % 16 == 0 && stride * (dtype == T_F32 ? 4 : 2) % 16 == 0;
+    const int vec = mx_rows_vec(out, stride, dtype);
     const unsigned g = mx_grid(total);
     if (dtype == T_F32) k_mx_dequantize<T_F32><<<g, 256, 0, s>>>(codes, scales, out, stride, total, groups, in_dim, vec);
     else if (dtype == T_F16) k_mx_dequantize<T_F16><<<g, 256, 0, s>>>(codes, scales, out, stride, total, groups, in_dim, vec);
@@ -441,6 +501,7 @@ namespace {
 // every 16 or 32 channels, are up to three times slower and not looked at.
 struct MxKernel {
     hipError_t (*go)(const MxArgs &, hipStream_t);
+    hipError_t (*go_float)(const MxArgs &, uint32_t, hipStream_t);  // or null
     int bm, bn, wk, unit, occ, max_tok, threads;
     float c0, c1, c2, c3;
     bool fits(const MxArgs &a) const {  // a launch holds less than 2^32 threads
@@ -456,11 +517,13 @@ struct MxKernel {
 };
 template <int MF, int NF, int WK> constexpr MxKernel mx_few(int occ, float c0, float c1, float c2, float c3) {
     using G = MxFew<MF, NF, WK>;
-    return {&mx_few_go<G>, G::BM, G::BN, WK, 512, occ, 128, 64 * WK, c0, c1, c2, c3};
+    hipError_t (*go_float)(const MxArgs &, uint32_t, hipStream_t) = nullptr;
+    if constexpr (NF == 1) go_float = &mx_few_float_go<G>;
+    return {&mx_few_go<G>, go_float, G::BM, G::BN, WK, 512, occ, 128, 64 * WK, c0, c1, c2, c3};
 }
 template <int WM, int WN, int MF, int NF, int ST> constexpr MxKernel mx_big(int occ, float c0, float c1, float c2) {
     using G = MxBig<WM, WN, MF, NF, ST>;
-    return {&mx_big_go<G>, G::BM, G::BN, 1, 256, occ, INT_MAX, G::kThreads, c0, c1, c2, 0.0f};
+    return {&mx_big_go<G>, nullptr, G::BM, G::BN, 1, 256, occ, INT_MAX, G::kThreads, c0, c1, c2, 0.0f};
 }
 const MxKernel kMxKernels[] = {
     mx_few<1, 1, 8>(2, 4.57f, 0.0f, 0.434f, 0.328f),  // 16 channels x 16 tokens
@@ -474,13 +537,10 @@ const MxKernel kMxKernels[] = {
     mx_big<2, 4, 4, 2, 3>(1, 0.0f, 5.10f, 0.768f),    // 128 x 128
     mx_big<4, 2, 3, 4, 2>(1, 0.54f, 4.50f, 1.153f),   // 192 x 128
     mx_big<2, 4, 8, 2, 2>(1, 2.66f, 4.56f, 1.351f),   // 256 x 128
-    {&mx_wide_224, 224, 256, 1, 256, 1, INT_MAX, 256, 0.0f, 10.26f, 1.216f, 0.0f},
+    {&mx_wide_224, nullptr, 224, 256, 1, 256, 1, INT_MAX, 256, 0.0f, 10.26f, 1.216f, 0.0f},
 };
 
-}  // namespace
-
-hipError_t launch_mx_matmul(const MxArgs &a, hipStream_t s) {
-    if (a.n_tok <= 0) return hipSuccess;
+const MxKernel *mx_choose(const MxArgs &a) {
     const MxKernel *best = nullptr;
     float us = 0.0f;
     for (const MxKernel &k : kMxKernels) {
@@ -491,7 +551,32 @@ hipError_t launch_mx_matmul(const MxArgs &a, hipStream_t s) {
             us = t;
         }
     }
-    return best ? best->go(a, s) : hipErrorInvalidValue;
+    return best;
+}
+
+}  // namespace
+
+hipError_t launch_mx_matmul(const MxArgs &a, hipStream_t s) {
+    if (a.n_tok <= 0) return hipSuccess;
+    const MxKernel *const k = mx_choose(a);
+    return k ? k->go(a, s) : hipErrorInvalidValue;
+}
+
+hipError_t launch_mx_matmul_float(MxArgs a, const void *x, size_t x_stride, uint32_t dtype_x, uint8_t *codes,
+                                  uint8_t *scales, hipStream_t s) {
+    if (a.n_tok <= 0) return hipSuccess;
+    const MxKernel *const k = mx_choose(a);
+    if (!k) return hipErrorInvalidValue;
+    if (k->go_float && a.n_tok <= kMxFloatTok) {
+        a.xf = x;
+        a.x_stride = x_stride;
+        a.x_vec = mx_rows_vec(x, x_stride, dtype_x);
+        return k->go_float(a, dtype_x, s);
+    }
+    a.x = codes;
+    a.xs = scales;
+    const hipError_t e = launch_mx_quantize(x, x_stride, codes, scales, a.n_tok, a.in_dim, dtype_x, s);
+    return e == hipSuccess ? k->go(a, s) : e;
 }
 
 }  // namespace rsllm_hip
