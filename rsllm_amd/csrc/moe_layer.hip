@@ -29,8 +29,9 @@ size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 __host__ __device__ constexpr int pad128(int n) { return (n + 127) / 128 * 128; }
 
 // What the tokens chose, in LDS: every token's slots (the k chosen experts, then the shared
-// ones; -1: none, or of weight 0), and the jobs: an expert, in rising order, and the tokens
-// that take it, a bit each, as many jobs as it takes with at most `cap` tokens.
+// ones; -1: none, or of weight 0), and the jobs: an expert and the tokens that take it, a bit
+// each, as many jobs as it takes with at most `cap` tokens, experts in rising order (one
+// token's in the order of its slots).
 struct MoePlan {
     int n_jobs;
     uint32_t tokens[kMoeMaxPairs];
@@ -358,21 +359,18 @@ __device__ __forceinline__ void moe_slot(const MoeLayerArgs &a, MoePlan &plan, i
     plan.weight[t * (a.k + a.n_shared) + i] = weight;
     if (on) atomicOr(&plan.takes[id], 1u << t);
 }
-// Token t's choice by this wavefront; ids and weights written if `write`, the plan filled if
-// there is one. keys: n_expert + n_group doubles of LDS.
+// Token t's choice by this wavefront, slot r's at lane r (-1 and 0 behind the k-th); ids and
+// weights written if `write`. keys: n_expert + n_group doubles of LDS.
 template <int R>
-__device__ __forceinline__ void moe_choose_token(const MoeLayerArgs &a, const MoeWork &w, int t, double *keys, bool write, MoePlan *plan) {
+__device__ __forceinline__ void moe_choose_token(const MoeLayerArgs &a, const MoeWork &w, int t, double *keys, bool write,
+                                                 int &id, float &weight) {
     const double *const l = w.logits + (size_t)t * a.n_expert, *const s = w.scores + (size_t)t * a.n_expert;
     const int lane = threadIdx.x & 63;
-    int id;
-    float weight;
     moe_choose<R>(a, l, s, keys, keys + a.n_expert, id, weight);
-    if (lane >= a.k) return;
-    if (write) {
+    if (write && lane < a.k) {
         a.ids[t * a.k + lane] = id;
         a.weights[t * a.k + lane] = weight;
     }
-    if (plan) moe_slot(a, *plan, t, lane, id, weight);
 }
 
 // The workgroup's plan, jobs of at most cap tokens. `choose`: the first `choose` wavefronts
@@ -383,22 +381,56 @@ template <int W> __device__ __forceinline__ void moe_plan(const MoeLayerArgs &a,
     __shared__ int part[W];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, slots = a.k + a.n_shared;
     const int all = a.n_expert + a.n_shared;
-    for (int e = tid; e < all; e += 64 * W)
-        plan.takes[e] = e < a.n_expert ? 0u : a.n_tok == 32 ? 0xFFFFFFFFu : (1u << a.n_tok) - 1u;
-    for (int i = tid; i < a.n_tok * a.n_shared; i += 64 * W) {
-        const int t = i / a.n_shared, j = i - t * a.n_shared;
-        plan.expert[t * slots + a.k + j] = (int16_t)(a.n_expert + j);
-        plan.weight[t * slots + a.k + j] = 1.0f;
+    const bool one = a.n_tok == 1;  // whose slots are its jobs, as they come
+    if (!one) {
+        for (int e = tid; e < all; e += 64 * W)
+            plan.takes[e] = e < a.n_expert ? 0u : a.n_tok == 32 ? 0xFFFFFFFFu : (1u << a.n_tok) - 1u;
+        for (int i = tid; i < a.n_tok * a.n_shared; i += 64 * W) {
+            const int t = i / a.n_shared, j = i - t * a.n_shared;
+            plan.expert[t * slots + a.k + j] = (int16_t)(a.n_expert + j);
+            plan.weight[t * slots + a.k + j] = 1.0f;
+        }
+        __syncthreads();
     }
-    __syncthreads();
+    int id = -1;
+    float weight = 0.0f;
     if (choose) {
-        for (int t = wv < choose ? wv : a.n_tok; t < a.n_tok; t += choose)
-            moe_choose_token<kChooseExperts / 64>(a, w, t, keys + wv * (a.n_expert + a.n_group), blockIdx.x == 0, &plan);
+        for (int t = wv < choose ? wv : a.n_tok; t < a.n_tok; t += choose) {
+            moe_choose_token<kChooseExperts / 64>(a, w, t, keys + wv * (a.n_expert + a.n_group), blockIdx.x == 0, id, weight);
+            if (!one && lane < a.k) moe_slot(a, plan, t, lane, id, weight);
+        }
+    } else if (one) {
+        if (tid < a.k) {
+            id = a.ids[tid];
+            weight = a.weights[tid];
+        }
     } else {
         for (int i = tid; i < a.n_tok * a.k; i += 64 * W) {
             const int t = i / a.k;
             moe_slot(a, plan, t, i - t * a.k, a.ids[i], a.weights[i]);
         }
+    }
+    if (one) {
+        if (wv == 0) {
+            if (lane >= a.k) {
+                id = lane < slots ? a.n_expert + lane - a.k : -1;
+                weight = 1.0f;
+            }
+            const bool on = id >= 0 && weight != 0.0f;
+            const unsigned long long mask = __ballot(on);
+            if (lane < slots) {
+                plan.expert[lane] = (int16_t)(on ? id : -1);
+                plan.weight[lane] = weight;
+            }
+            if (on) {
+                const int at = __popcll(mask & ((1ull << lane) - 1));
+                plan.job[at] = (uint16_t)id;
+                plan.tokens[at] = 1u;
+            }
+            if (lane == 0) plan.n_jobs = __popcll(mask);
+        }
+        __syncthreads();
+        return;
     }
     __syncthreads();
     // the jobs of a run of experts a thread, behind those of the threads before it
@@ -524,7 +556,9 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
 // it of for themselves.
 template <int R> __global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs a, MoeWork w) {
     extern __shared__ __align__(16) uint8_t smem[];
-    moe_choose_token<R>(a, w, blockIdx.x, reinterpret_cast<double *>(smem), true, nullptr);
+    int id;
+    float weight;
+    moe_choose_token<R>(a, w, blockIdx.x, reinterpret_cast<double *>(smem), true, id, weight);
 }
 
 // Gate and up products, and the weighted SwiGLU of their sums as bf16 terms. The pieces of K
