@@ -497,7 +497,7 @@ namespace {
 // with L workgroups a CU, r of them one after the other (`occ` run at once) and `slices`
 // pieces of `unit` codes a wavefront, fitted to 150 sizes (1 to 2048 tokens, weights from
 // memory). Slower than the fastest of sixteen kernels: 3% on average and 29% at most at
-// those sizes. From 129 tokens on the tiles without LDS, which read the tokens' codes for
+// those sizes (64 x 64's constants by nine of them, later). From 129 tokens on the tiles without LDS, which read the tokens' codes for
 // every 16 or 32 channels, are up to three times slower and not looked at.
 struct MxKernel {
     hipError_t (*go)(const MxArgs &, hipStream_t);
@@ -521,9 +521,9 @@ template <int MF, int NF, int WK> constexpr MxKernel mx_few(int occ, float c0, f
     if constexpr (NF == 1) go_float = &mx_few_float_go<G>;
     return {&mx_few_go<G>, go_float, G::BM, G::BN, WK, 512, occ, 128, 64 * WK, c0, c1, c2, c3};
 }
-template <int WM, int WN, int MF, int NF, int ST> constexpr MxKernel mx_big(int occ, float c0, float c1, float c2) {
+template <int WM, int WN, int MF, int NF, int ST> constexpr MxKernel mx_big(int occ, float c0, float c1, float c2, float c3 = 0.0f) {
     using G = MxBig<WM, WN, MF, NF, ST>;
-    return {&mx_big_go<G>, nullptr, G::BM, G::BN, 1, 256, occ, INT_MAX, G::kThreads, c0, c1, c2, 0.0f};
+    return {&mx_big_go<G>, nullptr, G::BM, G::BN, 1, 256, occ, INT_MAX, G::kThreads, c0, c1, c2, c3};
 }
 const MxKernel kMxKernels[] = {
     mx_few<1, 1, 8>(2, 4.57f, 0.0f, 0.434f, 0.328f),  // 16 channels x 16 tokens
@@ -532,7 +532,7 @@ const MxKernel kMxKernels[] = {
     mx_few<2, 2, 8>(1, 3.66f, 0.0f, 1.834f, 0.0f),    // 32 x 32
     mx_few<2, 2, 4>(2, 4.03f, 0.0f, 1.105f, 0.066f),
     mx_few<2, 4, 4>(1, 3.34f, 0.23f, 1.938f, 0.0f),   // 32 x 64
-    mx_big<4, 2, 1, 2, 4>(2, 1.43f, 3.01f, 0.409f),   // 64 x 64
+    mx_big<2, 2, 2, 2, 4>(2, 2.5f, 2.0f, 0.22f, 0.18f),  // 64 x 64 (eight wavefronts of 16 x 32: 10 to 25% slower)
     mx_big<2, 4, 2, 2, 4>(1, 0.39f, 4.36f, 0.499f),   // 64 x 128
     mx_big<2, 4, 4, 2, 3>(1, 0.0f, 5.10f, 0.768f),    // 128 x 128
     mx_big<4, 2, 3, 4, 2>(1, 0.54f, 4.50f, 1.153f),   // 192 x 128
