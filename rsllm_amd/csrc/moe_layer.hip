@@ -5,11 +5,20 @@
 // scale none), x and h are sums of bf16 terms: one for bf16 x, two for f16, three for
 // f32 (8 significant bits each, so 24), so that the products on the matrix cores are
 // exact and the sums f32. A term of a token is a column of the 16-wide products.
+//
+// The chosen experts' weights are read once and bound everything: 98 MB for one token of a
+// 4096-wide layer with n_ff 2048, 6 of 256 experts and a shared one, 1.83 GB for 32 (137
+// experts). Three launches (four beyond 8 tokens): 42.9 us and 420 us, of which the up kernel
+// is 26.6 and 233 (63 MB and 1.2 GB: 2.4 and 5.2 TB/s), the down kernel 13.9 and 151 (31 and
+// 610 MB: 2.3 and 4.0 TB/s), the router 4.9 and 18. A launch that only reads gets 4.3 TB/s of
+// 31 MB and 5.7 of 400. One token's up kernel is a chain before the stream, which takes 12 us
+// of it: the choice 4 us, its jobs 1, the first loads; and behind it 3 us for the last sums.
 #include "fp4_common.h"
 #include "route_scores.h"
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 namespace rsllm_hip {
@@ -17,11 +26,16 @@ namespace rsllm_hip {
 namespace {
 
 constexpr int kInWaves = 16, kWaves = 8;
-constexpr int kBatch = 4;
+constexpr int kBatch = 4;  // turns of the up kernel finished at once
 // Tokens (one a wavefront) and experts (keys in registers) up to which the up kernel's
-// workgroups make the choice for themselves.
+// workgroups make the choice for themselves, in place of a launch: 47.0 against 48.7 us for
+// one token of a 4096-wide layer of 256 experts, 168.0 against 169.7 for eight. From nine on
+// a wavefront has two tokens to choose for: 284 against 283 us for 16.
 constexpr int kChooseTok = kWaves, kChooseExperts = 256;
-constexpr int kDownColumns = 6;  // of a job: two tokens of three terms, three of two
+// Columns of a job of the down kernel: two tokens of three terms, three of two. With three
+// (one token of either) an expert's rows are read for each: 465 against 433 us for 32 tokens
+// of the layer above; more would not fit the registers of four items.
+constexpr int kDownColumns = 6;
 constexpr int kMoeMaxExpert = 1024, kMoeMaxShared = 8, kMoeMaxSlots = 40;
 constexpr int kMoeMaxPairs = kMoeMaxTok * kMoeMaxSlots, kMoeMaxAll = kMoeMaxExpert + kMoeMaxShared;
 
@@ -125,7 +139,9 @@ __device__ __forceinline__ void moe_logits(const MoeLayerArgs &a, int e, int t0,
 }  // namespace
 
 // Workgroup e < n_expert: the 64-bit logits (and scores) of expert e for every token, groups
-// of up to 8 tokens and parts of K over the wavefronts; the others: a token's x as bf16
+// of up to 8 tokens and parts of K over the wavefronts (4096-wide, 256 experts: 4.9 us for one
+// token, which is the latency of one chain; 18 for 32, whose rows every workgroup reads again,
+// 134 MB from L2, and widens to 64 bits); the others: a token's x as bf16
 // terms, zeros behind it, and whether it is finite.
 template <uint32_t DX, uint32_t DR>
 __global__ __launch_bounds__(64 * kInWaves) void k_moe_in(MoeLayerArgs a, MoeWork w, int vx, int vr) {
@@ -553,7 +569,8 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
 }  // namespace
 
 // A token's choice a wavefront, for more tokens or experts than the up kernel's workgroups make
-// it of for themselves.
+// it of for themselves. 6.8 us for 32 tokens of 256 experts: one chain of loads, 64-bit scores
+// and k reductions over the lanes.
 template <int R> __global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs a, MoeWork w) {
     extern __shared__ __align__(16) uint8_t smem[];
     int id;
@@ -565,8 +582,10 @@ template <int R> __global__ __launch_bounds__(64) void k_moe_choose(MoeLayerArgs
 // go over `kw` of the wavefronts, XP each, whose terms a wavefront keeps while it goes through
 // a run of (job, 16 rows): its loads are the weights' alone, NB turns ahead. (Loads return in
 // order: terms fetched for every turn would wait for weights asked for before them.) With
-// XP = 0 there are more pieces than that, and their terms come with every turn. The
-// wavefronts' sums meet in LDS, where kBatch turns are finished at once.
+// XP = 0 there are more pieces than that, and their terms come with every turn: at sizes that
+// XP = 1 holds (32 tokens of 4096, f32) that takes the layer from 433 to 589 us, where XP = 2
+// does (8 of 7168, bf16) from 244 to 269. The wavefronts' sums meet in LDS, where kBatch turns
+// are finished at once (one by one the layer took 506 in place of 464 us, two barriers a turn).
 template <int XP, int TERMS> __global__ __launch_bounds__(64 * kWaves)
 void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     constexpr int W = kWaves, NB = XP == 1 ? 3 : 2, TPT = 16 / TERMS, NX = XP > 0 ? XP : 1;
@@ -704,14 +723,18 @@ template <int N> __device__ __forceinline__ float moe_lane_after(float v) {
 }
 
 // The down products of 16 rows a turn over all jobs: the pieces of K over kw of the
-// wavefronts, runs of jobs over the groups of so many, so that neighbours read a job's rows
-// in full at about one time. Every one adds its jobs' columns to sums of its own for each token. An item's
-// weights and its terms of h, a row of h (a column) a load, are asked for NB items ahead and
-// in the order they are used in; the terms then go through LDS, the wavefront's own, to the
-// lanes that hold them for the products. Few columns a job: an expert of more tokens is read
-// again, mostly from the caches.
+// wavefronts, runs of jobs over the groups of so many; which split is a rule on the numbers
+// of both (32 tokens of 64 experts with n_ff 1300, three pieces: 214 us for the layer with the
+// jobs alone split, 294 with eight wavefronts a job). Every wavefront adds its jobs' columns
+// to sums of its own for each token. An item's weights and its terms of h, a row of h (a
+// column) a load, are asked for NB items ahead and in the order they are used in; the terms
+// then go through LDS, the wavefront's own, to the lanes that hold them for the products. Few
+// columns a job: an expert of more tokens is read again, mostly from the caches. With 32
+// tokens (151 us, 4.0 TB/s of weights) h comes to as many bytes from L2 as the weights, and
+// a workgroup a CU keeps its vector units busy a third of the time; the rest are waits.
 template <int TERMS> __global__ __launch_bounds__(64 * kWaves, 2)
-void k_moe_down(MoeLayerArgs a, MoeWork w, int kw) {
+void k_moe_down(MoeLayerArgs a, MoeWork w) {
+    static_assert(kWaves == 8, "the split");
     constexpr int W = kWaves, NB = 4, C = kDownColumns, CAP = C / TERMS, PITCH = 1024 + 16;  // (16: no bank conflicts)
     __shared__ MoePlan plan;
     __shared__ uint16_t pairs[kMoeMaxPairs * CAP];
@@ -729,8 +752,17 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int kw) {
     }
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
-    const int k = wv % kw, group = wv / kw, groups = W / kw;  // this wavefront's pieces and jobs
-    const int from = plan.n_jobs * group / groups, to = k < pieces ? plan.n_jobs * (group + 1) / groups : from;
+    // this wavefront's pieces and jobs: the split whose longest share is the shortest
+    const int n_jobs = __builtin_amdgcn_readfirstlane(plan.n_jobs);
+    int kw = 1, least = INT_MAX;
+#pragma unroll
+    for (int b = 3; b >= 0; b--) {
+        const int share = ((n_jobs + (W >> b) - 1) >> (3 - b)) * ((pieces + (1 << b) - 1) >> b);
+        kw = share < least ? 1 << b : kw;
+        least = min(share, least);
+    }
+    const int k = wv % kw, group = wv / kw, groups = W / kw;
+    const int from = n_jobs * group / groups, to = k < pieces ? n_jobs * (group + 1) / groups : from;
     const int total = (to - from) * ((pieces - k + kw - 1) / kw);
     struct At {
         int job, i;
@@ -891,10 +923,7 @@ template <int TERMS> hipError_t moe_down(const MoeLayerArgs &a, const MoeWork &w
     constexpr size_t columns = (size_t)kWaves * (kDownColumns + 1) * 1040, sums = (size_t)kWaves * 64;
     const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<TERMS>), columns + sums * kMoeMaxTok);
     if (e != hipSuccess) return e;
-    const int pieces = (int)mx_scale_bytes(a.n_ff) / 16;
-    int kw = kWaves;  // (at most a fifth of the wavefronts without a piece)
-    while (5 * pieces < 4 * kw * ((pieces + kw - 1) / kw)) kw /= 2;
-    k_moe_down<TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w, kw);
+    k_moe_down<TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w);
     return hipGetLastError();
 }
 
