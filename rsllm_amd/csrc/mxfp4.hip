@@ -56,7 +56,7 @@ __device__ __forceinline__ uint32_t mx_quantize8(const float (&v)[8], uint32_t &
 // and one instruction then divides two elements by the block's power of two, rounds them
 // to nearest even and saturates. One read and one write of everything, so the bytes bound
 // it: 14336 x 4096 bf16 (149 MB in and out) 32.8 us, 4.5 TB/s, a large copy's rate. One
-// row of 4096 f32: 2.1 us, a launch.
+// row of 4096 f32: 1.8 us, a launch.
 template <uint32_t DT>
 __global__ __launch_bounds__(256) void k_mx_quantize(const void *__restrict__ x, size_t stride,
                                                      uint8_t *__restrict__ codes, uint8_t *__restrict__ scales,
@@ -85,8 +85,9 @@ __device__ __forceinline__ float mx_unit_f32(uint32_t s) {
 // A lane's eight elements at a time, decoded by the conversion instruction and multiplied
 // by the block's power of two in f32, which rounds only what is below 2^-126 and
 // overflows only above f32's range, as the definition does. vec: rows of out are 16-byte
-// aligned. The bytes bound it: 14336 x 4096 to bf16 (149 MB) 23 us, 6.5 TB/s out of the
-// caches' reach of what was written; an element a lane, a table and ldexp took 86 us.
+// aligned. The bytes bound it: 14336 x 4096 to bf16 (149 MB) 24 us where the codes were
+// written just before and come from a cache, 117 MB of writes at 4.9 TB/s; an element a lane,
+// a table and ldexp took 86 us. One row of 4096 f32: 1.9 us, a launch.
 template <uint32_t DT>
 __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict__ codes,
                                                        const uint8_t *__restrict__ scales, void *__restrict__ out,
@@ -136,7 +137,12 @@ namespace {
 // A workgroup's tile: 16 MF channels x 16 NF tokens; its WK wavefronts take every WK-th
 // piece of 512 codes, and their sums are added through LDS. A lane reads 16 codes' bytes
 // of a row for each step of 128 and the 16 scale bytes of its row for the piece's four
-// steps; the operands of the next piece are on their way while this one is multiplied.
+// steps; the operands of the next piece are on their way while this one is multiplied. The
+// weights' bytes bound it, for small ones the latency of a launch, one piece a wavefront and
+// the sums' join: 14336 x 4096, one token, 31 MB, 8.8 us from memory (a launch that only
+// reads them 7.5); 4096 x 4096, 32 tokens, 6.5; 1001 x 2000, 77 tokens, 4.6. K is split over
+// the wavefronts since few channels a workgroup fill the chip (4096 channels: 256 or 128
+// workgroups), and since a lane that streams rows into registers needs no LDS and no barrier.
 template <int MF_, int NF_, int WK_> struct MxFew {
     static constexpr int MF = MF_, NF = NF_, WK = WK_, BM = 16 * MF, BN = 16 * NF;
 };
@@ -293,7 +299,10 @@ template <class G> hipError_t mx_few_float_go(const MxArgs &a, uint32_t dtype_x,
 // slice's next half are read into registers while the matrix cores work on this one. One
 // barrier a slice, in its middle: behind it the next slice has landed, and every
 // wavefront holds what is left of this one in registers, so the slice ST further on can be
-// copied over it.
+// copied over it. 300 tokens of 4096 to 2048 channels: 11.4 us with 64 x 64 (160 workgroups;
+// half a us a slice, most of it waits: deeper rings of 6 and 8 slices were no faster);
+// 1000 of 4100 to 5000: 26 with 192 x 128 (1.6 PFLOP/s), 2048 of 2048 to 2048: 12.2 with
+// 128 x 128 (1.4 PFLOP/s).
 template <int WM_, int WN_, int MF_, int NF_, int ST_> struct MxBig {
     static constexpr int WM = WM_, WN = WN_, MF = MF_, NF = NF_, ST = ST_, NW = WM * WN;
     static constexpr int BM = 16 * MF * WM, BN = 16 * NF * WN, kThreads = 64 * NW;
@@ -497,8 +506,10 @@ namespace {
 // with L workgroups a CU, r of them one after the other (`occ` run at once) and `slices`
 // pieces of `unit` codes a wavefront, fitted to 150 sizes (1 to 2048 tokens, weights from
 // memory). Slower than the fastest of sixteen kernels: 3% on average and 29% at most at
-// those sizes (64 x 64's constants by nine of them, later). From 129 tokens on the tiles without LDS, which read the tokens' codes for
-// every 16 or 32 channels, are up to three times slower and not looked at.
+// those sizes (64 x 64's constants by nine of them, later). From 129
+// tokens on the tiles without LDS, which read the tokens' codes for every 16 or 32 channels,
+// lose and are not looked at: 14.6 us at best in place of 10.5 for 129 tokens of 4096 x 4096,
+// 58 in place of 19 for 200 of 14336 x 4096.
 struct MxKernel {
     hipError_t (*go)(const MxArgs &, hipStream_t);
     hipError_t (*go_float)(const MxArgs &, uint32_t, hipStream_t);  // or null

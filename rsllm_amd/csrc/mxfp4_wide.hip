@@ -21,6 +21,10 @@ namespace {
 // most some three instructions. Wavefronts 0 and 1 copy channels, 2 and 3 tokens, each
 // from one buffer; the scales, 16 bytes a row for two slices, come as two more copies a
 // slice of wavefronts 0 (the channels') and 1.
+// 2048 tokens, 14336 x 4096, bf16 out: 75 us, 3.2 PFLOP/s, in two rounds of 256 workgroups. Of
+// a tile's some 32 us 3 pass before the first product, 23 in the loop (70% of the matrix
+// cores' rate at the 1.7 GHz that they get under this load) and 5 with the stores, in which
+// nothing multiplies. k_mx_big's widest tiles (128 x 128, 256 x 128) take 128 us here.
 template <int MF_, int NF_> struct MxWide {
     static constexpr int MF = MF_, NF = NF_, BM = 32 * MF, BN = 32 * NF;
     static constexpr int D = 2 * MF;  // a wavefront's copies of 8 rows x 128 bytes a slice
