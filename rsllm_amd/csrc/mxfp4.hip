@@ -506,10 +506,10 @@ namespace {
 // with L workgroups a CU, r of them one after the other (`occ` run at once) and `slices`
 // pieces of `unit` codes a wavefront, fitted to 150 sizes (1 to 2048 tokens, weights from
 // memory). Slower than the fastest of sixteen kernels: 3% on average and 29% at most at
-// those sizes (64 x 64's constants by nine of them, later). From 129
-// tokens on the tiles without LDS, which read the tokens' codes for every 16 or 32 channels,
-// lose and are not looked at: 14.6 us at best in place of 10.5 for 129 tokens of 4096 x 4096,
-// 58 in place of 19 for 200 of 14336 x 4096.
+// those sizes (64 x 64's constants by nine of them, later). From 129 tokens on the tiles
+// without LDS, which read the tokens' codes for every 16 or 32 channels, lose and are not
+// looked at: 14.6 us at best in place of 10.5 for 129 tokens of 4096 x 4096, 58 in place of
+// 19 for 200 of 14336 x 4096.
 struct MxKernel {
     hipError_t (*go)(const MxArgs &, hipStream_t);
     hipError_t (*go_float)(const MxArgs &, uint32_t, hipStream_t);  // or null
