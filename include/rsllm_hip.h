@@ -625,8 +625,10 @@ int rsllm_hip_matmul_mxfp4_dev(void *out, size_t out_len, size_t out_stride,
  * out: n_tok rows of n_embd values of dtype_out (F32, F16 or BF16), overwritten,
  * out_stride elements apart; x: rows of dtype_x likewise; ids, weights [n_tok x k] are
  * written. out must not overlap x. `work`: rsllm_hip_moe_mxfp4_work_bytes(layer, n_tok)
- * bytes of the caller's (0 for a layer or n_tok that is refused), 256-byte aligned, used
- * by this call alone until it has run; what it holds before does not matter. The struct
+ * bytes of the caller's (0 for a NULL layer and for sizes or an n_tok outside the ranges
+ * below), 256-byte aligned, used by this call alone until it has run: calls that may
+ * overlap, and graphs that may replay at once, get one each. What it holds before does not
+ * matter. The struct
  * is read during the call only; what it points to until the work is done.
  * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for n_tok above 32, n_embd
  * or n_ff 0 or above 65536, n_expert 0 or above 1024, n_shared above 8, k 0 or above
