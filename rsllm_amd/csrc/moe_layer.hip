@@ -8,9 +8,9 @@
 //
 // The chosen experts' weights are read once and bound everything: 98 MB for one token of a
 // 4096-wide layer with n_ff 2048, 6 of 256 experts and a shared one, 1.83 GB for 32 (137
-// experts). Three launches (four beyond 8 tokens): 42.9 us and 420 us, of which the up kernel
-// is 26.6 and 233 (63 MB and 1.2 GB: 2.4 and 5.2 TB/s), the down kernel 13.9 and 151 (31 and
-// 610 MB: 2.3 and 4.0 TB/s), the router 4.9 and 18. A launch that only reads gets 4.3 TB/s of
+// experts). Three launches (four beyond 8 tokens): 43.0 us and 406 us, of which the up kernel
+// is 26.0 and 234 (63 MB and 1.2 GB: 2.4 and 5.2 TB/s), the down kernel 13.4 and 145 (31 and
+// 610 MB: 2.3 and 4.2 TB/s), the router 4.9 and 18. A launch that only reads gets 4.3 TB/s of
 // 31 MB and 5.7 of 400. One token's up kernel is a chain before the stream, which takes 12 us
 // of it: the choice 4 us, its jobs 1, the first loads; and behind it 3 us for the last sums.
 #include "fp4_common.h"
@@ -32,10 +32,11 @@ constexpr int kBatch = 4;  // turns of the up kernel finished at once
 // one token of a 4096-wide layer of 256 experts, 168.0 against 169.7 for eight. From nine on
 // a wavefront has two tokens to choose for: 284 against 283 us for 16.
 constexpr int kChooseTok = kWaves, kChooseExperts = 256;
-// Columns of a job of the down kernel: two tokens of three terms, three of two. With three
-// (one token of either) an expert's rows are read for each: 465 against 433 us for 32 tokens
-// of the layer above; more would not fit the registers of four items.
-constexpr int kDownColumns = 6;
+// Columns of a job of the down kernel: three tokens of three terms, four of two. An expert's
+// rows are read again for more: with three columns 465 us for 32 tokens of the layer above,
+// with six 431, with nine 422, with twelve 421 (and 169.3 and 170.0 with the last two for
+// eight tokens).
+constexpr int kDownColumns = 9;
 constexpr int kMoeMaxExpert = 1024, kMoeMaxShared = 8, kMoeMaxSlots = 40;
 constexpr int kMoeMaxPairs = kMoeMaxTok * kMoeMaxSlots, kMoeMaxAll = kMoeMaxExpert + kMoeMaxShared;
 
@@ -727,15 +728,15 @@ template <int N> __device__ __forceinline__ float moe_lane_after(float v) {
 // of both (32 tokens of 64 experts with n_ff 1300, three pieces: 214 us for the layer with the
 // jobs alone split, 294 with eight wavefronts a job). Every wavefront adds its jobs' columns
 // to sums of its own for each token. An item's weights and its terms of h, a row of h (a
-// column) a load, are asked for NB items ahead and in the order they are used in; the terms
-// then go through LDS, the wavefront's own, to the lanes that hold them for the products. Few
-// columns a job: an expert of more tokens is read again, mostly from the caches. With 32
-// tokens (151 us, 4.0 TB/s of weights) h comes to as many bytes from L2 as the weights, and
-// a workgroup a CU keeps its vector units busy a third of the time; the rest are waits.
+// column) a load, are asked for NB items ahead (three and four were no faster) and in the
+// order they are used in; the terms then go through LDS, the wavefront's own, to the lanes
+// that hold them for the products. With 32 tokens (145 us, 4.2 TB/s of weights) h comes to
+// as many bytes from L2 as the weights, and a workgroup a CU keeps its vector units busy a
+// third of the time; the rest are waits.
 template <int TERMS> __global__ __launch_bounds__(64 * kWaves, 2)
 void k_moe_down(MoeLayerArgs a, MoeWork w) {
     static_assert(kWaves == 8, "the split");
-    constexpr int W = kWaves, NB = 4, C = kDownColumns, CAP = C / TERMS, PITCH = 1024 + 16;  // (16: no bank conflicts)
+    constexpr int W = kWaves, NB = 2, CAP = kDownColumns / TERMS, C = CAP * TERMS, PITCH = 1024 + 16;  // (16: no bank conflicts)
     __shared__ MoePlan plan;
     __shared__ uint16_t pairs[kMoeMaxPairs * CAP];
     extern __shared__ __align__(16) uint8_t smem[];  // [W][C + 1][PITCH], sums [W][n_tok][16]
@@ -843,8 +844,6 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
         for (int c = 0; c < total; c += NB) {
             part(std::integral_constant<int, 0>{});
             if (c + 1 < total) part(std::integral_constant<int, 1>{});
-            if (c + 2 < total) part(std::integral_constant<int, 2>{});
-            if (c + 3 < total) part(std::integral_constant<int, 3>{});
         }
         __syncthreads();
         for (int i = tid; i < a.n_tok * 16; i += 64 * W) {
