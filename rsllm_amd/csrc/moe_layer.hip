@@ -63,7 +63,19 @@ struct MoeWork {
     __bf16 *x;       // [n_tok][3][pad128(n_embd)]
     __bf16 *h;       // [n_tok * (k + n_shared)][3][pad128(n_ff)], weighted
     int *bad;        // [n_tok]: x is not finite
+    float *part;     // [parts][n_tok][n_embd]: the down kernel's sums, if more than one
 };
+// Parts of the jobs that workgroups of the down kernel take for each 16 rows: one, unless so
+// few rows leave half of the chip idle and a wavefront would still have four items of
+// each part (if every token chose experts of its own). The sums then take a launch more, 4
+// to 5 us: in all 23 in place of 90 us for 22 tokens of a 408-wide layer with n_ff 2687 (8 of
+// 32 experts, 9 parts), 24 in place of 28 for 8 tokens of 2048 / 1024 (8 of 128, 2 parts). Below
+// that a launch costs what it saves: 4 tokens of 1536 / 768 (6 of 64) take 13 undivided.
+int moe_down_parts(int n_tok, int n_embd, int n_ff, int slots) {
+    const long long tiles = (n_embd + 15) / 16, pieces = (long long)mx_scale_bytes(n_ff) / 16;
+    const long long most = std::min(256 / std::min(tiles, 256ll), 16ll);
+    return (int)std::max(1ll, std::min(most, n_tok * slots * pieces / (4 * kWaves)));
+}
 size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_shared, uint8_t *base, MoeWork *w) {
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -76,8 +88,10 @@ size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_sha
     uint8_t *const x = take((size_t)n_tok * 3 * pad128(n_embd) * 2);
     uint8_t *const h = take((size_t)n_tok * (k + n_shared) * 3 * pad128(n_ff) * 2);
     uint8_t *const bad = take((size_t)n_tok * 4);
+    const int parts = moe_down_parts(n_tok, n_embd, n_ff, k + n_shared);
+    uint8_t *const part = take(parts > 1 ? (size_t)parts * n_tok * n_embd * 4 : 0);
     if (w) *w = {reinterpret_cast<double *>(logits), reinterpret_cast<double *>(scores), reinterpret_cast<__bf16 *>(x),
-                 reinterpret_cast<__bf16 *>(h), reinterpret_cast<int *>(bad)};
+                 reinterpret_cast<__bf16 *>(h), reinterpret_cast<int *>(bad), reinterpret_cast<float *>(part)};
     return at;
 }
 
@@ -734,7 +748,7 @@ template <int N> __device__ __forceinline__ float moe_lane_after(float v) {
 // as many bytes from L2 as the weights, and a workgroup a CU keeps its vector units busy a
 // third of the time; the rest are waits.
 template <int TERMS> __global__ __launch_bounds__(64 * kWaves, 2)
-void k_moe_down(MoeLayerArgs a, MoeWork w) {
+void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
     static_assert(kWaves == 8, "the split");
     constexpr int W = kWaves, NB = 2, CAP = kDownColumns / TERMS, C = CAP * TERMS, PITCH = 1024 + 16;  // (16: no bank conflicts)
     __shared__ MoePlan plan;
@@ -753,8 +767,10 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
     }
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
-    // this wavefront's pieces and jobs: the split whose longest share is the shortest
-    const int n_jobs = __builtin_amdgcn_readfirstlane(plan.n_jobs);
+    // this workgroup's jobs, of which this wavefront's, and its pieces: the split whose longest
+    // share is the shortest
+    const int tiles = (int)gridDim.x / parts, me = (int)blockIdx.x / tiles;
+    const int all = __builtin_amdgcn_readfirstlane(plan.n_jobs), first = all * me / parts, n_jobs = all * (me + 1) / parts - first;
     int kw = 1, least = INT_MAX;
 #pragma unroll
     for (int b = 3; b >= 0; b--) {
@@ -763,7 +779,7 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
         least = min(share, least);
     }
     const int k = wv % kw, group = wv / kw, groups = W / kw;
-    const int from = n_jobs * group / groups, to = k < pieces ? n_jobs * (group + 1) / groups : from;
+    const int from = first + n_jobs * group / groups, to = k < pieces ? first + n_jobs * (group + 1) / groups : from;
     const int total = (to - from) * ((pieces - k + kw - 1) / kw);
     struct At {
         int job, i;
@@ -779,7 +795,7 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
         MoePiece<1> p;
         uint4 h[C];
     };
-    for (int r0 = blockIdx.x * 16; r0 < a.n_embd; r0 += gridDim.x * 16) {
+    for (int r0 = ((int)blockIdx.x - me * tiles) * 16; r0 < a.n_embd; r0 += tiles * 16) {
         __syncthreads();  // (pairs are there, the last turn's sums are read)
         for (int i = lane; i < a.n_tok * 16; i += 64) own[i] = 0.0f;
         const size_t row = (size_t)min(r0 + r, a.n_embd - 1);
@@ -851,9 +867,20 @@ void k_moe_down(MoeLayerArgs a, MoeWork w) {
             float y = 0.0f;
 #pragma unroll
             for (int v = 0; v < W; v++) y += sums[v * a.n_tok * 16 + i];
-            if (o < a.n_embd) mx_store(a.out, (size_t)t * a.out_stride + o, w.bad[t] ? __builtin_nanf("") : y, a.dtype_out);
+            if (o >= a.n_embd) continue;
+            if (parts > 1) w.part[((size_t)me * a.n_tok + t) * a.n_embd + o] = y;
+            else mx_store(a.out, (size_t)t * a.out_stride + o, w.bad[t] ? __builtin_nanf("") : y, a.dtype_out);
         }
     }
+}
+
+// The sum of the down kernel's parts, in their order: one chain of loads, 4 to 5 us.
+__global__ __launch_bounds__(256) void k_moe_sum(MoeLayerArgs a, MoeWork w, int parts) {
+    const int t = blockIdx.y, o = blockIdx.x * 256 + threadIdx.x;
+    if (o >= a.n_embd) return;
+    float y = 0.0f;
+    for (int i = 0; i < parts; i++) y += w.part[((size_t)i * a.n_tok + t) * a.n_embd + o];
+    mx_store(a.out, (size_t)t * a.out_stride + o, w.bad[t] ? __builtin_nanf("") : y, a.dtype_out);
 }
 
 size_t moe_layer_work_bytes(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_shared) {
@@ -922,7 +949,11 @@ template <int TERMS> hipError_t moe_down(const MoeLayerArgs &a, const MoeWork &w
     constexpr size_t columns = (size_t)kWaves * (kDownColumns + 1) * 1040, sums = (size_t)kWaves * 64;
     const hipError_t e = moe_allow_lds<TERMS>(reinterpret_cast<const void *>(&k_moe_down<TERMS>), columns + sums * kMoeMaxTok);
     if (e != hipSuccess) return e;
-    k_moe_down<TERMS><<<(unsigned)std::min((a.n_embd + 15) / 16, 512), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w);
+    const int tiles = std::min((a.n_embd + 15) / 16, 512), parts = moe_down_parts(a.n_tok, a.n_embd, a.n_ff, a.k + a.n_shared);
+    k_moe_down<TERMS><<<(unsigned)(tiles * parts), 64 * kWaves, columns + sums * a.n_tok, s>>>(a, w, parts);
+    const hipError_t d = hipGetLastError();
+    if (d != hipSuccess || parts == 1) return d;
+    k_moe_sum<<<dim3((unsigned)(a.n_embd + 255) / 256, (unsigned)a.n_tok), 256, 0, s>>>(a, w, parts);
     return hipGetLastError();
 }
 

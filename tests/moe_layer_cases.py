@@ -23,3 +23,10 @@ CASES = [
     # more rows than workgroups take at once
     ((0, 1, 2, None), dict(t=1, embd=8320, ff=16, kx="bf16", ky="bf16", experts=2, k=1)),
 ]
+#: Layers whose down products are summed in parts, up to sixteen: some of them empty, some of
+#: one row, tokens that are not finite among them.
+PART_CASES = [
+    dict(t=32, embd=16, ff=520, experts=8, k=8), dict(t=22, embd=408, ff=1100, experts=8, k=4, kx="bf16", y_gap=3, shared=1),
+    dict(t=32, embd=1, ff=600, experts=2, k=2, ky="f16"), dict(t=9, embd=100, ff=2600, experts=5, k=3, kx="f16", ky="bf16"),
+    dict(t=32, embd=40, ff=1030, experts=1, k=1, shared=3), dict(t=17, embd=2047, ff=64, experts=16, k=16, ky="bf16", y_gap=1),
+]

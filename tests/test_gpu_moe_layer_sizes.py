@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from moe_layer_cases import CASES
+from moe_layer_cases import CASES, PART_CASES
 from test_gpu_moe_layer import Layer
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +76,28 @@ def test_a_token_alone_and_among_others(hip):
         assert torch.equal(one.ids[0], ids[t]) and torch.equal(one.weights[0], weights[t])
         # (both are within tol of the same value)
         assert (np.abs((one.out[0] - out[t]).cpu().double().numpy()) <= 2 * tol[t]).all()
+
+
+@pytest.mark.parametrize("case", PART_CASES, ids=lambda c: "-".join(str(c[n]) for n in ("t", "embd", "ff", "experts", "k")))
+def test_down_products_in_parts(hip, case):
+    """Eager, then captured and replayed: the same bits, a token that is not finite among them."""
+    p = Layer(hip, **case)
+    p.x[2, 0] = np.nan
+    p.xt = torch.from_numpy(p.x).to(p.xt.dtype)
+    p.upload()
+    room = torch.full((p.work.numel() + 512,), 0xCD, dtype=torch.uint8, device="cuda")
+    p.work = room[:-512]
+    p.run()
+    p.check()
+    assert (room[-512:] == 0xCD).all()
+    want = p.out.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        p.run()
+    for _ in range(3):
+        p.out.fill_(77.0)
+        p.work.random_(0, 256)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(torch.nan_to_num(p.out), torch.nan_to_num(want))

@@ -100,3 +100,15 @@ for device in (0, 1, 0, 1):
 """).split()
     n = str(sum(new for new, _ in cases))
     assert out == [n, n, "0", "0"]
+
+
+def test_few_rows_and_many_jobs_are_summed_in_parts(tmp_path):
+    """Fewer rows than half of the chip takes, with enough for a wavefront to do: parts of the
+    down products and a launch that adds them; their workspace counts."""
+    sizes = [(32, 64, 2050, True), (22, 408, 2687, True), (32, 2048, 1024, True), (1, 64, 2050, False),
+             (3, 408, 128, False), (32, 2064, 1024, False), (32, 4096, 2048, False)]
+    out = hip_recorder.run(tmp_path, CALL + f"""
+for t, embd, ff, _ in {sizes!r}:
+    print(go(t, embd, ff, experts=32, k=8).count("k_moe_sum"))
+""").split()
+    assert out == [str(int(parts)) for *_, parts in sizes]
