@@ -580,6 +580,14 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
     for (int i = 0; i < n; i++) mask &= mask - 1;
     return mask ? __ffs((int)mask) - 1 : -1;
 }
+// The pairs (token, slot) of every job, CAP a job, 0xFFFF behind its last token.
+template <int W, int CAP> __device__ __forceinline__ void moe_pairs(const MoeLayerArgs &a, const MoePlan &plan, uint16_t *pairs) {
+    const int slots = a.k + a.n_shared;
+    for (int i = threadIdx.x; i < plan.n_jobs * CAP; i += 64 * W) {
+        const int job = i / CAP, t = moe_token(plan.tokens[job], i - job * CAP);
+        pairs[i] = t >= 0 ? (uint16_t)(t * slots + moe_slot_of(a, plan, t, plan.job[job])) : 0xFFFFu;
+    }
+}
 
 }  // namespace
 
@@ -606,6 +614,7 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     constexpr int W = kWaves, NB = XP == 1 ? 3 : 2, TPT = 16 / TERMS, NX = XP > 0 ? XP : 1;
     extern __shared__ __align__(16) uint8_t smem[];  // keys of the choice, then sums [kBatch][W][2][64][4]
     __shared__ MoePlan plan;
+    __shared__ uint16_t pairs[kMoeMaxPairs * TPT];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slots = a.k + a.n_shared, ff = a.n_ff, frow = pad128(ff), erow = pad128(a.n_embd);
@@ -650,6 +659,7 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     if (from < to) keep(from / per);
 #pragma unroll
     for (int b = 0; b < NB; b++) fetch(p[b], b);
+    moe_pairs<W, TPT>(a, plan, pairs);  // (for finish(), behind its barrier)
     int held = 0;  // rounds whose sums are in LDS
     // The last `held` rounds up to b0 + held: a token of one of them for every 16 lanes (rows).
     // (LDS alone is waited for, not the weights on their way.)
@@ -660,10 +670,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
             const int s0 = (int)blockIdx.x * groups + g0;
             const int turn = (int)((long long)turns * s0 / streams) + b0 + b;
             if (turn >= (int)((long long)turns * (s0 + 1) / streams)) continue;
-            const int job = turn / per, e = plan.job[job], r0 = turn % per * 16;
-            const int t = moe_token(plan.tokens[job], c0);
-            if (t < 0) continue;
-            const int slot = moe_slot_of(a, plan, t, e);
+            const int job = turn / per, r0 = turn % per * 16, pair = pairs[job * TPT + c0];
+            if (pair == 0xFFFF) continue;
             const float *const src = red + ((b * W + g0 * kw) * 2 * 64 + c0 * TERMS + 16 * (r >> 2)) * 4 + (r & 3);
             float g = 0.0f, v = 0.0f;
 #pragma unroll 2
@@ -678,8 +686,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
                 g = g > a.clamp ? a.clamp : g;
                 v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
             }
-            float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[t * slots + slot] : 0.0f;
-            __bf16 *const dst = w.h + (size_t)(t * slots + slot) * 3 * frow + r0 + r;
+            float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[pair] : 0.0f;
+            __bf16 *const dst = w.h + (size_t)pair * 3 * frow + r0 + r;
             for (int j = 0; j < hterms; j++) {
                 const __bf16 b16 = (__bf16)h;
                 dst[j * frow] = b16;
@@ -761,10 +769,7 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
     float *const sums = reinterpret_cast<float *>(smem + W * (C + 1) * PITCH), *const own = sums + wv * a.n_tok * 16;
     *reinterpret_cast<uint4 *>(mine + C * PITCH + 16 * lane) = make_uint4(0, 0, 0, 0);  // a column of zeros
     moe_plan<W>(a, w, plan, CAP, nullptr, 0);
-    for (int i = tid; i < plan.n_jobs * CAP; i += 64 * W) {
-        const int job = i / CAP, t = moe_token(plan.tokens[job], i - job * CAP);
-        pairs[i] = t >= 0 ? (uint16_t)(t * slots + moe_slot_of(a, plan, t, plan.job[job])) : 0xFFFFu;
-    }
+    moe_pairs<W, CAP>(a, plan, pairs);
     const size_t rb = mx_row_bytes(a.n_ff), sb = mx_scale_bytes(a.n_ff);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_ff + 31) / 32;
     // this workgroup's jobs, of which this wavefront's, and its pieces: the split whose longest
