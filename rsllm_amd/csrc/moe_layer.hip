@@ -8,7 +8,7 @@
 //
 // The chosen experts' weights are read once and bound everything: 98 MB for one token of a
 // 4096-wide layer with n_ff 2048, 6 of 256 experts and a shared one, 1.83 GB for 32 (137
-// experts). Three launches (four beyond 8 tokens): 43.0 us and 406 us, of which the up kernel
+// experts). Three launches (four beyond 8 tokens): 41.8 us and 408 us, of which the up kernel
 // is 26.0 and 234 (63 MB and 1.2 GB: 2.4 and 5.2 TB/s), the down kernel 13.4 and 145 (31 and
 // 610 MB: 2.3 and 4.2 TB/s), the router 4.9 and 18. A launch that only reads gets 4.3 TB/s of
 // 31 MB and 5.7 of 400. One token's up kernel is a chain before the stream, which takes 12 us
