@@ -96,6 +96,11 @@ size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_sha
 }
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
+// The first eight significant bits of v, cut off and not rounded: rounded, what lies above
+// bf16's largest number would be an infinity.
+__device__ __forceinline__ __bf16 moe_cut(float v) {
+    return __builtin_bit_cast(__bf16, (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16));
+}
 
 // f64 counterparts of the routing's scores.
 __device__ __forceinline__ double route_exp(double l, double m) { return l == m ? 1.0 : route_exp64(l - m); }
@@ -191,7 +196,7 @@ __global__ __launch_bounds__(64 * kInWaves) void k_moe_in(MoeLayerArgs a, MoeWor
             mx_bf8 b;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                b[k] = (__bf16)v[k];
+                b[k] = moe_cut(v[k]);
                 v[k] -= (float)b[k];
             }
             *reinterpret_cast<mx_bf8 *>(dst + j * row + i) = b;

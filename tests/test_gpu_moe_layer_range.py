@@ -1,0 +1,93 @@
+"""The 4-bit mixture-of-experts layer at the ends of its types' ranges, against its definition
+in 64 bits."""
+import numpy as np
+import pytest
+
+import mxfp4_ref as M
+import serving_ref as R
+from test_gpu_moe_layer import Layer
+
+pytestmark = pytest.mark.gpu
+
+FLT_MAX = float(np.finfo(np.float32).max)
+#: what rounds to bf16's infinity from here on
+NO_BF16 = 255.5 * 2.0 ** 120
+
+
+def moe(p):
+    """M.moe with a closer bound where a clamp holds a sum (its error is then nothing) and where
+    silu has vanished: (ids, weights, out, how far out may be off)."""
+    c = p.c
+    p.want()
+    gate, up, down = p.wide
+    with np.errstate(all="ignore"):
+        logits = np.stack([(row * p.router).sum(1) for row in p.x])
+    bias = None if p.bias is None else p.bias.astype(np.float64)
+    ids, weights = R.route(logits, bias, c["k"], c["groups"], c["top_groups"], c["group_top"], c["score"], c["renorm"],
+                           c["scale"])
+    y, err = np.zeros(p.x.shape), np.zeros(p.x.shape)
+    d, f, top = c["embd"], c["ff"], c["clamp"] if c["clamp"] > 1e-6 else np.inf
+    cut = 2.0 ** -24 if c["ky"] == "f32" else 2.0 ** -16
+    for t, x in enumerate(p.x):
+        slots = [(e, w) for e, w in zip(ids[t], weights[t]) if e >= 0 and np.float32(w) != 0]
+        slots += [(c["experts"] + j, 1.0) for j in range(c["shared"])]
+        total = np.zeros(d)
+        for e, w in slots:
+            g, u = gate[e] @ x, up[e] @ x
+            step = (d / 32 + 40) * 2.0 ** -23
+            eg, eu = step * (np.abs(gate[e]) @ np.abs(x)), step * (np.abs(up[e]) @ np.abs(x))
+            es = np.where((g - eg >= top) | (g + eg <= -200.0), 1e-80, 1.1 * eg)
+            eu = np.where(np.abs(u) - eu >= top, 0.0, eu)
+            g, u = np.minimum(g, top), np.clip(u, -top, top)
+            with np.errstate(over="ignore"):
+                s = g / (1.0 + np.exp(-g))
+            h = s * u
+            eh = es * (np.abs(u) + eu) + np.abs(s) * eu + np.abs(h) * (2.0 ** -20 + cut)
+            y[t] += w * (down[e] @ h)
+            err[t] += w * (np.abs(down[e]) @ eh)
+            total += w * (np.abs(down[e]) @ np.abs(h))
+        err[t] += (len(slots) * f / 32 + 40) * 2.0 ** -23 * total
+    return ids, weights, y, err + M.rounding(y, c["ky"])
+
+
+def check(p):
+    p.run()
+    want_ids, want_w, want, tol = moe(p)
+    got = p.out[:, :p.c["embd"]].cpu().double().numpy()
+    assert np.array_equal(p.ids.cpu().numpy(), want_ids)
+    got_w = p.weights.cpu().double().numpy()
+    assert (np.abs(got_w - want_w) <= np.abs(want_w) * (2.0 ** -24 + 2.0 ** -45) + 2.0 ** -150).all()
+    assert np.isfinite(want).all() and np.isfinite(tol).all()
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[:5], got[bad][:5], want[bad][:5], tol[bad][:5])
+
+
+def scales(p, name, low, high, seed=1):
+    rng = np.random.default_rng(seed)
+    s = p.m[name][1]
+    blocks = ((p.c["ff"] if name == "down" else p.c["embd"]) + 31) // 32
+    s[:, :blocks] = rng.integers(low, high + 1, (len(s), blocks))
+
+
+def tokens(p, x):
+    p.xt, p.x = R.as_type(x, p.c["kx"])
+
+
+#: f32 numbers that round to bf16's infinity, and the largest one that does not
+TOP = [FLT_MAX, -FLT_MAX, NO_BF16, -NO_BF16, float(np.nextafter(np.float32(NO_BF16), np.float32(0)))]
+
+
+@pytest.mark.parametrize("t,embd,ff", [(5, 256, 128), (5, 130, 64), (1, 4096, 96), (5, 4200, 40), (5, 8300, 33)])
+@pytest.mark.parametrize("ky", ["f32", "bf16"])
+def test_largest_x(hip, t, embd, ff, ky):
+    """A finite x gives a finite row where the clamp holds what it makes of the sums: every
+    weight is less than 1, so that the sums are finite in f32, too."""
+    p = Layer(hip, t=t, embd=embd, ff=ff, clamp=7.0, shared=1, ky=ky, score=2)
+    for name in ("gate", "up"):
+        scales(p, name, 118, 124)
+    x = p.x.copy()
+    for i in range(t):
+        x[i, [3, embd - 1][i % 2]] = TOP[i]
+    tokens(p, x)
+    p.upload()
+    check(p)
