@@ -95,6 +95,7 @@ size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_sha
     return at;
 }
 
+constexpr float kFltMax = 0x1.fffffep127f;
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 // The first eight significant bits of v, cut off and not rounded: rounded, what lies above
 // bf16's largest number would be an infinity.
@@ -691,6 +692,7 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
                 g = g > a.clamp ? a.clamp : g;
                 v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
             }
+            g = g < -kFltMax ? -kFltMax : g;  // (a sum below f32's range: silu is 0 there, not inf / inf)
             float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[pair] : 0.0f;
             __bf16 *const dst = w.h + (size_t)pair * 3 * frow + r0 + r;
             for (int j = 0; j < hterms; j++) {

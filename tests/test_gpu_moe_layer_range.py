@@ -91,3 +91,17 @@ def test_largest_x(hip, t, embd, ff, ky):
     tokens(p, x)
     p.upload()
     check(p)
+
+
+def test_x_that_overflows_the_sums(hip):
+    """Sums beyond f32's range, of one large term each: the clamp holds them; silu of such a
+    sum below 0 is 0."""
+    p = Layer(hip, t=5, embd=320, ff=64, clamp=10.0)
+    for name in ("gate", "up"):
+        scales(p, name, 128, 130)
+    x = p.x.copy()
+    for i in range(5):
+        x[i, 7] = TOP[i]
+    tokens(p, x)
+    p.upload()
+    check(p)
