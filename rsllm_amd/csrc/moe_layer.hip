@@ -95,7 +95,7 @@ size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_sha
     return at;
 }
 
-constexpr float kFltMax = 0x1.fffffep127f;
+constexpr float kFltMax = 0x1.fffffep127f, kBf16Max = 0x1.fep127f;
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 // The first eight significant bits of v, cut off and not rounded: rounded, what lies above
 // bf16's largest number would be an infinity.
@@ -696,7 +696,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
             float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[pair] : 0.0f;
             __bf16 *const dst = w.h + (size_t)pair * 3 * frow + r0 + r;
             for (int j = 0; j < hterms; j++) {
-                const __bf16 b16 = (__bf16)h;
+                // (an infinity stays one; a number has no term that is rounded to one)
+                const __bf16 b16 = (__bf16)(finite(h) ? fminf(fmaxf(h, -kBf16Max), kBf16Max) : h);
                 dst[j * frow] = b16;
                 h = finite(h) ? h - (float)b16 : 0.0f;
                 if (r0 + 16 >= ff)  // zeros up to whole steps

@@ -105,3 +105,25 @@ def test_x_that_overflows_the_sums(hip):
     tokens(p, x)
     p.upload()
     check(p)
+
+
+@pytest.mark.parametrize("t", [1, 3, 9])
+@pytest.mark.parametrize("ky", ["f32", "bf16"])
+def test_largest_h(hip, t, ky):
+    """h between bf16's largest number and f32's: finite outputs where the down weights are small."""
+    p = Layer(hip, t=t, embd=64, ff=128, experts=2, k=1, ky=ky)
+    for name, s in (("gate", 127 + 64), ("up", 127 + 63)):
+        codes, sc = p.m[name]
+        codes[:], sc[:] = 0, 127
+        # element 0 alone, 1 2^64 and +-1 2^63: h = +-x0^2 2^127
+        codes[:, 0] = 2
+        sc[:, 0] = s
+    p.m["up"][0][::3, 0] = 10
+    scales(p, "down", 100, 104)
+    x = p.x.copy()
+    x[:, 0] = np.sqrt(np.linspace(1.9975, 1.9999, t))
+    tokens(p, x)
+    p.upload()
+    h = p.x[:, 0] ** 2 * 2.0 ** 127
+    assert (h > NO_BF16).all() and (h < FLT_MAX).all()
+    check(p)
