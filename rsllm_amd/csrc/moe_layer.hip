@@ -4,7 +4,9 @@
 // The weights' codes are widened to bf16 (exactly: a code has two significant bits, a
 // scale none), x and h are sums of bf16 terms: one for bf16 x, two for f16, three for
 // f32 (8 significant bits each, so 24), so that the products on the matrix cores are
-// exact and the sums f32. A term of a token is a column of the 16-wide products.
+// exact and the sums f32. A term of a token is a column of the 16-wide products. The second
+// and third terms are held times 2^7 and 2^15, and their columns' sums divided by it: bf16 has
+// nothing below 2^-133, where the low bits of small numbers lie.
 //
 // The chosen experts' weights are read once and bound everything: 98 MB for one token of a
 // 4096-wide layer with n_ff 2048, 6 of 256 experts and a shared one, 1.83 GB for 32 (137
@@ -96,6 +98,11 @@ size_t moe_parts(int n_tok, int n_embd, int n_ff, int n_expert, int k, int n_sha
 }
 
 constexpr float kFltMax = 0x1.fffffep127f, kBf16Max = 0x1.fep127f;
+// What a sum of term j's is multiplied by. (2^7 and 2^15, not 2^8 and 2^16: a held term is
+// then no larger than the first one, so no sum overflows before its number does.)
+__device__ __forceinline__ constexpr float moe_unit_of(int j) { return j == 0 ? 1.0f : j == 1 ? 0x1p-7f : 0x1p-15f; }
+// From what is left behind term j to the next one.
+__device__ __forceinline__ constexpr float moe_next(int j) { return j == 0 ? 0x1p7f : 0x1p8f; }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 // The first eight significant bits of v, cut off and not rounded: rounded, what lies above
 // bf16's largest number would be an infinity.
@@ -198,7 +205,7 @@ __global__ __launch_bounds__(64 * kInWaves) void k_moe_in(MoeLayerArgs a, MoeWor
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 b[k] = moe_cut(v[k]);
-                v[k] -= (float)b[k];
+                v[k] = (v[k] - (float)b[k]) * moe_next(j);
             }
             *reinterpret_cast<mx_bf8 *>(dst + j * row + i) = b;
         }
@@ -684,8 +691,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
             for (int y = 0; y < kw; y++) {
 #pragma unroll
                 for (int j = 0; j < TERMS; j++) {
-                    g += src[(y * 2 * 64 + j) * 4];
-                    v += src[((y * 2 + 1) * 64 + j) * 4];
+                    g = fmaf(src[(y * 2 * 64 + j) * 4], moe_unit_of(j), g);
+                    v = fmaf(src[((y * 2 + 1) * 64 + j) * 4], moe_unit_of(j), v);
                 }
             }
             if (a.clamp > 1e-6f) {
@@ -699,7 +706,7 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
                 // (an infinity stays one; a number has no term that is rounded to one)
                 const __bf16 b16 = (__bf16)(finite(h) ? fminf(fmaxf(h, -kBf16Max), kBf16Max) : h);
                 dst[j * frow] = b16;
-                h = finite(h) ? h - (float)b16 : 0.0f;
+                h = finite(h) ? (h - (float)b16) * moe_next(j) : 0.0f;
                 if (r0 + 16 >= ff)  // zeros up to whole steps
                     for (int z = 16; r0 + r + z < frow; z += 16) dst[j * frow + z] = (__bf16)0.0f;
             }
@@ -842,8 +849,8 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
             mx_v4f y = acc[0];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                y[i] += moe_lane_after<1>(acc[0][i]);
-                if (TERMS == 3) y[i] += moe_lane_after<2>(acc[0][i]);
+                y[i] = fmaf(moe_lane_after<1>(acc[0][i]), moe_unit_of(1), y[i]);
+                if (TERMS == 3) y[i] = fmaf(moe_lane_after<2>(acc[0][i]), moe_unit_of(2), y[i]);
             }
             if (tok >= 0 && r % TERMS == 0) *reinterpret_cast<mx_v4f *>(own + tok * 16 + 4 * q) += y;
             acc[0] = mx_v4f{0.0f, 0.0f, 0.0f, 0.0f};

@@ -28,6 +28,9 @@ def moe(p):
     y, err = np.zeros(p.x.shape), np.zeros(p.x.shape)
     d, f, top = c["embd"], c["ff"], c["clamp"] if c["clamp"] > 1e-6 else np.inf
     cut = 2.0 ** -24 if c["ky"] == "f32" else 2.0 ** -16
+    # Small h: two roundings to f32, 2^-150 each, and half a step of the last term, bf16's 2^-133
+    # over 2^15 of three terms (2^-149), over 2^7 of two (2^-141)
+    least = 2.0 ** -148 if c["ky"] == "f32" else 2.0 ** -140
     for t, x in enumerate(p.x):
         slots = [(e, w) for e, w in zip(ids[t], weights[t]) if e >= 0 and np.float32(w) != 0]
         slots += [(c["experts"] + j, 1.0) for j in range(c["shared"])]
@@ -44,7 +47,7 @@ def moe(p):
             h = s * u
             eh = es * (np.abs(u) + eu) + np.abs(s) * eu + np.abs(h) * (2.0 ** -20 + cut)
             y[t] += w * (down[e] @ h)
-            err[t] += w * (np.abs(down[e]) @ eh)
+            err[t] += w * (np.abs(down[e]) @ eh) + least * np.abs(down[e]).sum(1)
             total += w * (np.abs(down[e]) @ np.abs(h))
         err[t] += (len(slots) * f / 32 + 40) * 2.0 ** -23 * total
     return ids, weights, y, err + M.rounding(y, c["ky"])
@@ -126,4 +129,28 @@ def test_largest_h(hip, t, ky):
     p.upload()
     h = p.x[:, 0] ** 2 * 2.0 ** 127
     assert (h > NO_BF16).all() and (h < FLT_MAX).all()
+    check(p)
+
+
+#: exponent of x, scales of gate and up, of down
+ENDS = {
+    "tiny x, large weights": (-126, (250, 252), (116, 120)),
+    "large x, the smallest weights": (118, (0, 4), (116, 120)),
+    "tiny h, large weights": (0, (58, 60), (248, 252)),
+    "large h, the smallest weights": (0, (170, 172), (0, 4)),
+}
+
+
+@pytest.mark.parametrize("name", ENDS)
+@pytest.mark.parametrize("kx,ky", [("f32", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("t,embd,ff", [(1, 256, 128), (9, 300, 200), (3, 4500, 48), (2, 8300, 40), (4, 64, 1100)])
+def test_scales_of_every_size(hip, name, kx, ky, t, embd, ff):
+    """Weights of every scale against x or h that bring the sums back to ordinary sizes."""
+    power, gate_up, down = ENDS[name]
+    p = Layer(hip, t=t, embd=embd, ff=ff, kx=kx, ky=ky, experts=4, shared=1)
+    scales(p, "gate", *gate_up)
+    scales(p, "up", *gate_up, seed=2)
+    scales(p, "down", *down, seed=3)
+    tokens(p, p.x * 2.0 ** power)
+    p.upload()
     check(p)
