@@ -615,8 +615,8 @@ int rsllm_hip_matmul_mxfp4_dev(void *out, size_t out_len, size_t out_stride,
  * the second sum over the n_shared experts that every token takes, which stand behind
  * the others in the weights. Experts of weight 0 are skipped. x and h are not
  * quantised: the products take x exactly (f32 x below 2^-125: to 2^-149), and h rounded
- * to 24 bits (f32 outputs) or 16 (f16 and bf16 ones), and sum in f32: a sum of which a part
- * leaves f32's range is infinite or NaN. A token with a non-finite value in x gets a row
+ * to 24 bits (f32 outputs) or 16 (f16 and bf16 ones), and sum in f32; a sum that comes out
+ * infinite or NaN is made again in 64 bits. A token with a non-finite value in x gets a row
  * of NaN (its ids and weights by the rules above, whatever its logits became).
  * The layer: `router` [n_expert x n_embd] of dtype_router (F32, F16 or BF16; router_len
  * elements), `bias` n_expert values or NULL (bias_len 0); gate, up: (n_expert +

@@ -593,6 +593,28 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
     for (int i = 0; i < n; i++) mask &= mask - 1;
     return mask ? __ffs((int)mask) - 1 : -1;
 }
+// A row of weights times a row of terms (`pitch` elements from one term to the next, zeros behind
+// its end) in 64 bits: for the rare sum that came out infinite or NaN. That happens where f32 is
+// left on the way, and where codes of scales 253 and 254, which no quantiser makes, passed bf16's
+// range. One lane's work.
+template <int TERMS>
+__device__ __forceinline__ double moe_again(const uint8_t *codes, const uint8_t *scales, const __bf16 *terms, int pitch, int n) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 2) {
+        const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)codes[i / 2], 1.0f, 0);
+        const uint32_t s = scales[i / 32];
+        double x0 = 0.0, x1 = 0.0;
+#pragma unroll
+        for (int j = 0; j < TERMS; j++) {
+            x0 += (double)(float)terms[j * pitch + i] * moe_unit_of(j);
+            x1 += (double)(float)terms[j * pitch + i + 1] * moe_unit_of(j);
+        }
+        const double part = fma((double)c[0], x0, (double)c[1] * x1);
+        sum += s == 255u ? __builtin_nan("") : part * __builtin_bit_cast(double, (uint64_t)(s + 1023u - 127u) << 52);
+    }
+    return sum;
+}
 // The pairs (token, slot) of every job, CAP a job, 0xFFFF behind its last token.
 template <int W, int CAP> __device__ __forceinline__ void moe_pairs(const MoeLayerArgs &a, const MoePlan &plan, uint16_t *pairs) {
     const int slots = a.k + a.n_shared;
@@ -673,6 +695,26 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
 #pragma unroll
     for (int b = 0; b < NB; b++) fetch(p[b], b);
     moe_pairs<W, TPT>(a, plan, pairs);  // (for finish(), behind its barrier)
+    __shared__ int again;  // whether a sum is to be made again, which h of NaN marks
+    if (tid == 0) again = 0;
+    // h of a pair's row r0 + r, from its sums
+    auto put = [&](float g, float v, int pair, int r0) __attribute__((always_inline)) {
+        if (a.clamp > 1e-6f) {
+            g = g > a.clamp ? a.clamp : g;
+            v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
+        }
+        g = g < -kFltMax ? -kFltMax : g;  // (a sum below f32's range: silu is 0 there, not inf / inf)
+        float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[pair] : 0.0f;
+        __bf16 *const dst = w.h + (size_t)pair * 3 * frow + r0 + r;
+        for (int j = 0; j < hterms; j++) {
+            // (an infinity stays one; a number has no term that is rounded to one)
+            const __bf16 b16 = (__bf16)(finite(h) ? fminf(fmaxf(h, -kBf16Max), kBf16Max) : h);
+            dst[j * frow] = b16;
+            h = finite(h) ? (h - (float)b16) * moe_next(j) : 0.0f;
+            if (r0 + 16 >= ff)  // zeros up to whole steps
+                for (int z = 16; r0 + r + z < frow; z += 16) dst[j * frow + z] = (__bf16)0.0f;
+        }
+    };
     int held = 0;  // rounds whose sums are in LDS
     // The last `held` rounds up to b0 + held: a token of one of them for every 16 lanes (rows).
     // (LDS alone is waited for, not the weights on their way.)
@@ -695,21 +737,11 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
                     v = fmaf(src[((y * 2 + 1) * 64 + j) * 4], moe_unit_of(j), v);
                 }
             }
-            if (a.clamp > 1e-6f) {
-                g = g > a.clamp ? a.clamp : g;
-                v = v > a.clamp ? a.clamp : v < -a.clamp ? -a.clamp : v;
+            if (!(finite(g) && finite(v))) {
+                g = __builtin_nanf("");
+                if (!w.bad[pair / slots]) again = 1;
             }
-            g = g < -kFltMax ? -kFltMax : g;  // (a sum below f32's range: silu is 0 there, not inf / inf)
-            float h = r0 + r < ff ? g / (1.0f + expf(-g)) * v * plan.weight[pair] : 0.0f;
-            __bf16 *const dst = w.h + (size_t)pair * 3 * frow + r0 + r;
-            for (int j = 0; j < hterms; j++) {
-                // (an infinity stays one; a number has no term that is rounded to one)
-                const __bf16 b16 = (__bf16)(finite(h) ? fminf(fmaxf(h, -kBf16Max), kBf16Max) : h);
-                dst[j * frow] = b16;
-                h = finite(h) ? (h - (float)b16) * moe_next(j) : 0.0f;
-                if (r0 + 16 >= ff)  // zeros up to whole steps
-                    for (int z = 16; r0 + r + z < frow; z += 16) dst[j * frow + z] = (__bf16)0.0f;
-            }
+            put(g, v, pair, r0);
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         held = 0;
@@ -752,6 +784,23 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
         }
         const int end = min(total, m + NB);
         if (held + (XP == 1 ? NB : 1) > kBatch || end == total) finish(end / np - held);
+    }
+    __syncthreads();
+    if (__builtin_expect(!again, 1)) return;
+    const int first = (int)((long long)turns * (int)blockIdx.x * groups / streams);
+    const int last = (int)((long long)turns * ((int)blockIdx.x + 1) * groups / streams);
+    for (int turn = first + wv; turn < last; turn += W) {  // (this workgroup's own h)
+        const int job = turn / per, r0 = turn % per * 16;
+        for (int c0 = q; c0 < TPT; c0 += 4) {
+            const int pair = pairs[job * TPT + c0];
+            if (pair == 0xFFFF || w.bad[pair / slots] || r0 + r >= ff) continue;
+            const float h = (float)w.h[(size_t)pair * 3 * frow + r0 + r];
+            if (h == h) continue;
+            const size_t row = (size_t)plan.job[job] * ff + r0 + r;
+            const __bf16 *const terms = w.x + (size_t)(pair / slots) * 3 * erow;
+            put((float)moe_again<TERMS>(a.gate + row * rb, a.gate_s + row * sb, terms, erow, a.n_embd),
+                (float)moe_again<TERMS>(a.up + row * rb, a.up_s + row * sb, terms, erow, a.n_embd), pair, r0);
+        }
     }
 }
 
@@ -888,6 +937,15 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
 #pragma unroll
             for (int v = 0; v < W; v++) y += sums[v * a.n_tok * 16 + i];
             if (o >= a.n_embd) continue;
+            if (__builtin_expect(!finite(y) && !w.bad[t], 0)) {
+                double again = 0.0;
+                for (int j = first * CAP; j < (first + n_jobs) * CAP; j++) {
+                    if (pairs[j] == 0xFFFF || pairs[j] / slots != t) continue;
+                    const size_t row = (size_t)plan.job[j / CAP] * a.n_embd + o;
+                    again += moe_again<TERMS>(a.down + row * rb, a.down_s + row * sb, w.h + (size_t)pairs[j] * 3 * frow, frow, a.n_ff);
+                }
+                y = (float)again;
+            }
             if (parts > 1) w.part[((size_t)me * a.n_tok + t) * a.n_embd + o] = y;
             else mx_store(a.out, (size_t)t * a.out_stride + o, w.bad[t] ? __builtin_nanf("") : y, a.dtype_out);
         }

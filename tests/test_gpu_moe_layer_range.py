@@ -1,5 +1,5 @@
-"""The 4-bit mixture-of-experts layer at the ends of its types' ranges, against its definition
-in 64 bits."""
+"""The 4-bit mixture-of-experts layer at the ends of its types' ranges: the largest and the
+smallest numbers in x and in h, weights of every scale, against its definition in 64 bits."""
 import numpy as np
 import pytest
 
@@ -135,8 +135,10 @@ def test_largest_h(hip, t, ky):
 #: exponent of x, scales of gate and up, of down
 ENDS = {
     "tiny x, large weights": (-126, (250, 252), (116, 120)),
+    "tiny x, the largest weights": (-127, (250, 254), (116, 120)),
     "large x, the smallest weights": (118, (0, 4), (116, 120)),
     "tiny h, large weights": (0, (58, 60), (248, 252)),
+    "tiny h, the largest weights": (0, (58, 61), (250, 254)),
     "large h, the smallest weights": (0, (170, 172), (0, 4)),
 }
 
@@ -154,3 +156,62 @@ def test_scales_of_every_size(hip, name, kx, ky, t, embd, ff):
     tokens(p, p.x * 2.0 ** power)
     p.upload()
     check(p)
+
+
+@pytest.mark.parametrize("t", [1, 6])
+def test_largest_weights_and_f16_x(hip, t):
+    """f16 x has no small numbers to bring such sums back: the clamp does."""
+    p = Layer(hip, t=t, embd=200, ff=72, kx="f16", ky="f16", clamp=5.0)
+    scales(p, "gate", 240, 254)
+    scales(p, "up", 240, 254, seed=2)
+    x = np.zeros_like(p.x)
+    x[:, 5::64] = p.x[:, 5::64] * 2.0 ** -12
+    tokens(p, x)
+    p.upload()
+    check(p)
+
+
+@pytest.mark.parametrize("t,embd,ff", [(1, 256, 96), (7, 300, 130), (3, 4200, 40), (2, 8300, 33)])
+@pytest.mark.parametrize("kx", ["f32", "bf16"])
+def test_sums_that_leave_f32_on_the_way(hip, t, embd, ff, kx):
+    """Terms of both signs beyond f32's range: what the clamp makes of their sum is finite."""
+    p = Layer(hip, t=t, embd=embd, ff=ff, kx=kx, clamp=6.0, shared=1)
+    for name in ("gate", "up"):
+        scales(p, name, 126, 130, seed=ff)
+    tokens(p, p.x * 5e37)
+    p.upload()
+    check(p)
+
+
+@pytest.mark.parametrize("t,embd", [(1, 64), (9, 4400)])
+def test_down_sums_that_leave_f32_on_the_way(hip, t, embd):
+    """Two terms of h beyond f32's range that cancel; in parts (few rows) and whole."""
+    p = Layer(hip, t=t, embd=embd, ff=1024, experts=2, k=1, ky="f32", clamp=8.0)
+    for name in ("gate", "up"):  # rows 0 and 700 of every expert are the same: so is their h
+        for a in p.m[name]:
+            a.reshape(2, 1024, -1)[:, 700] = a.reshape(2, 1024, -1)[:, 0]
+    codes, sc = p.m["down"]
+    sc[:, 0], sc[:, 700 // 32] = 252, 252
+    codes[:, 0], codes[:, 700 // 2] = 7, 15  # 6 and -6 2^125; nothing else in these bytes
+    codes[:, 1:16], codes[:, 336:350], codes[:, 351:352] = 0, 0, 0
+    x = p.x * 2.0 ** 20
+    tokens(p, x)
+    p.upload()
+    _, _, want, _ = moe(p)
+    p.run()
+    got = p.out.cpu().double().numpy()
+    # 1024 additions in 64 bits beside terms of 64 x 6 x 2^125
+    assert (np.abs(got - want) <= 1024 * 2.0 ** -53 * 64 * 6 * 2.0 ** 125).all()
+
+
+def test_nan_scales_stay_nan(hip):
+    """Scales of 255 beside the largest ones: NaN, in the tokens that took that expert alone."""
+    p = Layer(hip, t=6, experts=4, k=1, clamp=5.0)
+    for name in ("gate", "up"):
+        scales(p, name, 253, 254)
+    p.m["gate"][1][2 * 128 + 5, 3] = 255
+    tokens(p, p.x * 2.0 ** -127)
+    p.upload()
+    p.run()
+    took = (p.ids.cpu().numpy() == 2).any(1)
+    assert np.array_equal(np.isnan(p.out.cpu().numpy()).all(1), took)
