@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict
         const size_t at = row * stride + 8 * g;
         if (vec && 8 * g + 8 <= in_dim) {
             const mx_v4f lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
-            const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 zero = make_float4(-0.0f, -0.0f, -0.0f, -0.0f);  // (-0 + -0 is -0, and +0 + -0 is +0)
             if constexpr (DT == T_F32) {
                 float4 *const d = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
                 d[0] = make_float4(v[0], v[1], v[2], v[3]);
