@@ -653,6 +653,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int slots = a.k + a.n_shared, ff = a.n_ff, frow = pad128(ff), erow = pad128(a.n_embd);
+    __shared__ int again;  // whether a sum is to be made again, which h of NaN marks
+    if (tid == 0) again = 0;
     moe_plan<W>(a, w, plan, TPT, reinterpret_cast<double *>(smem), choose);
     const size_t rb = mx_row_bytes(a.n_embd), sb = mx_scale_bytes(a.n_embd);
     const int steps = (int)(rb / 64), pieces = (int)(sb / 16), blocks = (a.n_embd + 31) / 32;
@@ -695,8 +697,6 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
 #pragma unroll
     for (int b = 0; b < NB; b++) fetch(p[b], b);
     moe_pairs<W, TPT>(a, plan, pairs);  // (for finish(), behind its barrier)
-    __shared__ int again;  // whether a sum is to be made again, which h of NaN marks
-    if (tid == 0) again = 0;
     // h of a pair's row r0 + r, from its sums
     auto put = [&](float g, float v, int pair, int r0) __attribute__((always_inline)) {
         if (a.clamp > 1e-6f) {
@@ -785,8 +785,8 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
         const int end = min(total, m + NB);
         if (held + (XP == 1 ? NB : 1) > kBatch || end == total) finish(end / np - held);
     }
-    __syncthreads();
-    if (__builtin_expect(!again, 1)) return;
+    if (__builtin_expect(!again, 1)) return;  // (everyone's: finish() ends with a barrier)
+    __syncthreads();                          // (h has been written)
     const int first = (int)((long long)turns * (int)blockIdx.x * groups / streams);
     const int last = (int)((long long)turns * ((int)blockIdx.x + 1) * groups / streams);
     for (int turn = first + wv; turn < last; turn += W) {  // (this workgroup's own h)
@@ -932,12 +932,12 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
         }
         __syncthreads();
         for (int i = tid; i < a.n_tok * 16; i += 64 * W) {
-            const int t = i >> 4, o = r0 + (i & 15);
+            const int t = i >> 4, o = r0 + (i & 15), bad = w.bad[t];
             float y = 0.0f;
 #pragma unroll
             for (int v = 0; v < W; v++) y += sums[v * a.n_tok * 16 + i];
             if (o >= a.n_embd) continue;
-            if (__builtin_expect(!finite(y) && !w.bad[t], 0)) {
+            if (__builtin_expect(!finite(y) && !bad, 0)) {
                 double again = 0.0;
                 for (int j = first * CAP; j < (first + n_jobs) * CAP; j++) {
                     if (pairs[j] == 0xFFFF || pairs[j] / slots != t) continue;
@@ -947,7 +947,7 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
                 y = (float)again;
             }
             if (parts > 1) w.part[((size_t)me * a.n_tok + t) * a.n_embd + o] = y;
-            else mx_store(a.out, (size_t)t * a.out_stride + o, w.bad[t] ? __builtin_nanf("") : y, a.dtype_out);
+            else mx_store(a.out, (size_t)t * a.out_stride + o, bad ? __builtin_nanf("") : y, a.dtype_out);
         }
     }
 }
