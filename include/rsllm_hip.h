@@ -570,7 +570,8 @@ int rsllm_hip_matmul_int8_dev(void *out, size_t out_len, size_t out_stride, cons
  * overlap what its call reads.
  * `work`: rsllm_hip_mxfp4_work_bytes(n_tok, in_dim, out_dim) bytes of the caller's (0
  * for sizes that are refused), 256-byte aligned, used by this call alone until it has run:
- * calls that may overlap, and graphs that may replay at once, get one each.
+ * calls that may overlap, and graphs that may replay at once, get one each. (The prequant
+ * form asks for it too, and so far does not write to it.)
  * Errors: UNIMPLEMENTED for another dtype; INVALID_ARGUMENT for in_dim 0 or above
  * 1048576, out_dim 0, NULL or misaligned pointers; SHAPE_MISMATCH for n_rows, n_tok or
  * out_dim above 8388607 (what a launch holds), a stride below its row, x_len or out_len
@@ -615,8 +616,8 @@ int rsllm_hip_matmul_mxfp4_dev(void *out, size_t out_len, size_t out_stride,
  * the second sum over the n_shared experts that every token takes, which stand behind
  * the others in the weights. Experts of weight 0 are skipped. x and h are not
  * quantised: the products take x exactly (f32 x below 2^-125: to 2^-149), and h rounded
- * to 24 bits (f32 outputs) or 16 (f16 and bf16 ones), and sum in f32; a sum that comes out
- * infinite or NaN is made again in 64 bits. A token with a non-finite value in x gets a row
+ * to 24 bits (f32 outputs) or 16 (f16 and bf16 ones), and sum in f32; a row's sum that comes
+ * out infinite or NaN is made again in 64 bits and rounded to f32. A token with a non-finite value in x gets a row
  * of NaN (its ids and weights by the rules above, whatever its logits became).
  * The layer: `router` [n_expert x n_embd] of dtype_router (F32, F16 or BF16; router_len
  * elements), `bias` n_expert values or NULL (bias_len 0); gate, up: (n_expert +

@@ -2,18 +2,22 @@
 // gate and up products, SwiGLU, down product, weighted sum.
 //
 // The weights' codes are widened to bf16 (exactly: a code has two significant bits, a
-// scale none), x and h are sums of bf16 terms: one for bf16 x, two for f16, three for
-// f32 (8 significant bits each, so 24), so that the products on the matrix cores are
-// exact and the sums f32. A term of a token is a column of the 16-wide products. The second
-// and third terms are held times 2^7 and 2^15, and their columns' sums divided by it: bf16 has
-// nothing below 2^-133, where the low bits of small numbers lie.
+// scale none; codes of scales 253 and 254 can be infinite there, which moe_again mends), x and
+// h are sums of bf16 terms: one for bf16 x, two for f16, three for f32 (8 significant bits
+// each, so 24), so that the products on the matrix cores are exact and the sums f32. A term of
+// a token is a column of the 16-wide products. The second and third terms are held times 2^7
+// and 2^15, and their columns' sums divided by it: bf16 has nothing below 2^-133, where the
+// low bits of small numbers lie.
 //
-// The chosen experts' weights are read once and bound everything: 98 MB for one token of a
-// 4096-wide layer with n_ff 2048, 6 of 256 experts and a shared one, 1.83 GB for 32 (137
-// experts). Three launches (four beyond 8 tokens): 41.8 us and 408 us, of which the up kernel
-// is 26.0 and 234 (63 MB and 1.2 GB: 2.4 and 5.2 TB/s), the down kernel 13.4 and 145 (31 and
-// 610 MB: 2.3 and 4.2 TB/s), the router 4.9 and 18. A launch that only reads gets 4.3 TB/s of
-// 31 MB and 5.7 of 400. One token's up kernel is a chain before the stream, which takes 12 us
+// The chosen experts' weights bound everything. An expert's are read once a job, which holds 16
+// / terms of its tokens in the up kernel (5 of f32 x) and three or four in the down kernel: once
+// where experts are many and tokens few, seven and eleven times for an expert that 32 tokens of
+// f32 take. (8 of 8 experts of the layer below, 32 tokens, take 212 us for 107 MB, 8 of 64 294 for
+// 843.) 98 MB for one token of a 4096-wide layer with n_ff 2048, 6 of 256 experts and a shared
+// one, 1.83 GB for 32 (137 experts). Three launches (four beyond 8 tokens): 42.7 us and 408 us,
+// of which the up kernel is 25.5 and 235 (63 MB and 1.2 GB: 2.5 and 5.2 TB/s), the down kernel
+// 13.6 and 146 (31 and 610 MB: 2.3 and 4.2 TB/s), the router 4.9 and 18. A launch that only reads
+// gets 4.3 TB/s of 31 MB and 5.7 of 400. One token's up kernel is a chain before the stream, which takes 12 us
 // of it: the choice 4 us, its jobs 1, the first loads; and behind it 3 us for the last sums.
 #include "fp4_common.h"
 #include "route_scores.h"
@@ -785,6 +789,7 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
         const int end = min(total, m + NB);
         if (held + (XP == 1 ? NB : 1) > kBatch || end == total) finish(end / np - held);
     }
+    // The sums to make again: here, where nothing of the loop is live (in finish() it spills).
     if (__builtin_expect(!again, 1)) return;  // (everyone's: finish() ends with a barrier)
     __syncthreads();                          // (h has been written)
     const int first = (int)((long long)turns * (int)blockIdx.x * groups / streams);
@@ -1019,6 +1024,9 @@ template <int TERMS> hipError_t moe_up(const MoeLayerArgs &a, const MoeWork &w, 
     const int pieces = (int)mx_scale_bytes(a.n_embd) / 16;
     if (pieces > 2 * kWaves) return moe_up_go<0, TERMS>(a, w, hterms, kWaves, s);
     if (pieces > kWaves) return moe_up_go<2, TERMS>(a, w, hterms, kWaves, s);
+    // (Wavefronts idle at 3, 5 to 7 and 9 to 15 pieces. 32 tokens of 6 of 256 experts and a shared
+    // one, n_ff 2048, bytes of weights over the layer's time: 3.4 TB/s 2048 wide, 3.1 at 2560, 4.0
+    // at 4096, 3.1 and 3.3 at 4608 and 5120, 4.0 at 7168.)
     const int kw = pieces > 4 ? 8 : pieces > 2 ? 4 : pieces;
     return moe_up_go<1, TERMS>(a, w, hterms, kw, s);
 }
@@ -1041,6 +1049,10 @@ hipError_t launch_moe_layer(const MoeLayerArgs &a, uint8_t *work, hipStream_t s)
     if (a.n_tok <= 0) return hipSuccess;
     MoeWork w;
     moe_parts(a.n_tok, a.n_embd, a.n_ff, a.n_expert, a.k, a.n_shared, work, &w);
+    // h as 16 bits where the output has 8 or 11: an output then differs by a rounding now and then
+    // (bf16, 7168 / 2048, 8 of 64 experts, 8 tokens: 0.29% of the elements, 0.06% with 24 bits), the
+    // error against 64 bits is the same to four digits. 24 bits take 236 in place of 229 us there,
+    // 417 in place of 397 for 32 tokens of 4096 / 2048.
     const int hterms = a.dtype_out == T_F32 ? 3 : 2;
     if (a.dtype_x == T_F32) moe_in_go<T_F32>(a, w, s);
     else if (a.dtype_x == T_F16) moe_in_go<T_F16>(a, w, s);

@@ -139,8 +139,8 @@ namespace {
 // of a row for each step of 128 and the 16 scale bytes of its row for the piece's four
 // steps; the operands of the next piece are on their way while this one is multiplied. The
 // weights' bytes bound it, for small ones the latency of a launch, one piece a wavefront and
-// the sums' join: 14336 x 4096, one token, 31 MB, 8.8 us from memory (a launch that only
-// reads them 7.5); 4096 x 4096, 32 tokens, 6.5; 1001 x 2000, 77 tokens, 4.6. K is split over
+// the sums' join: 14336 x 4096, one token, 31 MB, 9.6 to 10.7 us in traces' medians, 10.0 a
+// call in a graph (a launch that only reads them 7.5); 4096 x 4096, 32 tokens, 6.5; 1001 x 2000, 77 tokens, 4.6. K is split over
 // the wavefronts since few channels a workgroup fill the chip (4096 channels: 256 or 128
 // workgroups), and since a lane that streams rows into registers needs no LDS and no barrier.
 template <int MF_, int NF_, int WK_> struct MxFew {
@@ -505,8 +505,12 @@ namespace {
 //   us = c0 + r c1 + (L c2 + r c3) slices
 // with L workgroups a CU, r of them one after the other (`occ` run at once) and `slices`
 // pieces of `unit` codes a wavefront, fitted to 150 sizes (1 to 2048 tokens, weights from
-// memory). Slower than the fastest of sixteen kernels: 3% on average and 29% at most at
-// those sizes (64 x 64's constants by nine of them, later). From 129 tokens on the tiles
+// memory; 64 x 64's constants by nine of them, later). At 200 other sizes the kernel it takes is
+// slower than the fastest of the twelve by 5.5% on average up to 32 tokens (60 sizes; 49% at
+// most: 4.9 in place of 3.3 us for 6 of 226 x 426), 3.6% from 33 to 300 (80; 66%: 26.2 in place of
+// 15.8 us for 83 of 6656 x 6848), and 0.0% beyond (60; 0.8%). One or two float tokens, which the
+// product quantises, are estimated alike: 2.4% on average at 38 sizes, 13.5% at most. From 129
+// tokens on the tiles
 // without LDS, which read the tokens' codes for every 16 or 32 channels, lose and are not
 // looked at: 14.6 us at best in place of 10.5 for 129 tokens of 4096 x 4096, 58 in place of
 // 19 for 200 of 14336 x 4096.

@@ -55,7 +55,8 @@ template <int U> __device__ __forceinline__ void mx_mfma_acc(mx_v4f &acc, const 
 // A copy in two parts with a product between them (which stands in for the wait state
 // that M0 needs): where in LDS, then 16 bytes a lane from voff of the buffer there.
 // M0 is not restored: nothing else in this file uses it (LDS needs none, and the compiler
-// sets it before each use of its own).
+// sets it before each use of its own; it takes no declaration of it as overwritten). Between
+// the two parts nothing may be added that needs it.
 __device__ __forceinline__ void mx_dma_to(uint32_t lds, int at) {
     asm volatile("s_add_u32 m0, %0, %1" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "s"(at) : "memory", "scc");
 }
