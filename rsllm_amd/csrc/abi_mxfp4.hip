@@ -77,6 +77,15 @@ bool layer_sizes_ok(const rsllm_hip_moe_mxfp4 &l) {
     return l.n_embd >= 1 && l.n_embd <= 65536 && l.n_ff >= 1 && l.n_ff <= 65536 && l.n_expert >= 1 &&
            l.n_expert <= 1024 && l.n_shared <= 8 && l.k >= 1 && l.k <= 32;
 }
+// What is wrong with its groups and k (of sizes that are right), or null.
+const char *groups_refused(const rsllm_hip_moe_mxfp4 &l) {
+    if (l.n_group == 0 || l.n_expert % l.n_group != 0) return "moe_mxfp4: n_group must divide n_expert";
+    if (l.topk_group == 0 || l.topk_group > l.n_group) return "moe_mxfp4: topk_group must be 1..n_group";
+    if (l.group_top != 1 && l.group_top != 2) return "moe_mxfp4: group_top must be 1 or 2";
+    if (l.k > l.topk_group * (l.n_expert / l.n_group))
+        return "moe_mxfp4: k must be at most the experts of topk_group groups";
+    return nullptr;
+}
 int check_layer(const rsllm_hip_moe_mxfp4 &l) {
     if (!float_type(l.dtype_router))
         return set_error(RSLLM_HIP_ERR_UNIMPLEMENTED, "moe_mxfp4: router dtype not implemented");
@@ -84,13 +93,7 @@ int check_layer(const rsllm_hip_moe_mxfp4 &l) {
     if (!layer_sizes_ok(l))
         return invalid("moe_mxfp4: n_embd and n_ff must be 1..65536, n_expert 1..1024, n_shared at "
                        "most 8, k 1..32");
-    if (l.n_group == 0 || l.n_expert % l.n_group != 0)
-        return invalid("moe_mxfp4: n_group must divide n_expert");
-    if (l.topk_group == 0 || l.topk_group > l.n_group)
-        return invalid("moe_mxfp4: topk_group must be 1..n_group");
-    if (l.group_top != 1 && l.group_top != 2) return invalid("moe_mxfp4: group_top must be 1 or 2");
-    if (l.k > l.topk_group * (l.n_expert / l.n_group))
-        return invalid("moe_mxfp4: k must be at most the experts of topk_group groups");
+    if (const char *why = groups_refused(l)) return invalid(why);
     if (!std::isfinite(l.scale)) return invalid("moe_mxfp4: scale must be finite");
     if (std::isnan(l.clamp)) return invalid("moe_mxfp4: clamp must be a number");
     if (!product_is(l.n_expert, l.n_embd, l.router_len))
@@ -216,6 +219,7 @@ int rsllm_hip_matmul_mxfp4_dev(void *out, size_t out_len, size_t out_stride,
 
 size_t rsllm_hip_moe_mxfp4_work_bytes(const rsllm_hip_moe_mxfp4 *layer, size_t n_tok) {
     if (!layer || n_tok > (size_t)kMoeMaxTok || !layer_sizes_ok(*layer)) return 0;
+    if (groups_refused(*layer)) return 0;
     return moe_layer_work_bytes((int)n_tok, (int)layer->n_embd, (int)layer->n_ff, (int)layer->n_expert,
                                 (int)layer->k, (int)layer->n_shared);
 }
