@@ -600,22 +600,32 @@ __device__ __forceinline__ int moe_token(uint32_t mask, int n) {
 // A row of weights times a row of terms (`pitch` elements from one term to the next, zeros behind
 // its end) in 64 bits: for the rare sum that came out infinite or NaN. That happens where f32 is
 // left on the way, and where codes of scales 253 and 254, which no quantiser makes, passed bf16's
-// range. One lane's work.
+// range. One lane's work, eight elements at a time; a NaN scale ends it. (With an expert of NaN
+// weights that three of 32 tokens take, the 4096-wide layer takes 0.65 in place of 0.41 ms.)
 template <int TERMS>
 __device__ __forceinline__ double moe_again(const uint8_t *codes, const uint8_t *scales, const __bf16 *terms, int pitch, int n) {
-    double sum = 0.0;
+    bool nan = false;
+#pragma unroll 8
+    for (int b = 0; b < (n + 31) / 32; b++) nan |= scales[b] == 255u;
+    double sum = nan ? __builtin_nan("") : 0.0;
 #pragma unroll 1
-    for (int i = 0; i < n; i += 2) {
-        const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)codes[i / 2], 1.0f, 0);
-        const uint32_t s = scales[i / 32];
-        double x0 = 0.0, x1 = 0.0;
+    for (int i = 0; i < n && sum == sum; i += 8) {  // (a NaN stays one)
+        const uint32_t c = *reinterpret_cast<const uint32_t *>(codes + i / 2);
+        mx_bf8 x[TERMS];
 #pragma unroll
-        for (int j = 0; j < TERMS; j++) {
-            x0 += (double)(float)terms[j * pitch + i] * moe_unit_of(j);
-            x1 += (double)(float)terms[j * pitch + i + 1] * moe_unit_of(j);
+        for (int j = 0; j < TERMS; j++) x[j] = *reinterpret_cast<const mx_bf8 *>(terms + j * pitch + i);
+        const auto c0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), c1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+        const auto c2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), c3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+        const float w[8] = {c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+        double part = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            double v = 0.0;
+#pragma unroll
+            for (int j = 0; j < TERMS; j++) v = fma((double)(float)x[j][k], (double)moe_unit_of(j), v);
+            part = fma((double)w[k], v, part);
         }
-        const double part = fma((double)c[0], x0, (double)c[1] * x1);
-        sum += s == 255u ? __builtin_nan("") : part * __builtin_bit_cast(double, (uint64_t)(s + 1023u - 127u) << 52);
+        sum = fma(part, __builtin_bit_cast(double, (uint64_t)(scales[i / 32] + 1023u - 127u) << 52), sum);
     }
     return sum;
 }
@@ -803,8 +813,9 @@ void k_moe_up(MoeLayerArgs a, MoeWork w, int hterms, int kw, int choose) {
             if (h == h) continue;
             const size_t row = (size_t)plan.job[job] * ff + r0 + r;
             const __bf16 *const terms = w.x + (size_t)(pair / slots) * 3 * erow;
-            put((float)moe_again<TERMS>(a.gate + row * rb, a.gate_s + row * sb, terms, erow, a.n_embd),
-                (float)moe_again<TERMS>(a.up + row * rb, a.up_s + row * sb, terms, erow, a.n_embd), pair, r0);
+            const float g = (float)moe_again<TERMS>(a.gate + row * rb, a.gate_s + row * sb, terms, erow, a.n_embd);
+            const float v = g == g ? (float)moe_again<TERMS>(a.up + row * rb, a.up_s + row * sb, terms, erow, a.n_embd) : 0.0f;
+            put(g, v, pair, r0);
         }
     }
 }
@@ -944,7 +955,7 @@ void k_moe_down(MoeLayerArgs a, MoeWork w, int parts) {
             if (o >= a.n_embd) continue;
             if (__builtin_expect(!finite(y) && !bad, 0)) {
                 double again = 0.0;
-                for (int j = first * CAP; j < (first + n_jobs) * CAP; j++) {
+                for (int j = first * CAP; j < (first + n_jobs) * CAP && again == again; j++) {
                     if (pairs[j] == 0xFFFF || pairs[j] / slots != t) continue;
                     const size_t row = (size_t)plan.job[j / CAP] * a.n_embd + o;
                     again += moe_again<TERMS>(a.down + row * rb, a.down_s + row * sb, w.h + (size_t)pairs[j] * 3 * frow, frow, a.n_ff);
