@@ -2,6 +2,7 @@
 smallest numbers in x and in h, weights of every scale, against its definition in 64 bits."""
 import numpy as np
 import pytest
+import torch
 
 import mxfp4_ref as M
 import serving_ref as R
@@ -183,7 +184,7 @@ def test_sums_that_leave_f32_on_the_way(hip, t, embd, ff, kx):
     check(p)
 
 
-@pytest.mark.parametrize("t,embd", [(1, 64), (9, 4400)])
+@pytest.mark.parametrize("t,embd", [(1, 64), (32, 64), (9, 4400)])
 def test_down_sums_that_leave_f32_on_the_way(hip, t, embd):
     """Two terms of h beyond f32's range that cancel; in parts (few rows) and whole."""
     p = Layer(hip, t=t, embd=embd, ff=1024, experts=2, k=1, ky="f32", clamp=8.0)
@@ -215,3 +216,30 @@ def test_nan_scales_stay_nan(hip):
     p.run()
     took = (p.ids.cpu().numpy() == 2).any(1)
     assert np.array_equal(np.isnan(p.out.cpu().numpy()).all(1), took)
+
+
+@pytest.mark.parametrize("t,embd,ff", [(1, 256, 96), (6, 300, 130), (32, 64, 1100), (9, 5000, 40)])
+def test_replayed_with_large_and_ordinary_x(hip, t, embd, ff):
+    """Recorded once, replayed with x that leaves f32 on the way and with x that does not, in
+    turn: every replay gives the eager run's bits, and the value."""
+    p = Layer(hip, t=t, embd=embd, ff=ff, clamp=6.0, shared=1)
+    for name in ("gate", "up"):
+        scales(p, name, 126, 130, seed=ff)
+    p.upload()
+    x = p.x.copy()
+    p.run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p.run()
+    for power in (5e37, 1.0, -5e37, 0.25):
+        tokens(p, x * power)
+        p.d["x"].copy_(p.xt.reshape(p.d["x"].shape))
+        p.out.fill_(77.0)
+        p.work.random_(0, 256)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        first = [a.clone() for a in (p.out, p.ids, p.weights)]
+        check(p)
+        assert all(torch.equal(a, b) for a, b in zip(first, (p.out, p.ids, p.weights)))
